@@ -290,6 +290,63 @@ int nanoep_stream_probe(int kind, const void* src, void* dst, int64_t dst_rows, 
  * scale the profiler's HBM byte counters.  No counterpart in the reference. */
 int nanoep_copy_bytes(const void* src, void* dst, size_t bytes, void* stream);
 
+/*
+ * The expert layer's operators around dispatch and combine.  They have no counterpart in the reference.
+ *
+ * Rows in 8 bits are records: `columns` e4m3 values (OCP, largest 448), then one fp32 scale for every 128 columns, then
+ * zeros up to a multiple of 512 bytes, so that nanoep_dispatch moves a record as a bf16 row.  A value stands for
+ * itself times its group's scale; a scale is the group's largest magnitude (at least 2^-64) over 448.  Products take the two
+ * parts of a row separately, with strides of their own.
+ */
+
+/* Bytes of a record; 0 for columns <= 0.  A host function. */
+int64_t nanoep_fp8_record_bytes(int64_t columns);
+
+/*
+ * s = x + residual (residual NULL: x), n = s / sqrt(mean(s^2) + eps) * gamma, in fp32: n in 8 bits (records
+ * [T][nanoep_fp8_record_bytes(hidden)]), s in residual_out (bf16 [T, hidden]; NULL exactly when residual is) and n in normalized
+ * (bf16 [T, hidden], may be NULL), each rounded once.  x, residual, gamma: bf16; hidden % 16 == 0, hidden <= 65536; all pointers
+ * 16-byte aligned.  A group that holds an infinity or a NaN has an infinite or NaN scale.  Outputs overlap no input.
+ */
+int nanoep_rms_norm_fp8(const void* x, const void* residual, const void* gamma, int64_t num_tokens, int hidden, float eps, void* records,
+                        void* residual_out, void* normalized, void* stream);
+
+/*
+ * Products of rows in 8 bits with every expert's weight in 8 bits: for row s of expert e
+ *   z[s][n] = sum over blocks b of 128 of scales[s][b] * weight_scales[e][n / 128][b] * sum over k in b of values[s][k] * weight[e][n][k]
+ * summed in fp32.  Expert e has the rows [expert_offsets[e], expert_offsets[e] + expert_counts[e]) (int64 [E + 1], from 0 on,
+ * and [E], as nanoep_layout writes them); the rows up to expert_offsets[e + 1], and those behind the last segment, are no
+ * expert's: their outputs are zero and their inputs are not looked at.  Both NULL: one expert, all rows.
+ * Values and scales that point outside the rows are never followed.
+ *   linear : out[s] = z[s], bf16 [rows, columns]; columns % 8 == 0
+ *   gated  : records of silu(z[s][n]) * z[s][columns / 2 + n], n < columns / 2; columns % 32 == 0; needs
+ *            nanoep_experts_gated_workspace_bytes of device scratch (may be 0)
+ * values: rows value_stride bytes apart (a multiple of 16, at least inner); scales: rows scale_stride floats apart;
+ * weight: e4m3 [E, columns, inner], contiguous; weight_scales: fp32 [E, ceil(columns / 128), ceil(inner / 128)]; inner % 16 == 0;
+ * values, weight and outputs 16-byte aligned.
+ */
+int nanoep_experts_linear(const void* values, int64_t value_stride, const float* scales, int64_t scale_stride, const void* weight,
+                          const float* weight_scales, const int64_t* expert_offsets, const int64_t* expert_counts, int64_t rows,
+                          int64_t experts, int inner, int columns, void* out, void* stream);
+size_t nanoep_experts_gated_workspace_bytes(int64_t rows, int64_t experts, int inner, int columns);
+int nanoep_experts_gated(const void* values, int64_t value_stride, const float* scales, int64_t scale_stride, const void* weight,
+                         const float* weight_scales, const int64_t* expert_offsets, const int64_t* expert_counts, int64_t rows,
+                         int64_t experts, int inner, int columns, void* records, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Combine with the gate weights applied: out[t] = bf16_rne( sum over valid k ascending of weights[t][k] * f32(y[slot[t][k]])
+ * (+ f32(bias[t])) ), for the slot table of an expanded handle; a slot outside [0, y_rows) counts as masked, and its weight is not
+ * looked at.  y: bf16 [y_rows, hidden], weights: fp32 [T, K], bias: bf16 [T, hidden] or NULL; hidden % 8 == 0, K <= 32.
+ * The gradient: grad_y[slot[t][k]] = weights[t][k] * grad[t], grad_weights[t][k] = <y[slot[t][k]], grad[t]>, 0 where masked; no two
+ * choices may name one row.  Rows that no choice names get zero: with expert_offsets (int64 [L + 1]) and expert_counts (int64
+ * [L]) only the rows that are no expert's are cleared, without (both NULL) all of them are, ahead of the gradient.
+ */
+int nanoep_combine_weighted(const void* y, int64_t y_rows, const int32_t* token_slots, const float* weights, const void* bias,
+                            int64_t num_tokens, int hidden, int num_topk, void* out, void* stream);
+int nanoep_combine_weighted_backward(const void* grad, const void* y, int64_t y_rows, const int32_t* token_slots, const float* weights,
+                                     const int64_t* expert_offsets, const int64_t* expert_counts, int64_t num_local_experts,
+                                     int64_t num_tokens, int hidden, int num_topk, void* grad_y, float* grad_weights, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -25,7 +25,11 @@ KERNEL_LIBRARY = PACKAGE / "libnanoep_hip.so"
 EXTENSION_NAME = "_nanoep_torch"
 EXTENSION_LIBRARY = PACKAGE / f"{EXTENSION_NAME}.so"
 
-KERNEL_SOURCES = ["nanoep_layout.hip", "nanoep_dispatch.hip", "nanoep_combine.hip", "nanoep_abi.hip"]
+KERNEL_SOURCES = [
+    "nanoep_layout.hip", "nanoep_dispatch.hip", "nanoep_combine.hip", "nanoep_abi.hip", "nanoep_norm.hip", "nanoep_experts.hip",
+    "nanoep_weighted.hip",
+]
+EXTENSION_SOURCES = ["nanoep_torch.cpp", "nanoep_operators.cpp"]
 
 OFFLOAD_ARCH = "gfx950"
 # Packed fp32 instructions are disabled for every HIP translation unit of this project.
@@ -88,7 +92,7 @@ def build_extension(verbose: bool = False) -> Path:
         f"-DTORCH_EXTENSION_NAME={EXTENSION_NAME}",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
         *[f"-I{path}" for path in include_dirs],
-        str(CSRC / "nanoep_torch.cpp"),
+        *[str(CSRC / name) for name in EXTENSION_SOURCES],
         "-o",
         str(EXTENSION_LIBRARY),
         f"-L{torch_lib}",

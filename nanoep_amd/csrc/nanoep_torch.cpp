@@ -33,6 +33,7 @@
 #include <vector>
 
 #include "nanoep_hip.h"
+#include "nanoep_operators_host.h"
 
 namespace py = pybind11;
 
@@ -1667,6 +1668,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, module) {
         .def("close", &nanoep::PeerRuntime::close);
     py::class_<nanoep::CompletionEvent, std::shared_ptr<nanoep::CompletionEvent>>(module, "CompletionEvent")
         .def("current_stream_wait", &nanoep::CompletionEvent::current_stream_wait);
+    nanoep::bind_operators(module);
     static nanoep::CallAhead dispatch_ahead, combine_ahead;
     nanoep::call_ahead_of(module, dispatch_ahead, "dispatch", &nanoep::call_dispatch, nanoep::g_bound_dispatch);
     nanoep::call_ahead_of(module, combine_ahead, "combine", &nanoep::call_combine, nanoep::g_bound_combine);
