@@ -328,7 +328,8 @@ int nanoep_rms_norm_fp8(const void* x, const void* residual, const void* gamma, 
 int nanoep_experts_linear(const void* values, int64_t value_stride, const float* scales, int64_t scale_stride, const void* weight,
                           const float* weight_scales, const int64_t* expert_offsets, const int64_t* expert_counts, int64_t rows,
                           int64_t experts, int inner, int columns, void* out, void* stream);
-size_t nanoep_experts_gated_workspace_bytes(int64_t rows, int64_t experts, int inner, int columns);
+size_t nanoep_experts_gated_workspace_bytes(int64_t rows, int64_t experts, int inner, int columns, int64_t value_stride,
+                                            int64_t scale_stride);
 int nanoep_experts_gated(const void* values, int64_t value_stride, const float* scales, int64_t scale_stride, const void* weight,
                          const float* weight_scales, const int64_t* expert_offsets, const int64_t* expert_counts, int64_t rows,
                          int64_t experts, int inner, int columns, void* records, void* workspace, size_t workspace_bytes, void* stream);

@@ -12,6 +12,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTile = 16;  // rows and columns of one matrix instruction's result
+constexpr int kUnitRows = 4, kUnitCols = 8;  // neighbouring tiles that one XCD works on at a time
 
 struct Product {
     const char* values;  // rows of e4m3, value_stride bytes apart
@@ -80,13 +81,13 @@ __device__ __forceinline__ RowTile find_row_tile(const Product& p, int index) {
         const uint64_t behind = __ballot(before + through > index);
         if (behind != 0) {
             const int found = __ffsll(static_cast<long long>(behind)) - 1;
-            const int64_t begin = __shfl(segment.begin, found, kWave);
-            const int64_t end = __shfl(segment.end, found, kWave);
-            const int64_t live = __shfl(segment.live, found, kWave);
-            const int64_t skipped = static_cast<int64_t>(index - before - (__shfl(through, found, kWave) - __shfl(tiles, found, kWave))) * kRows;
-            const int64_t size = end - begin - skipped, rows_live = live - skipped;
-            return {first + found, begin + skipped, static_cast<int>(rows_live < 0 ? 0 : rows_live > kRows ? kRows : rows_live),
-                    static_cast<int>(size > kRows ? kRows : size)};
+            // (row numbers fit 31 bits)
+            const int begin = __builtin_amdgcn_readlane(static_cast<int>(segment.begin), found);
+            const int end = __builtin_amdgcn_readlane(static_cast<int>(segment.end), found);
+            const int live = __builtin_amdgcn_readlane(static_cast<int>(segment.live), found);
+            const int skipped = (index - before - __builtin_amdgcn_readlane(through - tiles, found)) * kRows;
+            const int size = end - begin - skipped, rows_live = live - skipped;
+            return {first + found, begin + skipped, rows_live < 0 ? 0 : rows_live > kRows ? kRows : rows_live, size > kRows ? kRows : size};
         }
         before += __builtin_amdgcn_readlane(through, kWave - 1);
     }
@@ -250,6 +251,278 @@ __global__ void __launch_bounds__(kBlockThreads) experts_stream_kernel(const Pro
     }
 }
 
+// ------------------------------------------------------------------ many rows an expert
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)(p)));
+}
+
+// Copies 16 (kBytes == 16) or 4 bytes a lane from memory into LDS without registers on the way: lane l's go to
+// `to` + l * kBytes.  `to` and `from` are wave-uniform, `offset` is a lane's own.  Nothing waits for it but loads_landed().
+template <int kBytes>
+__device__ __forceinline__ void load_to_lds(const char* from, uint32_t offset, uint32_t to) {
+    if constexpr (kBytes == 16)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(from) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(from) : "memory");
+}
+
+// The same with a whole address of each lane's own.
+__device__ __forceinline__ void load_to_lds(const char* from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+}
+
+// What is read in the place of a piece that lies past its row's end.
+__device__ const u32x4 kZeroPiece = {0u, 0u, 0u, 0u};
+
+// Every wavefront's copies into LDS are there, and every wavefront has read what the next ones overwrite.
+__device__ __forceinline__ void loads_landed() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// The products of a tile of 16 * kRowTiles * kRowWaves rows and 16 * kColTiles * kColWaves weight rows, one workgroup.
+template <int kRowTiles, int kColTiles, int kRowWaves, int kColWaves>
+struct TileShape {
+    static constexpr int kWaves = kRowWaves * kColWaves;
+    static constexpr int kThreads = kWaves * kWave;
+    static constexpr int kRows = kTile * kRowTiles * kRowWaves;
+    static constexpr int kCols = kTile * kColTiles * kColWaves;
+    static constexpr int kStageRows = kRows + kCols;  // 128-byte rows of one stage: the weights', then the activations'
+    static constexpr int kLoads = kStageRows / 8 / kWaves;
+    static_assert(kCols % (8 * kWaves) == 0 && kRows % (8 * kWaves) == 0 && kRows % kWave == 0 && kRows / kWave <= kWaves);
+};
+
+template <int kRowTiles, int kColTiles, int kRowWaves, int kColWaves, bool kGated>
+__global__ void __launch_bounds__(kRowWaves * kColWaves * kWave)
+    experts_tile_kernel(const Product p, char* __restrict__ out, int64_t out_stride, int column_tiles, int column_groups, XcdMap xcd) {
+    using Shape = TileShape<kRowTiles, kColTiles, kRowWaves, kColWaves>;
+    constexpr int kStageBytes = Shape::kStageRows * kScaleBlock;
+    __shared__ __attribute__((aligned(1024))) char stages[2][kStageBytes];
+    __shared__ float row_scales[2][Shape::kRows];
+    __shared__ uint32_t group_amax[kGated ? Shape::kRows : 1][kColWaves];
+
+    // units of kUnitRows x kUnitCols neighbouring tiles, which share their rows and weights in one XCD's L2, go round the XCDs
+    const uint32_t turn = fast_divide(blockIdx.x, xcd.magic, xcd.shift);
+    const uint32_t on_xcd = blockIdx.x - turn * xcd.count;
+    const uint32_t unit = turn / (kUnitRows * kUnitCols) * xcd.count + on_xcd;
+    const uint32_t in_unit = turn % (kUnitRows * kUnitCols);
+    const int row_group = static_cast<int>(unit / column_groups), column_group = static_cast<int>(unit % column_groups);
+    const int column_tile = column_group * kUnitCols + static_cast<int>(in_unit / kUnitRows);
+    if (column_tile >= column_tiles)
+        return;
+    const RowTile tile = find_row_tile<Shape::kRows>(p, row_group * kUnitRows + static_cast<int>(in_unit % kUnitRows));
+    if (tile.expert < 0)
+        return;
+
+    const int lane = threadIdx.x % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int col_wave = wave % kColWaves, row_wave = wave / kColWaves;
+    const int group = lane / kTile, in_tile = lane % kTile;
+    constexpr int kOutTiles = kGated ? kColTiles / 2 : kColTiles;  // column tiles of the output a wavefront makes
+    constexpr int kOutCols = kGated ? Shape::kCols / 2 : Shape::kCols;
+    const int out_columns = kGated ? p.columns / 2 : p.columns;
+    const int first_column = column_tile * kOutCols;
+
+    f32x4 acc[kColTiles][kRowTiles];
+#pragma unroll
+    for (int c = 0; c < kColTiles; ++c)
+#pragma unroll
+        for (int r = 0; r < kRowTiles; ++r)
+            acc[c][r] = {0.0f, 0.0f, 0.0f, 0.0f};
+
+    if (tile.live > 0) {
+        // This lane's part of a stage: load i brings in row 8 * (i * kWaves + wave) + lane / 8 of it, eight lanes a row.  Within its
+        // row the 16-byte piece that the lane fetches, and so where that piece lies in LDS, is turned by the row, so
+        // that eight rows' same piece, which a matrix operand reads at once, lie in different banks.
+        const int piece = (lane % 8) ^ (lane / 8);
+        const char* weight = p.weight + static_cast<int64_t>(tile.expert) * p.columns * p.inner;
+        const char* values = p.values + tile.row * p.value_stride;
+        constexpr int kWeightLoads = Shape::kCols / (8 * Shape::kWaves);
+        uint32_t row_offset[Shape::kLoads];
+#pragma unroll
+        for (int i = 0; i < Shape::kLoads; ++i) {
+            const int first = 8 * (i * Shape::kWaves + wave);
+            const int row = first + lane / 8;
+            if (i < kWeightLoads) {
+                int column;
+                if constexpr (kGated) {
+                    const int in_wave = row % (kTile * kColTiles), half = in_wave / (kTile * kOutTiles);
+                    column = first_column + row / (kTile * kColTiles) * (kTile * kOutTiles) + in_wave % (kTile * kOutTiles);
+                    column = (column < out_columns ? column : out_columns - 1) + half * out_columns;
+                } else {
+                    column = first_column + row;
+                    column = column < out_columns ? column : out_columns - 1;
+                }
+                row_offset[i] = static_cast<uint32_t>(column) * static_cast<uint32_t>(p.inner);
+            } else {
+                const int in_rows = row - Shape::kCols;
+                row_offset[i] = static_cast<uint32_t>(in_rows < tile.live ? in_rows : tile.live - 1) * static_cast<uint32_t>(p.value_stride);
+            }
+        }
+        const int scale_row = wave * kWave + lane < tile.live ? wave * kWave + lane : tile.live - 1;
+        const uint32_t scale_offset = static_cast<uint32_t>(scale_row) * static_cast<uint32_t>(p.scale_stride) * 4u;
+        const char* scales = reinterpret_cast<const char*>(p.scales + tile.row * p.scale_stride);
+        const uint32_t stages_at = lds_address(stages), scales_at = lds_address(row_scales);
+
+        const auto fetch = [&](int block) {
+            const int64_t at = static_cast<int64_t>(block) * kScaleBlock;
+            const bool whole = at + kScaleBlock <= p.inner, in_row = at + piece * 16 < p.inner;
+            const uint32_t to = stages_at + (block & 1) * kStageBytes + static_cast<uint32_t>(wave) * 8 * kScaleBlock;
+            constexpr uint32_t kStep = Shape::kWaves * 8 * kScaleBlock;
+            if (whole) {
+#pragma unroll
+                for (int i = 0; i < Shape::kLoads; ++i)
+                    load_to_lds<16>((i < kWeightLoads ? weight : values) + at, row_offset[i] + piece * 16, to + i * kStep);
+            } else {
+#pragma unroll
+                for (int i = 0; i < Shape::kLoads; ++i)
+                    load_to_lds(in_row ? (i < kWeightLoads ? weight : values) + at + row_offset[i] + piece * 16 : reinterpret_cast<const char*>(&kZeroPiece),
+                                to + i * kStep);
+            }
+            if (wave < Shape::kRows / kWave)
+                load_to_lds<4>(scales + static_cast<int64_t>(block) * 4, scale_offset, scales_at + ((block & 1) * Shape::kRows + static_cast<uint32_t>(wave * kWave)) * 4u);
+        };
+
+        // the scales' blocks of this wavefront's column tiles: one block where they are neighbours within 128 columns
+        constexpr int kScales = kGated ? kColTiles : 1;
+        static_assert(kGated || kScaleBlock % (kColTiles * kTile) == 0);
+        const float* weight_scales[kScales];
+#pragma unroll
+        for (int c = 0; c < kScales; ++c) {
+            int column = first_column + (col_wave * kOutTiles + c % kOutTiles) * kTile;
+            column = (column < out_columns ? column : out_columns - 1) + (c / kOutTiles) * out_columns;
+            weight_scales[c] = p.weight_scales + (static_cast<int64_t>(tile.expert) * p.column_blocks + column / kScaleBlock) * p.blocks;
+        }
+
+        fetch(0);
+        float next_scale[kScales];
+#pragma unroll
+        for (int c = 0; c < kScales; ++c)
+            next_scale[c] = uniform_load(weight_scales[c]);
+        for (int block = 0; block < p.blocks; ++block) {
+            loads_landed();
+            if (block + 1 < p.blocks)
+                fetch(block + 1);
+            const char* stage = stages[block & 1];
+            const int turned = (group ^ (lane & 7)) * 16;
+            const char* weight_at = stage + (col_wave * kColTiles * kTile + in_tile) * kScaleBlock;
+            const char* value_at = stage + (Shape::kCols + row_wave * kRowTiles * kTile + in_tile) * kScaleBlock;
+            float column_scale[kScales];
+#pragma unroll
+            for (int c = 0; c < kScales; ++c)
+                column_scale[c] = next_scale[c];
+            const int next_block = block + 1 < p.blocks ? block + 1 : block;
+#pragma unroll
+            for (int c = 0; c < kScales; ++c)
+                next_scale[c] = uniform_load(weight_scales[c] + next_block);
+            i32x8 weights[kColTiles];
+#pragma unroll
+            for (int c = 0; c < kColTiles; ++c)
+                weights[c] = operand(*reinterpret_cast<const u32x4*>(weight_at + c * kTile * kScaleBlock + turned),
+                                     *reinterpret_cast<const u32x4*>(weight_at + c * kTile * kScaleBlock + (turned ^ 64)));
+            const auto row_operand = [&](int r) {
+                return operand(*reinterpret_cast<const u32x4*>(value_at + r * kTile * kScaleBlock + turned),
+                               *reinterpret_cast<const u32x4*>(value_at + r * kTile * kScaleBlock + (turned ^ 64)));
+            };
+            const float* scale_at = &row_scales[block & 1][row_wave * kRowTiles * kTile + in_tile];
+            i32x8 rows[2];
+            rows[0] = row_operand(0);
+            float scale[2] = {scale_at[0], 0.0f};
+#pragma unroll
+            for (int r = 0; r < kRowTiles; ++r) {
+                // a step's operand is read during the step ahead of it, and not earlier: there are no registers for more
+                __builtin_amdgcn_sched_barrier(0);
+                if (r + 1 < kRowTiles) {
+                    rows[(r + 1) & 1] = row_operand(r + 1);
+                    scale[(r + 1) & 1] = scale_at[(r + 1) * kTile];
+                }
+                f32x4 product[kColTiles];
+#pragma unroll
+                for (int c = 0; c < kColTiles; ++c)
+                    product[c] = block_product<kGated>(weights[c], rows[r & 1]);
+#pragma unroll
+                for (int c = 0; c < kColTiles; ++c) {
+                    const float factor = column_scale[c % kScales] * scale[r & 1];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        acc[c][r][i] = fmaf(factor, product[c][i], acc[c][r][i]);
+                }
+            }
+        }
+    }
+
+    const int first_row = row_wave * kRowTiles * kTile + in_tile;
+    if constexpr (!kGated) {
+#pragma unroll
+        for (int r = 0; r < kRowTiles; ++r) {
+            const int in_rows = first_row + r * kTile;
+            if (in_rows >= tile.size)
+                continue;
+            uint16_t* row = reinterpret_cast<uint16_t*>(out) + (tile.row + in_rows) * out_stride;
+#pragma unroll
+            for (int c = 0; c < kColTiles; ++c) {
+                const int column = first_column + (col_wave * kColTiles + c) * kTile + group * 4;
+                if (column >= out_columns)
+                    continue;
+                const f32x4 v = in_rows < tile.live ? acc[c][r] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                uint2 packed;
+                packed.x = to_bf16_pair(v[0], v[1]);
+                packed.y = to_bf16_pair(v[2], v[3]);
+                *reinterpret_cast<uint2*>(row + column) = packed;
+            }
+        }
+    } else {
+        // the tile's output columns are one group of 128: its largest value is found over the wavefronts through LDS
+        static_assert(!kGated || kOutCols == kScaleBlock);
+#pragma unroll
+        for (int r = 0; r < kRowTiles; ++r) {
+            uint32_t amax = 0;
+            const bool live = first_row + r * kTile < tile.live;
+#pragma unroll
+            for (int c = 0; c < kOutTiles; ++c) {
+                const int column = first_column + (col_wave * kOutTiles + c) * kTile + group * 4;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float act = live && column < out_columns ? silu(acc[c][r][i]) * acc[c + kOutTiles][r][i] : 0.0f;
+                    acc[c][r][i] = act;
+                    amax = larger(amax, magnitude_bits(act));
+                }
+            }
+            amax = larger(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 16, kWave)));
+            amax = larger(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 32, kWave)));
+            if (group == 0)
+                group_amax[first_row + r * kTile][col_wave] = amax;
+        }
+        __syncthreads();
+        const int groups = (out_columns + kScaleBlock - 1) / kScaleBlock;
+#pragma unroll
+        for (int r = 0; r < kRowTiles; ++r) {
+            const int in_rows = first_row + r * kTile;
+            uint32_t amax = group_amax[in_rows][0];
+#pragma unroll
+            for (int w = 1; w < kColWaves; ++w)
+                amax = larger(amax, group_amax[in_rows][w]);
+            const GroupScale scale = group_scale(amax);
+            if (in_rows >= tile.size)
+                continue;
+            char* record = out + (tile.row + in_rows) * out_stride;
+#pragma unroll
+            for (int c = 0; c < kOutTiles; ++c) {
+                const int column = first_column + (col_wave * kOutTiles + c) * kTile + group * 4;
+                if (column < out_columns)
+                    *reinterpret_cast<uint32_t*>(record + column) = to_fp8_quad(acc[c][r][0] * scale.inverse, acc[c][r][1] * scale.inverse,
+                                                                               acc[c][r][2] * scale.inverse, acc[c][r][3] * scale.inverse);
+            }
+            if (col_wave == 0 && group == 0)
+                reinterpret_cast<float*>(record + out_columns)[column_tile] = scale.scale;
+            // the record's padding goes with its last group
+            if (column_tile == column_tiles - 1 && col_wave == kColWaves - 1)
+                for (int word = out_columns / 4 + groups + group; word < static_cast<int>(out_stride / 4); word += 4)
+                    reinterpret_cast<uint32_t*>(record)[word] = 0u;
+        }
+    }
+}
+
 // fp32 rows in 8 bits with a scale for every 128 columns: a wavefront a row, 16 lanes a group of 128 columns.
 __global__ void __launch_bounds__(kBlockThreads) quantize_rows_kernel(const float* __restrict__ rows,
                                                                       char* __restrict__ records,
@@ -327,6 +600,32 @@ int launch_stream(const Product& p, void* out, int64_t out_stride, hipStream_t s
     return NANOEP_OK;
 }
 
+template <int kRowTiles, int kColTiles, int kRowWaves, int kColWaves, bool kGated>
+int launch_tiles(const Product& p, void* out, int64_t out_stride, hipStream_t stream) {
+    using Shape = TileShape<kRowTiles, kColTiles, kRowWaves, kColWaves>;
+    constexpr int kOutCols = kGated ? Shape::kCols / 2 : Shape::kCols;
+    const int out_columns = kGated ? p.columns / 2 : p.columns;
+    const XcdMap xcd = make_xcd_map(current_topology(current_tuning()).xcds);
+    const int column_tiles = (out_columns + kOutCols - 1) / kOutCols;
+    const int column_groups = (column_tiles + kUnitCols - 1) / kUnitCols;
+    const int64_t row_groups = (most_row_tiles(p, Shape::kRows) + kUnitRows - 1) / kUnitRows;
+    const int64_t units = (row_groups * column_groups + xcd.count - 1) / xcd.count * xcd.count;
+    if (units * kUnitRows * kUnitCols > 0x7fffffff)
+        return NANOEP_ERR_INVALID_ARGUMENT;
+    experts_tile_kernel<kRowTiles, kColTiles, kRowWaves, kColWaves, kGated>
+        <<<dim3(static_cast<unsigned>(units * kUnitRows * kUnitCols)), Shape::kThreads, 0, stream>>>(p, static_cast<char*>(out), out_stride,
+                                                                                                    column_tiles, column_groups, xcd);
+    NANOEP_HIP_TRY(hipGetLastError());
+    return NANOEP_OK;
+}
+
+// Whether the tile kernel takes a product: enough rows an expert, and an expert's weight and a tile's rows within the 32-bit
+// offsets it addresses them with.
+bool takes_tiles(int64_t rows, int64_t experts, int inner, int columns, int64_t value_stride, int64_t scale_stride) {
+    constexpr int64_t kMost = int64_t{1} << 32;
+    return rows / experts > 64 && static_cast<int64_t>(columns) * inner <= kMost && value_stride <= kMost / 256 && scale_stride <= kMost / 1024;
+}
+
 template <bool kGated, bool kExact>
 int launch_product(const Product& p, void* out, int64_t out_stride, hipStream_t stream) {
     const int64_t rows_each = p.rows / p.experts;
@@ -354,13 +653,17 @@ int nanoep_experts_linear(const void* values, int64_t value_stride, const float*
     if (out == nullptr || !aligned16(out))
         return NANOEP_ERR_INVALID_ARGUMENT;
     // up to 64 inner columns the 16-bit instructions take no longer than the one 128-wide 8-bit one
+    if (inner > kScaleBlock / 2 && takes_tiles(rows, experts, inner, columns, value_stride, scale_stride))
+        return launch_tiles<8, 4, 2, 4, false>(p, out, columns, static_cast<hipStream_t>(stream));
     if (inner <= kScaleBlock / 2)
         return launch_product<false, true>(p, out, columns, static_cast<hipStream_t>(stream));
     return launch_product<false, false>(p, out, columns, static_cast<hipStream_t>(stream));
 }
 
-size_t nanoep_experts_gated_workspace_bytes(int64_t rows, int64_t experts, int inner, int columns) {
-    if (rows <= 0 || experts <= 0 || inner <= 0 || columns <= 0)
+size_t nanoep_experts_gated_workspace_bytes(int64_t rows, int64_t experts, int inner, int columns, int64_t value_stride,
+                                            int64_t scale_stride) {
+    if (rows <= 0 || experts <= 0 || inner <= 0 || columns <= 0 ||
+        nanoep::takes_tiles(rows, experts, inner, columns, value_stride, scale_stride))
         return 0;
     return static_cast<size_t>(rows) * static_cast<size_t>(columns / 2) * sizeof(float);
 }
@@ -376,12 +679,14 @@ int nanoep_experts_gated(const void* values, int64_t value_stride, const float* 
         return status;
     if (records == nullptr || !aligned16(records))
         return NANOEP_ERR_INVALID_ARGUMENT;
-    const size_t needed = nanoep_experts_gated_workspace_bytes(rows, experts, inner, columns);
+    const size_t needed = nanoep_experts_gated_workspace_bytes(rows, experts, inner, columns, value_stride, scale_stride);
     if (workspace_bytes < needed)
         return NANOEP_ERR_WORKSPACE;
     if (needed > 0 && (workspace == nullptr || !aligned16(workspace)))
         return NANOEP_ERR_INVALID_ARGUMENT;
     const auto on = static_cast<hipStream_t>(stream);
+    if (takes_tiles(rows, experts, inner, columns, value_stride, scale_stride))
+        return launch_tiles<8, 4, 2, 4, true>(p, records, record_bytes_of(columns / 2), on);
     const int launched = launch_product<true, true>(p, workspace, columns / 2, on);
     if (launched != NANOEP_OK)
         return launched;

@@ -221,12 +221,13 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> experts_gated(const torc
     const Device device = values.device();
     const DeviceGuard guard(device);
     Records rows = make_records(p.rows, p.columns / 2, device);
-    const size_t bytes = nanoep_experts_gated_workspace_bytes(p.rows, p.experts, static_cast<int>(p.inner), static_cast<int>(p.columns));
+    const int64_t value_stride = row_stride(values, p.inner, 16), scale_stride = row_stride(scales, scales.size(1), 1);
+    const size_t bytes = nanoep_experts_gated_workspace_bytes(p.rows, p.experts, static_cast<int>(p.inner), static_cast<int>(p.columns),
+                                                              value_stride, scale_stride);
     torch::Tensor workspace;
     if (bytes > 0)
         workspace = make({static_cast<int64_t>(bytes)}, at::kByte, device);
-    check(nanoep_experts_gated(values.data_ptr(), row_stride(values, p.inner, 16), static_cast<const float*>(scales.data_ptr()),
-                               row_stride(scales, scales.size(1), 1), weight.data_ptr(), static_cast<const float*>(weight_scales.data_ptr()),
+    check(nanoep_experts_gated(values.data_ptr(), value_stride, static_cast<const float*>(scales.data_ptr()), scale_stride, weight.data_ptr(), static_cast<const float*>(weight_scales.data_ptr()),
                                p.offsets, p.counts, p.rows, p.experts, static_cast<int>(p.inner), static_cast<int>(p.columns),
                                rows.payload.data_ptr(), bytes > 0 ? workspace.data_ptr() : nullptr, bytes, current_stream(device)),
           what);
