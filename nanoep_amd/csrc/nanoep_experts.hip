@@ -1,18 +1,21 @@
 // The experts' products: rows in 8 bits, one scale for every 128 columns, times weights in 8 bits, one scale a
 // 128 x 128 block, over the expert-major segments that a dispatch leaves.
 
+#include <algorithm>
+
 #include "nanoep_operators.h"
 
 namespace nanoep {
 namespace {
 
 typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTile = 16;  // rows and columns of one matrix instruction's result
-constexpr int kUnitRows = 4, kUnitCols = 8;  // neighbouring tiles that one XCD works on at a time
+constexpr int kUnitRows = 4;  // neighbouring row tiles whose column tiles an XCD works through together
 
 struct Product {
     const char* values;  // rows of e4m3, value_stride bytes apart
@@ -258,7 +261,7 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 }
 
 // Copies 16 (kBytes == 16) or 4 bytes a lane from memory into LDS without registers on the way: lane l's go to
-// `to` + l * kBytes.  `to` and `from` are wave-uniform, `offset` is a lane's own.  Nothing waits for it but loads_landed().
+// `to` + l * kBytes.  `to` and `from` are wave-uniform, `offset` is a lane's own.  Only all_but_newest() waits for it.
 template <int kBytes>
 __device__ __forceinline__ void load_to_lds(const char* from, uint32_t offset, uint32_t to) {
     if constexpr (kBytes == 16)
@@ -275,77 +278,199 @@ __device__ __forceinline__ void load_to_lds(const char* from, uint32_t to) {
 // What is read in the place of a piece that lies past its row's end.
 __device__ const u32x4 kZeroPiece = {0u, 0u, 0u, 0u};
 
-// Every wavefront's copies into LDS are there, and every wavefront has read what the next ones overwrite.
-__device__ __forceinline__ void loads_landed() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+// The same number, which the compiler takes for another: what is computed from it is computed where it is
+// needed, and holds no registers over the loops around that place.
+__device__ __forceinline__ int afresh(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
 }
 
+// Waits until all but the newest kNewer of this wavefront's loads and stores are done, and its reads of LDS, and
+// then for the other wavefronts to say the same.
+template <int kNewer>
+__device__ __forceinline__ void all_but_newest() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kNewer) : "memory");
+}
+
+// Waits for this wavefront's reads and writes of LDS, and for the other wavefronts'.
+__device__ __forceinline__ void lds_settled() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // The products of a tile of 16 * kRowTiles * kRowWaves rows and 16 * kColTiles * kColWaves weight rows, one workgroup.
-template <int kRowTiles, int kColTiles, int kRowWaves, int kColWaves>
+template <int kRowTiles, int kColTiles, int kRowWaves, int kColWaves, bool kGated>
 struct TileShape {
     static constexpr int kWaves = kRowWaves * kColWaves;
     static constexpr int kThreads = kWaves * kWave;
     static constexpr int kRows = kTile * kRowTiles * kRowWaves;
     static constexpr int kCols = kTile * kColTiles * kColWaves;
-    static constexpr int kStageRows = kRows + kCols;  // 128-byte rows of one stage: the weights', then the activations'
-    static constexpr int kLoads = kStageRows / 8 / kWaves;
-    static_assert(kCols % (8 * kWaves) == 0 && kRows % (8 * kWaves) == 0 && kRows % kWave == 0 && kRows / kWave <= kWaves);
+    static constexpr int kOutCols = kGated ? kCols / 2 : kCols;
+    static constexpr int kRowLoads = kRows / 8 / kWaves;     // loads of a wavefront that bring in a block of the rows
+    static constexpr int kWeightLoads = kCols / 8 / kWaves;  // ... and of the weights
+    // stores of a wavefront that write a tile's output
+    static constexpr int kStores = kGated ? kRowTiles * kColTiles / 2 : kRowTiles * kColTiles;
+    static_assert(kRows % (8 * kWaves) == 0 && kCols % (8 * kWaves) == 0 && kRows % kWave == 0);
 };
 
+// One tile of the list that a workgroup works through.
+struct Item {
+    int expert;
+    int row;
+    int live_size;  // live rows, and those that are written, above them (at most 256 each)
+    int column_tile;
+};
+
+constexpr int kMostItems = 256;        // tiles of a list; a workgroup with more makes several
+constexpr int kMostSegments = 1 << 14;  // segments whose prefix sums fit the memory the list is made in
+
+// Fills `items` with this workgroup's tiles from its `first`-th on and returns how many there are.  All tiles, of which
+// every workgroup counts the same number, are numbered so that kUnit neighbours are kUnitRows row tiles by
+// as many column tiles: these share rows and weights, and go to one XCD's workgroups at a time.  `before` has room
+// for the segments' prefix sums, `wave_sums` for one number a wavefront.
+template <int kRows, int kThreads>
+__device__ __forceinline__ int list_tiles(const Product& p, int column_tiles, uint32_t xcd, uint32_t on_xcd, uint32_t xcds, uint32_t unit, int first,
+                                          int* before, int* wave_sums, Item* items) {
+    const int segments = p.experts + (p.expert_offsets != nullptr ? 1 : 0);
+    const int each = (segments + kThreads - 1) / kThreads;
+    const int from = static_cast<int>(threadIdx.x) * each;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    int mine = 0;
+    for (int e = from; e < from + each && e < segments; ++e) {
+        const Segment segment = segment_of(p, e);
+        mine += static_cast<int>((segment.end - segment.begin + kRows - 1) / kRows);
+    }
+    int through = mine;
+#pragma unroll
+    for (int step = 1; step < kWave; step *= 2) {
+        const int other = __shfl_up(through, step, kWave);
+        if (lane >= step)
+            through += other;
+    }
+    if (lane == kWave - 1)
+        wave_sums[wave] = through;
+    lds_settled();
+    int at = through - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / kWave; ++w) {
+        at += w < wave ? wave_sums[w] : 0;
+        total += wave_sums[w];
+    }
+    total = __builtin_amdgcn_readfirstlane(total);
+    for (int e = from; e < from + each && e < segments; ++e) {
+        const Segment segment = segment_of(p, e);
+        before[e] = at;
+        at += static_cast<int>((segment.end - segment.begin + kRows - 1) / kRows);
+    }
+    lds_settled();
+    const uint32_t tiles = static_cast<uint32_t>(total) * static_cast<uint32_t>(column_tiles);
+    for (int i = threadIdx.x; i < kMostItems; i += kThreads) {
+        const uint64_t number = (static_cast<uint64_t>(first + i) * xcds + xcd) * unit + on_xcd;
+        if (number >= tiles)
+            continue;
+        const uint32_t group_tiles = kUnitRows * static_cast<uint32_t>(column_tiles);
+        const uint32_t group = static_cast<uint32_t>(number) / group_tiles, in_group = static_cast<uint32_t>(number) - group * group_tiles;
+        const uint32_t left = static_cast<uint32_t>(total) - group * kUnitRows, group_rows = left < kUnitRows ? left : kUnitRows;
+        const int row_tile = static_cast<int>(group * kUnitRows + in_group % group_rows);
+        // the segment that holds it: the last one that begins at or before it (those behind begin later, or are empty)
+        int low = 0, high = segments;
+        while (high - low > 1) {
+            const int middle = (low + high) / 2;
+            if (before[middle] <= row_tile)
+                low = middle;
+            else
+                high = middle;
+        }
+        const Segment segment = segment_of(p, low);
+        const int skipped = (row_tile - before[low]) * kRows;
+        const int size = static_cast<int>(segment.end - segment.begin) - skipped, live = static_cast<int>(segment.live) - skipped;
+        // (a layout whose segments lie over one another may number more tiles than fit an int: no tile then)
+        if (skipped < 0 || size <= 0) {
+            items[i] = {0, 0, 0, 0};
+            continue;
+        }
+        items[i] = {low, static_cast<int>(segment.begin) + skipped, (live < 0 ? 0 : live > kRows ? kRows : live) | (size > kRows ? kRows : size) << 16,
+                    static_cast<int>(in_group / group_rows)};
+    }
+    lds_settled();
+    const uint64_t start = (static_cast<uint64_t>(first) * xcds + xcd) * unit + on_xcd;
+    const uint64_t stride = static_cast<uint64_t>(xcds) * unit;
+    const uint64_t count = start < tiles ? (tiles - start + stride - 1) / stride : 0;
+    return static_cast<int>(count > kMostItems ? kMostItems : count);
+}
+
+// Products of many rows an expert.  As many workgroups as compute units work through their lists of tiles, 256 rows by 256
+// weight rows (a gated product's: 128 of the gate's and the same 128 of the up projection's, so that its 128 output
+// columns are one group of the output's scales).  A block of 128 inner columns of both lies in LDS, brought there
+// straight from memory; eight wavefronts of 64 weight rows x 128 rows each read their operands from it.
+//
+// What the order below is about is keeping loads and matrix instructions going.  A wavefront reads a block's weights into
+// registers while it works on the last row tile of the block before; half a block on, when all have, their place takes
+// the weights of the block after next.  Those come from HBM, all at once for an XCD's workgroups, and have 1.5 blocks'
+// time for it.  Rows mostly come from L2 and have one block's.  The two cursors run on into the next tile, whose first
+// operands so arrive while this one's output is written.
+//
+// Measured (32 experts, 29500 rows): 2048 -> 7168 590 us, 1.47 PFLOP/s; gated 7168 -> 2 x 2048 1690 us, 1.02 PFLOP/s (its bf16
+// instructions have half the rate).  A block of a tile takes 2.0 us; its matrix instructions alone take 0.98 us, its
+// loads alone 1.36 us: 64 KB that L2 hands out in 64-byte requests, of which a block of all tiles needs about as many
+// clocks as its matrix instructions.  One block's time ahead for the weights, the loads alone took 1.76 us.
 template <int kRowTiles, int kColTiles, int kRowWaves, int kColWaves, bool kGated>
 __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave)
-    experts_tile_kernel(const Product p, char* __restrict__ out, int64_t out_stride, int column_tiles, int column_groups, XcdMap xcd) {
-    using Shape = TileShape<kRowTiles, kColTiles, kRowWaves, kColWaves>;
-    constexpr int kStageBytes = Shape::kStageRows * kScaleBlock;
-    __shared__ __attribute__((aligned(1024))) char stages[2][kStageBytes];
+    experts_tile_kernel(const Product p, char* __restrict__ out, int64_t out_stride, int column_tiles, XcdMap xcds) {
+    using Shape = TileShape<kRowTiles, kColTiles, kRowWaves, kColWaves, kGated>;
+    constexpr int kWeightBytes = Shape::kCols * kScaleBlock, kRowBytes = Shape::kRows * kScaleBlock;
+    __shared__ __attribute__((aligned(1024))) char weight_blocks[2][kWeightBytes];
+    __shared__ __attribute__((aligned(1024))) char row_blocks[2][kRowBytes];
     __shared__ float row_scales[2][Shape::kRows];
     __shared__ uint32_t group_amax[kGated ? Shape::kRows : 1][kColWaves];
-
-    // units of kUnitRows x kUnitCols neighbouring tiles, which share their rows and weights in one XCD's L2, go round the XCDs
-    const uint32_t turn = fast_divide(blockIdx.x, xcd.magic, xcd.shift);
-    const uint32_t on_xcd = blockIdx.x - turn * xcd.count;
-    const uint32_t unit = turn / (kUnitRows * kUnitCols) * xcd.count + on_xcd;
-    const uint32_t in_unit = turn % (kUnitRows * kUnitCols);
-    const int row_group = static_cast<int>(unit / column_groups), column_group = static_cast<int>(unit % column_groups);
-    const int column_tile = column_group * kUnitCols + static_cast<int>(in_unit / kUnitRows);
-    if (column_tile >= column_tiles)
-        return;
-    const RowTile tile = find_row_tile<Shape::kRows>(p, row_group * kUnitRows + static_cast<int>(in_unit % kUnitRows));
-    if (tile.expert < 0)
-        return;
+    __shared__ int wave_sums[Shape::kWaves];
+    __shared__ Item items[kMostItems];
+    static_assert(sizeof(weight_blocks) >= kMostSegments * sizeof(int));
 
     const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int col_wave = wave % kColWaves, row_wave = wave / kColWaves;
     const int group = lane / kTile, in_tile = lane % kTile;
-    constexpr int kOutTiles = kGated ? kColTiles / 2 : kColTiles;  // column tiles of the output a wavefront makes
-    constexpr int kOutCols = kGated ? Shape::kCols / 2 : Shape::kCols;
+    constexpr int kOutTiles = kGated ? kColTiles / 2 : kColTiles;  // column tiles of the output that a wavefront makes
     const int out_columns = kGated ? p.columns / 2 : p.columns;
-    const int first_column = column_tile * kOutCols;
+    const uint32_t on_xcd = fast_divide(blockIdx.x, xcds.magic, xcds.shift);
+    const uint32_t xcd = blockIdx.x - on_xcd * xcds.count;
+    const uint32_t unit = fast_divide(gridDim.x, xcds.magic, xcds.shift);
 
-    f32x4 acc[kColTiles][kRowTiles];
-#pragma unroll
-    for (int c = 0; c < kColTiles; ++c)
-#pragma unroll
-        for (int r = 0; r < kRowTiles; ++r)
-            acc[c][r] = {0.0f, 0.0f, 0.0f, 0.0f};
+    // A lane's part of a load: row lane / 8 of the load's eight and, of that row, a 16-byte piece that is turned by the row,
+    // and with it the piece's place in LDS, so that the same piece of eight rows, which a matrix operand reads at
+    // once, lies in different banks.
+    const int piece = (lane % 8) ^ (lane / 8);
+    const uint32_t weights_at = lds_address(weight_blocks) + wave * 8 * kScaleBlock, rows_at = lds_address(row_blocks) + wave * 8 * kScaleBlock;
+    const uint32_t scales_at = lds_address(row_scales) + (wave * kWave % Shape::kRows) * 4;
+    constexpr uint32_t kStep = Shape::kWaves * 8 * kScaleBlock;
 
-    if (tile.live > 0) {
-        // This lane's part of a stage: load i brings in row 8 * (i * kWaves + wave) + lane / 8 of it, eight lanes a row.  Within its
-        // row the 16-byte piece that the lane fetches, and so where that piece lies in LDS, is turned by the row, so
-        // that eight rows' same piece, which a matrix operand reads at once, lie in different banks.
-        const int piece = (lane % 8) ^ (lane / 8);
-        const char* weight = p.weight + static_cast<int64_t>(tile.expert) * p.columns * p.inner;
-        const char* values = p.values + tile.row * p.value_stride;
-        constexpr int kWeightLoads = Shape::kCols / (8 * Shape::kWaves);
-        uint32_t row_offset[Shape::kLoads];
+    for (int listed = 0;; listed += kMostItems) {
+        const int count = list_tiles<Shape::kRows, Shape::kThreads>(p, column_tiles, xcd, on_xcd, xcds.count, unit, listed,
+                                                                    reinterpret_cast<int*>(weight_blocks), wave_sums, items);
+        const auto item_at = [&](int i) -> Item {
+            const Item item = items[i];
+            return {__builtin_amdgcn_readfirstlane(item.expert), __builtin_amdgcn_readfirstlane(item.row),
+                    __builtin_amdgcn_readfirstlane(item.live_size), __builtin_amdgcn_readfirstlane(item.column_tile)};
+        };
+        const auto next_live = [&](int i) {
+            while (i < count && (__builtin_amdgcn_readfirstlane(items[i].live_size) & 0xffff) == 0)
+                ++i;
+            return i;
+        };
+
+        // the weights' cursor
+        int weight_item = next_live(0), weight_block = 0, weight_slot = 0;
+        const char* weight = nullptr;
+        uint32_t weight_offset[Shape::kWeightLoads];
+        const auto aim_weights = [&]() {
+            const Item item = item_at(weight_item);
+            weight = p.weight + static_cast<int64_t>(item.expert) * p.columns * p.inner;
+            const int first_column = item.column_tile * Shape::kOutCols;
+            const int row_in_load = afresh(lane) / 8;
 #pragma unroll
-        for (int i = 0; i < Shape::kLoads; ++i) {
-            const int first = 8 * (i * Shape::kWaves + wave);
-            const int row = first + lane / 8;
-            if (i < kWeightLoads) {
+            for (int i = 0; i < Shape::kWeightLoads; ++i) {
+                const int row = 8 * (i * Shape::kWaves + wave) + row_in_load;
                 int column;
                 if constexpr (kGated) {
+                    // a wavefront's weight rows: its tiles of the gate, then the same ones of the up projection
                     const int in_wave = row % (kTile * kColTiles), half = in_wave / (kTile * kOutTiles);
                     column = first_column + row / (kTile * kColTiles) * (kTile * kOutTiles) + in_wave % (kTile * kOutTiles);
                     column = (column < out_columns ? column : out_columns - 1) + half * out_columns;
@@ -353,173 +478,304 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave)
                     column = first_column + row;
                     column = column < out_columns ? column : out_columns - 1;
                 }
-                row_offset[i] = static_cast<uint32_t>(column) * static_cast<uint32_t>(p.inner);
-            } else {
-                const int in_rows = row - Shape::kCols;
-                row_offset[i] = static_cast<uint32_t>(in_rows < tile.live ? in_rows : tile.live - 1) * static_cast<uint32_t>(p.value_stride);
+                weight_offset[i] = static_cast<uint32_t>(column) * static_cast<uint32_t>(p.inner);
             }
-        }
-        const int scale_row = wave * kWave + lane < tile.live ? wave * kWave + lane : tile.live - 1;
-        const uint32_t scale_offset = static_cast<uint32_t>(scale_row) * static_cast<uint32_t>(p.scale_stride) * 4u;
-        const char* scales = reinterpret_cast<const char*>(p.scales + tile.row * p.scale_stride);
-        const uint32_t stages_at = lds_address(stages), scales_at = lds_address(row_scales);
-
-        const auto fetch = [&](int block) {
-            const int64_t at = static_cast<int64_t>(block) * kScaleBlock;
-            const bool whole = at + kScaleBlock <= p.inner, in_row = at + piece * 16 < p.inner;
-            const uint32_t to = stages_at + (block & 1) * kStageBytes + static_cast<uint32_t>(wave) * 8 * kScaleBlock;
-            constexpr uint32_t kStep = Shape::kWaves * 8 * kScaleBlock;
-            if (whole) {
+        };
+        // brings in the cursor's block; whether there was one
+        const auto fetch_weights = [&]() {
+            if (weight_item >= count)
+                return false;
+            const int64_t at = static_cast<int64_t>(weight_block) * kScaleBlock;
+            const uint32_t to = weights_at + weight_slot * kWeightBytes;
+            if (at + kScaleBlock <= p.inner) {
 #pragma unroll
-                for (int i = 0; i < Shape::kLoads; ++i)
-                    load_to_lds<16>((i < kWeightLoads ? weight : values) + at, row_offset[i] + piece * 16, to + i * kStep);
+                for (int i = 0; i < Shape::kWeightLoads; ++i)
+                    load_to_lds<16>(weight + at, weight_offset[i] + piece * 16, to + i * kStep);
             } else {
 #pragma unroll
-                for (int i = 0; i < Shape::kLoads; ++i)
-                    load_to_lds(in_row ? (i < kWeightLoads ? weight : values) + at + row_offset[i] + piece * 16 : reinterpret_cast<const char*>(&kZeroPiece),
+                for (int i = 0; i < Shape::kWeightLoads; ++i)
+                    load_to_lds(at + piece * 16 < p.inner ? weight + at + weight_offset[i] + piece * 16 : reinterpret_cast<const char*>(&kZeroPiece),
                                 to + i * kStep);
             }
-            if (wave < Shape::kRows / kWave)
-                load_to_lds<4>(scales + static_cast<int64_t>(block) * 4, scale_offset, scales_at + ((block & 1) * Shape::kRows + static_cast<uint32_t>(wave * kWave)) * 4u);
+            weight_slot ^= 1;
+            if (++weight_block == p.blocks) {
+                weight_block = 0;
+                weight_item = next_live(weight_item + 1);
+                if (weight_item < count)
+                    aim_weights();
+            }
+            return true;
         };
 
-        // the scales' blocks of this wavefront's column tiles: one block where they are neighbours within 128 columns
-        constexpr int kScales = kGated ? kColTiles : 1;
-        static_assert(kGated || kScaleBlock % (kColTiles * kTile) == 0);
-        const float* weight_scales[kScales];
+        // the rows' cursor; rows past the live ones are the last one again, and what they give is not written
+        int row_item = weight_item, row_block = 0, row_slot = 0;
+        const char *values = nullptr, *scales = nullptr;
+        uint32_t row_offset[Shape::kRowLoads], scale_offset = 0;
+        const auto aim_rows = [&]() {
+            const Item item = item_at(row_item);
+            const int live = item.live_size & 0xffff;
+            values = p.values + static_cast<int64_t>(item.row) * p.value_stride;
+            scales = reinterpret_cast<const char*>(p.scales + static_cast<int64_t>(item.row) * p.scale_stride);
+            const int row_in_load = afresh(lane) / 8;
 #pragma unroll
-        for (int c = 0; c < kScales; ++c) {
-            int column = first_column + (col_wave * kOutTiles + c % kOutTiles) * kTile;
-            column = (column < out_columns ? column : out_columns - 1) + (c / kOutTiles) * out_columns;
-            weight_scales[c] = p.weight_scales + (static_cast<int64_t>(tile.expert) * p.column_blocks + column / kScaleBlock) * p.blocks;
-        }
+            for (int i = 0; i < Shape::kRowLoads; ++i) {
+                const int row = 8 * (i * Shape::kWaves + wave) + row_in_load;
+                row_offset[i] = static_cast<uint32_t>(row < live ? row : live - 1) * static_cast<uint32_t>(p.value_stride);
+            }
+            const int scaled = wave * kWave % Shape::kRows + afresh(lane);
+            scale_offset = static_cast<uint32_t>(scaled < live ? scaled : live - 1) * static_cast<uint32_t>(p.scale_stride) * 4u;
+        };
+        const auto fetch_rows = [&]() {
+            if (row_item >= count)
+                return;
+            const int64_t at = static_cast<int64_t>(row_block) * kScaleBlock;
+            const uint32_t to = rows_at + row_slot * kRowBytes;
+            if (at + kScaleBlock <= p.inner) {
+#pragma unroll
+                for (int i = 0; i < Shape::kRowLoads; ++i)
+                    load_to_lds<16>(values + at, row_offset[i] + piece * 16, to + i * kStep);
+            } else {
+#pragma unroll
+                for (int i = 0; i < Shape::kRowLoads; ++i)
+                    load_to_lds(at + piece * 16 < p.inner ? values + at + row_offset[i] + piece * 16 : reinterpret_cast<const char*>(&kZeroPiece),
+                                to + i * kStep);
+            }
+            // (where there are more wavefronts than 64 rows, some bring in the same scales)
+            load_to_lds<4>(scales + static_cast<int64_t>(row_block) * 4, scale_offset, scales_at + row_slot * Shape::kRows * 4);
+            row_slot ^= 1;
+            if (++row_block == p.blocks) {
+                row_block = 0;
+                row_item = next_live(row_item + 1);
+                if (row_item < count)
+                    aim_rows();
+            }
+        };
 
-        fetch(0);
-        float next_scale[kScales];
-#pragma unroll
-        for (int c = 0; c < kScales; ++c)
-            next_scale[c] = uniform_load(weight_scales[c]);
-        for (int block = 0; block < p.blocks; ++block) {
-            loads_landed();
-            if (block + 1 < p.blocks)
-                fetch(block + 1);
-            const char* stage = stages[block & 1];
-            const int turned = (group ^ (lane & 7)) * 16;
-            const char* weight_at = stage + (col_wave * kColTiles * kTile + in_tile) * kScaleBlock;
-            const char* value_at = stage + (Shape::kCols + row_wave * kRowTiles * kTile + in_tile) * kScaleBlock;
-            float column_scale[kScales];
-#pragma unroll
-            for (int c = 0; c < kScales; ++c)
-                column_scale[c] = next_scale[c];
-            const int next_block = block + 1 < p.blocks ? block + 1 : block;
-#pragma unroll
-            for (int c = 0; c < kScales; ++c)
-                next_scale[c] = uniform_load(weight_scales[c] + next_block);
-            i32x8 weights[kColTiles];
+        int slot = 0;
+        const int turned = (group ^ (lane & 7)) * 16;
+        const int weight_at = (col_wave * kColTiles * kTile + in_tile) * kScaleBlock, row_at = (row_wave * kRowTiles * kTile + in_tile) * kScaleBlock;
+        const int scale_at = row_wave * kRowTiles * kTile + in_tile;
+        // a lane's two pieces of a row: columns group * 16 on of the block, and 64 further
+        const auto weight_piece = [&](int in_slot, int c, int half) {
+            return *reinterpret_cast<const u32x4*>(weight_blocks[in_slot] + weight_at + c * kTile * kScaleBlock + (turned ^ half * 64));
+        };
+        const auto row_piece = [&](int in_slot, int r, int half) {
+            return *reinterpret_cast<const u32x4*>(row_blocks[in_slot] + row_at + r * kTile * kScaleBlock + (turned ^ half * 64));
+        };
+        i32x8 weights[kGated ? 1 : kColTiles];
+        bf16x8 wide_weights[kGated ? kColTiles : 1][4];
+        const auto read_weights = [&](int in_slot, int c) {
+            const u32x4 low = weight_piece(in_slot, c, 0), high = weight_piece(in_slot, c, 1);
+            if constexpr (kGated) {
+                wide_weights[c][0] = widened(low.x, low.y);
+                wide_weights[c][1] = widened(low.z, low.w);
+                wide_weights[c][2] = widened(high.x, high.y);
+                wide_weights[c][3] = widened(high.z, high.w);
+            } else {
+                weights[c] = operand(low, high);
+            }
+        };
+        u32x4 rows[2][2];
+        float scale[2];
+        const auto read_rows = [&](int in_slot, int r, int to) {
+            rows[to][0] = row_piece(in_slot, r, 0);
+            rows[to][1] = row_piece(in_slot, r, 1);
+            scale[to] = row_scales[in_slot][scale_at + r * kTile];
+        };
+        if (weight_item < count) {
+            aim_weights();
+            aim_rows();
+            fetch_weights();
+            fetch_rows();
+            all_but_newest<0>();
+            fetch_weights();
+            fetch_rows();
 #pragma unroll
             for (int c = 0; c < kColTiles; ++c)
-                weights[c] = operand(*reinterpret_cast<const u32x4*>(weight_at + c * kTile * kScaleBlock + turned),
-                                     *reinterpret_cast<const u32x4*>(weight_at + c * kTile * kScaleBlock + (turned ^ 64)));
-            const auto row_operand = [&](int r) {
-                return operand(*reinterpret_cast<const u32x4*>(value_at + r * kTile * kScaleBlock + turned),
-                               *reinterpret_cast<const u32x4*>(value_at + r * kTile * kScaleBlock + (turned ^ 64)));
-            };
-            const float* scale_at = &row_scales[block & 1][row_wave * kRowTiles * kTile + in_tile];
-            i32x8 rows[2];
-            rows[0] = row_operand(0);
-            float scale[2] = {scale_at[0], 0.0f};
-#pragma unroll
-            for (int r = 0; r < kRowTiles; ++r) {
-                // a step's operand is read during the step ahead of it, and not earlier: there are no registers for more
-                __builtin_amdgcn_sched_barrier(0);
-                if (r + 1 < kRowTiles) {
-                    rows[(r + 1) & 1] = row_operand(r + 1);
-                    scale[(r + 1) & 1] = scale_at[(r + 1) * kTile];
-                }
-                f32x4 product[kColTiles];
-#pragma unroll
-                for (int c = 0; c < kColTiles; ++c)
-                    product[c] = block_product<kGated>(weights[c], rows[r & 1]);
-#pragma unroll
-                for (int c = 0; c < kColTiles; ++c) {
-                    const float factor = column_scale[c % kScales] * scale[r & 1];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        acc[c][r][i] = fmaf(factor, product[c][i], acc[c][r][i]);
-                }
-            }
+                read_weights(0, c);
+            read_rows(0, 0, 0);
         }
-    }
+        bool weights_ahead = false;
+        bool stored = false;  // the newest accesses are a tile's stores
+        for (int i = 0; i < count; ++i) {
+            const Item item = item_at(i);
+            const int live = item.live_size & 0xffff, size = item.live_size >> 16;
+            const int first_column = item.column_tile * Shape::kOutCols;
+            f32x4 acc[kColTiles][kRowTiles];
+#pragma unroll
+            for (int c = 0; c < kColTiles; ++c)
+#pragma unroll
+                for (int r = 0; r < kRowTiles; ++r)
+                    acc[c][r] = {0.0f, 0.0f, 0.0f, 0.0f};
 
-    const int first_row = row_wave * kRowTiles * kTile + in_tile;
-    if constexpr (!kGated) {
+            if (live > 0) {
+                // the scales of this wavefront's column tiles: one where they are neighbours within 128 columns
+                constexpr int kScales = kGated ? kColTiles : 1;
+                static_assert(kGated || kScaleBlock % (kColTiles * kTile) == 0);
+                static_assert(kRowTiles % 2 == 0);  // a step's place of the two that hold row operands goes by its number
+                constexpr int kRefill = kRowTiles / 2 - 1;
+                const float* weight_scales[kScales];
+                float next_scale[kScales];
 #pragma unroll
-        for (int r = 0; r < kRowTiles; ++r) {
-            const int in_rows = first_row + r * kTile;
-            if (in_rows >= tile.size)
-                continue;
-            uint16_t* row = reinterpret_cast<uint16_t*>(out) + (tile.row + in_rows) * out_stride;
+                for (int c = 0; c < kScales; ++c) {
+                    int column = first_column + (col_wave * kOutTiles + c % kOutTiles) * kTile;
+                    column = (column < out_columns ? column : out_columns - 1) + (c / kOutTiles) * out_columns;
+                    weight_scales[c] = p.weight_scales + (static_cast<int64_t>(item.expert) * p.column_blocks + column / kScaleBlock) * p.blocks;
+                    next_scale[c] = uniform_load(weight_scales[c]);
+                }
+                for (int block = 0; block < p.blocks; ++block) {
+                    float column_scale[kScales];
+                    const int next_block = block + 1 < p.blocks ? block + 1 : block;
 #pragma unroll
-            for (int c = 0; c < kColTiles; ++c) {
-                const int column = first_column + (col_wave * kColTiles + c) * kTile + group * 4;
-                if (column >= out_columns)
-                    continue;
-                const f32x4 v = in_rows < tile.live ? acc[c][r] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                uint2 packed;
-                packed.x = to_bf16_pair(v[0], v[1]);
-                packed.y = to_bf16_pair(v[2], v[3]);
-                *reinterpret_cast<uint2*>(row + column) = packed;
-            }
-        }
-    } else {
-        // the tile's output columns are one group of 128: its largest value is found over the wavefronts through LDS
-        static_assert(!kGated || kOutCols == kScaleBlock);
+                    for (int c = 0; c < kScales; ++c) {
+                        column_scale[c] = next_scale[c];
+                        next_scale[c] = uniform_load(weight_scales[c] + next_block);
+                    }
 #pragma unroll
-        for (int r = 0; r < kRowTiles; ++r) {
-            uint32_t amax = 0;
-            const bool live = first_row + r * kTile < tile.live;
+                    for (int r = 0; r < kRowTiles; ++r) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (r == kRefill) {
+                            // every wavefront has read the block's weights: the next but one's may come
+                            lds_settled();
+                            weights_ahead = fetch_weights();
+                        }
+                        if (r + 1 < kRowTiles) {
+                            read_rows(slot, r + 1, (r + 1) & 1);
+                        } else {
+                            // The next block's operands are there, and every wavefront has read this block's last row tile. The
+                            // matrix instructions of that tile hide the first reads of the next block.
+                            if (!weights_ahead)
+                                all_but_newest<0>();
+                            else if (stored)
+                                all_but_newest<Shape::kWeightLoads + Shape::kStores>();
+                            else
+                                all_but_newest<Shape::kWeightLoads>();
+                            stored = false;
+                            fetch_rows();
+                            read_rows(slot ^ 1, 0, 0);
+                        }
+                        f32x4 product[kColTiles];
 #pragma unroll
-            for (int c = 0; c < kOutTiles; ++c) {
-                const int column = first_column + (col_wave * kOutTiles + c) * kTile + group * 4;
+                        for (int c = 0; c < kColTiles; ++c)
+                            product[c] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        if constexpr (kGated) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float act = live && column < out_columns ? silu(acc[c][r][i]) * acc[c + kOutTiles][r][i] : 0.0f;
-                    acc[c][r][i] = act;
-                    amax = larger(amax, magnitude_bits(act));
+                            for (int part = 0; part < 4; ++part) {
+                                const u32x4 raw = rows[r & 1][part / 2];
+                                const bf16x8 wide = part % 2 == 0 ? widened(raw.x, raw.y) : widened(raw.z, raw.w);
+#pragma unroll
+                                for (int c = 0; c < kColTiles; ++c)
+                                    product[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wide_weights[c][part], wide, product[c], 0, 0, 0);
+                            }
+                        } else {
+                            const i32x8 row = operand(rows[r & 1][0], rows[r & 1][1]);
+#pragma unroll
+                            for (int c = 0; c < kColTiles; ++c)
+                                product[c] = block_product<false>(weights[c], row);
+                        }
+                        if (r + 1 == kRowTiles) {
+                            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                            for (int c = 0; c < kColTiles; ++c)
+                                read_weights(slot ^ 1, c);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+#pragma unroll
+                        for (int c = 0; c < kColTiles; ++c) {
+                            const float factor = column_scale[c % kScales] * scale[r & 1];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                acc[c][r][j] = fmaf(factor, product[c][j], acc[c][r][j]);
+                        }
+                        // (done here, not where the sums are next used, with all products kept until then)
+                        static_assert(kColTiles == 4);
+                        asm volatile("" : "+v"(acc[0][r]), "+v"(acc[1][r]), "+v"(acc[2][r]), "+v"(acc[3][r]));
+                    }
+                    slot ^= 1;
                 }
             }
-            amax = larger(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 16, kWave)));
-            amax = larger(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 32, kWave)));
-            if (group == 0)
-                group_amax[first_row + r * kTile][col_wave] = amax;
-        }
-        __syncthreads();
-        const int groups = (out_columns + kScaleBlock - 1) / kScaleBlock;
+
+            // Stores past the tile's rows or columns are dropped by the buffer's bounds, not branched around: a wavefront's
+            // number of them is always the same, which the count of newest accesses above relies on.
+            const int out_lane = afresh(lane), in_group = out_lane / kTile;
+            const int first_row = row_wave * kRowTiles * kTile + out_lane % kTile;
+            constexpr uint32_t kNowhere = 0xffffffffu;
+            char* tile_out = out + item.row * out_stride;
+            const __amdgpu_buffer_rsrc_t tile_rows = __builtin_amdgcn_make_buffer_rsrc(tile_out, 0, static_cast<int>(size * out_stride), 0x00020000);
+            if constexpr (!kGated) {
 #pragma unroll
-        for (int r = 0; r < kRowTiles; ++r) {
-            const int in_rows = first_row + r * kTile;
-            uint32_t amax = group_amax[in_rows][0];
+                for (int r = 0; r < kRowTiles; ++r) {
+                    const int in_rows = first_row + r * kTile;
+                    const uint32_t row = static_cast<uint32_t>(in_rows) * static_cast<uint32_t>(out_stride);
 #pragma unroll
-            for (int w = 1; w < kColWaves; ++w)
-                amax = larger(amax, group_amax[in_rows][w]);
-            const GroupScale scale = group_scale(amax);
-            if (in_rows >= tile.size)
-                continue;
-            char* record = out + (tile.row + in_rows) * out_stride;
+                    for (int c = 0; c < kColTiles; ++c) {
+                        const int column = first_column + (col_wave * kColTiles + c) * kTile + in_group * 4;
+                        const f32x4 v = in_rows < live ? acc[c][r] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                        const u32x2 packed = {to_bf16_pair(v[0], v[1]), to_bf16_pair(v[2], v[3])};
+                        __builtin_amdgcn_raw_buffer_store_b64(packed, tile_rows, column < out_columns ? row + column * 2 : kNowhere, 0, 0);
+                    }
+                }
+            } else {
+                // the tile's output columns are one group of 128: its largest value is found over the wavefronts through LDS
+                static_assert(!kGated || Shape::kOutCols == kScaleBlock);
 #pragma unroll
-            for (int c = 0; c < kOutTiles; ++c) {
-                const int column = first_column + (col_wave * kOutTiles + c) * kTile + group * 4;
-                if (column < out_columns)
-                    *reinterpret_cast<uint32_t*>(record + column) = to_fp8_quad(acc[c][r][0] * scale.inverse, acc[c][r][1] * scale.inverse,
-                                                                               acc[c][r][2] * scale.inverse, acc[c][r][3] * scale.inverse);
+                for (int r = 0; r < kRowTiles; ++r) {
+                    uint32_t amax = 0;
+                    const bool is_live = first_row + r * kTile < live;
+#pragma unroll
+                    for (int c = 0; c < kOutTiles; ++c) {
+                        const int column = first_column + (col_wave * kOutTiles + c) * kTile + in_group * 4;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float act = is_live && column < out_columns ? silu(acc[c][r][j]) * acc[c + kOutTiles][r][j] : 0.0f;
+                            acc[c][r][j] = act;
+                            amax = larger(amax, magnitude_bits(act));
+                        }
+                    }
+                    amax = larger(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 16, kWave)));
+                    amax = larger(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 32, kWave)));
+                    if (in_group == 0)
+                        group_amax[first_row + r * kTile][col_wave] = amax;
+                }
+                lds_settled();
+#pragma unroll
+                for (int r = 0; r < kRowTiles; ++r) {
+                    const int in_rows = first_row + r * kTile;
+                    uint32_t amax = group_amax[in_rows][0];
+#pragma unroll
+                    for (int w = 1; w < kColWaves; ++w)
+                        amax = larger(amax, group_amax[in_rows][w]);
+                    const GroupScale scale = group_scale(amax);
+                    const uint32_t row = static_cast<uint32_t>(in_rows) * static_cast<uint32_t>(out_stride);
+                    // the scale, and the record's padding with its last group
+                    if (col_wave == 0 && in_group == 0 && in_rows < size)
+                        reinterpret_cast<float*>(tile_out + row + out_columns)[item.column_tile] = scale.scale;
+                    if (item.column_tile == column_tiles - 1 && col_wave == kColWaves - 1 && in_rows < size)
+                        for (int word = out_columns / 4 + column_tiles + in_group; word < static_cast<int>(out_stride / 4); word += 4)
+                            reinterpret_cast<uint32_t*>(tile_out + row)[word] = 0u;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int c = 0; c < kOutTiles; ++c)
+                            acc[c][r][j] *= scale.inverse;
+                }
+#pragma unroll
+                for (int r = 0; r < kRowTiles; ++r) {
+                    const uint32_t row = static_cast<uint32_t>(first_row + r * kTile) * static_cast<uint32_t>(out_stride);
+#pragma unroll
+                    for (int c = 0; c < kOutTiles; ++c) {
+                        const int column = first_column + (col_wave * kOutTiles + c) * kTile + in_group * 4;
+                        __builtin_amdgcn_raw_buffer_store_b32(to_fp8_quad(acc[c][r][0], acc[c][r][1], acc[c][r][2], acc[c][r][3]), tile_rows,
+                                                              column < out_columns ? row + column : kNowhere, 0, 0);
+                    }
+                }
             }
-            if (col_wave == 0 && group == 0)
-                reinterpret_cast<float*>(record + out_columns)[column_tile] = scale.scale;
-            // the record's padding goes with its last group
-            if (column_tile == column_tiles - 1 && col_wave == kColWaves - 1)
-                for (int word = out_columns / 4 + groups + group; word < static_cast<int>(out_stride / 4); word += 4)
-                    reinterpret_cast<uint32_t*>(record)[word] = 0u;
+            stored = true;
         }
+        // (the list's memory is the weights': nothing may still be on its way there)
+        if (count < kMostItems)
+            return;
+        all_but_newest<0>();
     }
 }
 
@@ -602,28 +858,37 @@ int launch_stream(const Product& p, void* out, int64_t out_stride, hipStream_t s
 
 template <int kRowTiles, int kColTiles, int kRowWaves, int kColWaves, bool kGated>
 int launch_tiles(const Product& p, void* out, int64_t out_stride, hipStream_t stream) {
-    using Shape = TileShape<kRowTiles, kColTiles, kRowWaves, kColWaves>;
-    constexpr int kOutCols = kGated ? Shape::kCols / 2 : Shape::kCols;
+    using Shape = TileShape<kRowTiles, kColTiles, kRowWaves, kColWaves, kGated>;
+    const Topology topology = current_topology(current_tuning());
+    const XcdMap xcds = make_xcd_map(topology.xcds);
     const int out_columns = kGated ? p.columns / 2 : p.columns;
-    const XcdMap xcd = make_xcd_map(current_topology(current_tuning()).xcds);
-    const int column_tiles = (out_columns + kOutCols - 1) / kOutCols;
-    const int column_groups = (column_tiles + kUnitCols - 1) / kUnitCols;
-    const int64_t row_groups = (most_row_tiles(p, Shape::kRows) + kUnitRows - 1) / kUnitRows;
-    const int64_t units = (row_groups * column_groups + xcd.count - 1) / xcd.count * xcd.count;
-    if (units * kUnitRows * kUnitCols > 0x7fffffff)
+    const int column_tiles = (out_columns + Shape::kOutCols - 1) / Shape::kOutCols;
+    if (most_row_tiles(p, Shape::kRows) * column_tiles > 0x7fffffff)
         return NANOEP_ERR_INVALID_ARGUMENT;
+    // a workgroup a compute unit, the same number on every XCD
+    const unsigned workgroups = xcds.count * std::max(1u, static_cast<unsigned>(topology.cus) / xcds.count);
     experts_tile_kernel<kRowTiles, kColTiles, kRowWaves, kColWaves, kGated>
-        <<<dim3(static_cast<unsigned>(units * kUnitRows * kUnitCols)), Shape::kThreads, 0, stream>>>(p, static_cast<char*>(out), out_stride,
-                                                                                                    column_tiles, column_groups, xcd);
+        <<<dim3(workgroups), Shape::kThreads, 0, stream>>>(p, static_cast<char*>(out), out_stride, column_tiles, xcds);
     NANOEP_HIP_TRY(hipGetLastError());
     return NANOEP_OK;
 }
 
-// Whether the tile kernel takes a product: enough rows an expert, and an expert's weight and a tile's rows within the 32-bit
-// offsets it addresses them with.
+// Tiles of 256 rows, of 128 where an expert has fewer rows than that on average.  Of 32 experts, 2048 -> 7168: 115 rows
+// each 136 us with 128-row tiles and 175 with 256-row ones, 230 rows 207 and 202 (gated, 7168 -> 2048: 580 and 626), 460 rows 355
+// and 338 (gated 973 and 891).
+template <bool kGated>
+int launch_tiles_by_rows(const Product& p, void* out, int64_t out_stride, hipStream_t stream) {
+    if (p.rows / p.experts > 256)
+        return launch_tiles<8, 4, 2, 4, kGated>(p, out, out_stride, stream);
+    return launch_tiles<4, 4, 2, 4, kGated>(p, out, out_stride, stream);
+}
+
+// Whether the tile kernel takes a product: enough rows an expert, no more experts than its list of tiles is made from, and an
+// expert's weight and a tile's rows, in and out, within the 32-bit offsets it addresses them with.
 bool takes_tiles(int64_t rows, int64_t experts, int inner, int columns, int64_t value_stride, int64_t scale_stride) {
     constexpr int64_t kMost = int64_t{1} << 32;
-    return rows / experts > 64 && static_cast<int64_t>(columns) * inner <= kMost && value_stride <= kMost / 256 && scale_stride <= kMost / 1024;
+    return rows / experts > 64 && experts < kMostSegments && columns <= 1 << 21 && static_cast<int64_t>(columns) * inner <= kMost &&
+           value_stride <= kMost / 256 && scale_stride <= kMost / 1024;
 }
 
 template <bool kGated, bool kExact>
@@ -654,7 +919,7 @@ int nanoep_experts_linear(const void* values, int64_t value_stride, const float*
         return NANOEP_ERR_INVALID_ARGUMENT;
     // up to 64 inner columns the 16-bit instructions take no longer than the one 128-wide 8-bit one
     if (inner > kScaleBlock / 2 && takes_tiles(rows, experts, inner, columns, value_stride, scale_stride))
-        return launch_tiles<8, 4, 2, 4, false>(p, out, columns, static_cast<hipStream_t>(stream));
+        return launch_tiles_by_rows<false>(p, out, static_cast<int64_t>(columns) * 2, static_cast<hipStream_t>(stream));
     if (inner <= kScaleBlock / 2)
         return launch_product<false, true>(p, out, columns, static_cast<hipStream_t>(stream));
     return launch_product<false, false>(p, out, columns, static_cast<hipStream_t>(stream));
@@ -686,7 +951,7 @@ int nanoep_experts_gated(const void* values, int64_t value_stride, const float* 
         return NANOEP_ERR_INVALID_ARGUMENT;
     const auto on = static_cast<hipStream_t>(stream);
     if (takes_tiles(rows, experts, inner, columns, value_stride, scale_stride))
-        return launch_tiles<8, 4, 2, 4, true>(p, records, record_bytes_of(columns / 2), on);
+        return launch_tiles_by_rows<true>(p, records, record_bytes_of(columns / 2), on);
     const int launched = launch_product<true, true>(p, workspace, columns / 2, on);
     if (launched != NANOEP_OK)
         return launched;

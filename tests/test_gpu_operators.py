@@ -236,6 +236,21 @@ def test_products_of_rows_beyond_32_bit_offsets(device):
         close(got[part], z, slack)
 
 
+def test_products_of_more_tiles_than_a_workgroup_lists(device):
+    # 66000 tiles of 256 rows; whole numbers, whose products and sums are exact whatever adds them
+    rows, inner, columns = 66_000 * 256 + 17, 128, 8
+    whole = torch.randint(-4, 5, (rows, inner), dtype=torch.int8, device=device)
+    values = torch.empty(rows, inner, dtype=torch.float8_e4m3fn, device=device)
+    for part in range(0, rows, 1 << 20):
+        values[part : part + (1 << 20)] = whole[part : part + (1 << 20)].to(torch.float8_e4m3fn)
+    scales = 2.0 ** torch.randint(-3, 4, (rows, 1), device=device)
+    weight = torch.randint(-4, 5, (1, columns, inner), generator=torch.Generator().manual_seed(6)).float()
+    got = ep.experts_linear(ep.Fp8Rows(values, scales), ep.Fp8Weight(weight.to(torch.float8_e4m3fn).to(device), torch.ones(1, 1, 1, device=device)))
+    for part in range(0, rows, 1 << 20):
+        z = (whole[part : part + (1 << 20)].float() @ weight[0].T.to(device)) * scales[part : part + (1 << 20)]
+        assert torch.equal(got[part : part + (1 << 20)], z.to(torch.bfloat16))
+
+
 # ------------------------------------------------------------------ weighted combine
 
 
