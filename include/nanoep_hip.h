@@ -78,6 +78,8 @@ int nanoep_device_topology(int* out_cus, int* out_xcds, int64_t* out_l2_bytes);
  *                     rows a token and the slot table; 1 = the one-token kernel)
  *   LAYOUT_LAUNCHES (0; 1 | 2 | 3: layout plan)  WINDOW_TOKENS (0; window of the slot-order list)
  *   RECALL_ORDER, FRESH_OUTPUTS, REBUILD_ORDER (-1; 0 | 1: host-extension policies)
+ *   EXPERTS_TILE (0: by size; 64 | 128 | 256 rows a tile of the experts' products, 1: their stream kernel; a gated product's
+ *                     workspace follows it)
  *   XCDS, L2_BYTES (0: ask the device)
  * nanoep_set_tuning / nanoep_get_tuning return NANOEP_ERR_INVALID_ARGUMENT for an unknown name;
  * nanoep_reset_tuning reads every switch from the environment again.

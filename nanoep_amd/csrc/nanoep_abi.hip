@@ -27,6 +27,7 @@ constexpr SwitchSlot kSwitches[] = {
     {"REBUILD_ORDER", &Tuning::rebuild_order},       {"XCDS", &Tuning::xcds},
     {"L2_BYTES", &Tuning::l2_bytes},                 {"DISPATCH_PREFETCH", &Tuning::dispatch_prefetch},
     {"COMBINE_STORES", &Tuning::combine_stores},     {"DISPATCH_PACK", &Tuning::dispatch_pack}, {"COMBINE_UNITS", &Tuning::combine_units},
+    {"EXPERTS_TILE", &Tuning::experts_tile},
 };
 constexpr int kSwitchCount = sizeof(kSwitches) / sizeof(kSwitches[0]);
 

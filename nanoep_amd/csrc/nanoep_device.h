@@ -99,6 +99,7 @@ struct Tuning {
     int fresh_outputs = -1;         // FRESH_OUTPUTS: 0 | 1 where a fresh dispatch's outputs are allocated (host extension)
     int rebuild_order = -1;         // REBUILD_ORDER: 0 | 1 never / always rebuild the private tensors of a seven-tensor handle
     int xcds = 0;                   // XCDS: number of XCDs the block remap assumes, 0 = ask the device
+    int experts_tile = 0;           // EXPERTS_TILE: 64 | 128 | 256 rows a tile of the experts' products, 1 = none (the stream kernel), 0 = by size
     int l2_bytes = 0;               // L2_BYTES: size of one XCD's L2 the windows are sized for, 0 = ask the device
 };
 

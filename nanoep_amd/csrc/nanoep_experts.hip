@@ -15,7 +15,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTile = 16;  // rows and columns of one matrix instruction's result
-constexpr int kUnitRows = 4;  // neighbouring row tiles whose column tiles an XCD works through together
+constexpr int kUnitRows = 4, kUnitCols = 8;  // neighbouring tiles that an XCD works on together
 
 struct Product {
     const char* values;  // rows of e4m3, value_stride bytes apart
@@ -34,12 +34,11 @@ struct Product {
     int column_blocks;
 };
 
-// What one workgroup computes: `live` rows from `row` on that are an expert's, then zeros up to `end`.
+// What one workgroup computes: `live` rows from `row` on that are an expert's.
 struct RowTile {
     int expert;  // -1: nothing
     int64_t row;
     int live;
-    int size;
 };
 
 // Segment e of the rows: [begin, end), the first `live` of which are the expert's.  The last one (e == experts) is
@@ -62,18 +61,17 @@ __device__ __forceinline__ Segment segment_of(const Product& p, int e) {
     return {begin, end, live};
 }
 
-// The `index`-th tile of kRows rows, counted over the segments: every wavefront finds it by a prefix sum over the
-// segments' tiles, 64 at a time.
+// The `index`-th tile of kRows rows, counted over the experts' rows: every wavefront finds it by a prefix sum over the
+// experts' tiles, 64 at a time.
 template <int kRows>
 __device__ __forceinline__ RowTile find_row_tile(const Product& p, int index) {
     const int lane = threadIdx.x % kWave;
-    const int segments = p.experts + (p.expert_offsets != nullptr ? 1 : 0);
     int before = 0;
-    for (int first = 0; first < segments; first += kWave) {
+    for (int first = 0; first < p.experts; first += kWave) {
         Segment segment = {0, 0, 0};
-        if (first + lane < segments)
+        if (first + lane < p.experts)
             segment = segment_of(p, first + lane);
-        const int tiles = static_cast<int>((segment.end - segment.begin + kRows - 1) / kRows);
+        const int tiles = static_cast<int>((segment.live + kRows - 1) / kRows);
         int through = tiles;
 #pragma unroll
         for (int step = 1; step < kWave; step *= 2) {
@@ -86,16 +84,50 @@ __device__ __forceinline__ RowTile find_row_tile(const Product& p, int index) {
             const int found = __ffsll(static_cast<long long>(behind)) - 1;
             // (row numbers fit 31 bits)
             const int begin = __builtin_amdgcn_readlane(static_cast<int>(segment.begin), found);
-            const int end = __builtin_amdgcn_readlane(static_cast<int>(segment.end), found);
             const int live = __builtin_amdgcn_readlane(static_cast<int>(segment.live), found);
             const int skipped = (index - before - __builtin_amdgcn_readlane(through - tiles, found)) * kRows;
-            const int size = end - begin - skipped, rows_live = live - skipped;
-            return {first + found, begin + skipped, rows_live < 0 ? 0 : rows_live > kRows ? kRows : rows_live, size > kRows ? kRows : size};
+            const int left = live - skipped;
+            return {first + found, begin + skipped, left > kRows ? kRows : left};
         }
         before += __builtin_amdgcn_readlane(through, kWave - 1);
     }
-    return {-1, 0, 0, 0};
+    return {-1, 0, 0};
 }
+
+// The rows of no expert, behind every expert's and behind the last segment, in kGapParts parts each: `part` of all
+// (experts + 1) * kGapParts, as rows [begin, end).
+constexpr int kGapParts = 8;
+struct RowRange {
+    int64_t begin;
+    int64_t end;
+};
+__device__ __forceinline__ RowRange gap_part(const Product& p, int part) {
+    if (part >= (p.experts + 1) * kGapParts)
+        return {0, 0};
+    const Segment segment = segment_of(p, part / kGapParts);
+    const int64_t begin = segment.begin + segment.live, rows = segment.end - begin;
+    return {begin + rows * (part % kGapParts) / kGapParts, begin + rows * (part % kGapParts + 1) / kGapParts};
+}
+
+// What a product's output holds in the rows [begin, end) of no expert: zeros, and in records the scale of a group of zeros.
+template <bool kRecords, int kThreads, int kValueBytes = 2>
+__device__ __forceinline__ void clear_rows(char* out, int64_t stride, int columns, RowRange rows) {
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    const int groups = (columns + kScaleBlock - 1) / kScaleBlock;
+    const float scale = group_scale(0).scale;
+    for (int64_t row = rows.begin; row < rows.end; ++row) {
+        char* at = out + row * stride;
+        if constexpr (kRecords) {
+            // (a record is a multiple of 512 bytes; its scales are words of it)
+            for (int word = threadIdx.x; word < static_cast<int>(stride / 4); word += kThreads)
+                reinterpret_cast<uint32_t*>(at)[word] = word >= columns / 4 && word < columns / 4 + groups ? __float_as_uint(scale) : 0u;
+        } else {
+            for (int vector = threadIdx.x; vector < columns / (16 / kValueBytes); vector += kThreads)
+                reinterpret_cast<u32x4*>(at)[vector] = zero;
+        }
+    }
+}
+
 
 __device__ __forceinline__ i32x8 operand(const u32x4 low, const u32x4 high) {
     return {static_cast<int>(low.x), static_cast<int>(low.y), static_cast<int>(low.z), static_cast<int>(low.w),
@@ -134,21 +166,70 @@ __device__ __forceinline__ f32x4 block_product(const i32x8 weight, const i32x8 r
 
 __device__ __forceinline__ float silu(float v) { return v / (1.0f + __expf(-v)); }
 
-// Products of few rows with much weight: every wavefront streams its weights from memory straight into registers.
-// A workgroup computes kColumns * 16 columns of kRows * 16 rows; its four wavefronts take every fourth block of 128
-// inner columns, sum the blocks' products, each times its two scales, in fp32 registers, and add their sums through LDS.
-// A gated product takes half of its column tiles from the gate and half from the up weights.
-template <int kColumns, int kRows, bool kGated, bool kExact>
-__global__ void __launch_bounds__(kBlockThreads) experts_stream_kernel(const Product p, void* __restrict__ out, int64_t out_stride) {
-    __shared__ f32x4 sums[kWavesPerBlock][kColumns * kRows][kWave];
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)(p)));
+}
+
+// Copies 16 (kBytes == 16) or 4 bytes a lane from memory into LDS without registers on the way: lane l's go to
+// `to` + l * kBytes.  `to` and `from` are wave-uniform, `offset` is a lane's own.  Waits are the caller's, by counting.
+template <int kBytes>
+__device__ __forceinline__ void load_to_lds(const char* from, uint32_t offset, uint32_t to) {
+    if constexpr (kBytes == 16)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(from) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(from) : "memory");
+}
+
+// The same with a whole address of each lane's own.
+template <int kBytes>
+__device__ __forceinline__ void load_to_lds(const char* from, uint32_t to) {
+    if constexpr (kBytes == 16)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "memory");
+}
+
+// What is read in the place of a piece that lies past its row's end.
+__device__ const u32x4 kZeroPiece = {0u, 0u, 0u, 0u};
+
+// Waits until all but the newest kNewer of this wavefront's loads are done, and its reads of LDS.
+template <int kNewer>
+__device__ __forceinline__ void loaded_but_newest() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kNewer) : "memory");
+}
+
+// ------------------------------------------------------------------ few rows an expert
+
+// Products of few rows with much weight: what counts is that HBM is kept busy.  A workgroup computes kColumns * 16 columns of
+// kRows * 16 rows; its four wavefronts take every fourth block of 128 inner columns, sum the blocks' products, each
+// times its two scales, in fp32 registers, and add their sums through LDS.  Each wavefront has a ring of kDepth blocks' operands in
+// LDS of its own, filled straight from memory, whole 128-byte lines at a time, and needs no barrier to read it: kDepth - 1
+// blocks are on their way.  (Two blocks' operands in registers, loaded there in their layout, took the same time on one token's
+// eight experts; what is left there is the workgroups' start, their sums and the scales' launch.)  A gated product takes half of its column tiles from the gate and half from the up weights.
+template <int kColumns, int kRows, int kDepth, bool kGated, bool kExact>
+__global__ void __launch_bounds__(kBlockThreads) experts_stream_kernel(const Product p, void* __restrict__ out, int64_t out_stride, int row_tiles) {
+    constexpr int kTileBytes = kTile * kScaleBlock;
+    constexpr int kScalesAt = (kColumns + kRows) * kTileBytes, kBlockBytes = kScalesAt + kWave * 4;
+    constexpr int kLoads = 2 * (kColumns + kRows) + 1;  // of a block
+    constexpr int kSumBytes = kColumns * kRows * kWave * 16;
+    constexpr int kWaveBytes = kDepth * kBlockBytes > kSumBytes ? kDepth * kBlockBytes : kSumBytes;
+    static_assert(kRows * kTile <= kWave && (kDepth - 1) * kLoads < 64);
+    __shared__ __attribute__((aligned(1024))) char memory[kWavesPerBlock][kWaveBytes];
+    constexpr int kOutTiles = kGated ? kColumns / 2 : kColumns;
+    const int out_columns = kGated ? p.columns / 2 : p.columns;
+    if (static_cast<int>(blockIdx.x) >= row_tiles) {
+        // workgroups of their own for the rows of no expert
+        constexpr int kValueBytes = kGated ? 4 : 2;
+        clear_rows<false, kBlockThreads, kValueBytes>(static_cast<char*>(out), out_stride * kValueBytes, out_columns,
+                                                      gap_part(p, static_cast<int>((blockIdx.x - row_tiles) * gridDim.y + blockIdx.y)));
+        return;
+    }
     const RowTile tile = find_row_tile<kRows * kTile>(p, static_cast<int>(blockIdx.x));
     if (tile.expert < 0)
         return;
     const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int group = lane / kTile, in_tile = lane % kTile;
-    constexpr int kOutTiles = kGated ? kColumns / 2 : kColumns;
-    const int out_columns = kGated ? p.columns / 2 : p.columns;
     const int first_column = static_cast<int>(blockIdx.y) * kOutTiles * kTile;
 
     f32x4 acc[kColumns][kRows];
@@ -158,90 +239,132 @@ __global__ void __launch_bounds__(kBlockThreads) experts_stream_kernel(const Pro
         for (int r = 0; r < kRows; ++r)
             acc[c][r] = {0.0f, 0.0f, 0.0f, 0.0f};
 
-    if (tile.live > 0) {
-        // rows and columns past the end are clamped to the last one: what they give is not written
-        const char* weight_rows[kColumns];
+    {
+        // A lane's part of a load: row lane / 8 of its eight and, of that row, a 16-byte piece that is turned by the row, and with
+        // it its place in LDS, so that the same piece of eight rows, which an operand reads at once, lies in different banks.
+        // Rows and columns past the end are the last one again: what they give is not written.
+        const int piece = (lane % 8) ^ (lane / 8);
+        const char* weight = p.weight + static_cast<int64_t>(tile.expert) * p.columns * p.inner;
+        const char* values = p.values + tile.row * p.value_stride;
+        const char* scales = reinterpret_cast<const char*>(p.scales + tile.row * p.scale_stride);
+        const char* weight_rows[kColumns][2];
+        const char* value_rows[kRows][2];
         const float* weight_scales[kColumns];
 #pragma unroll
         for (int c = 0; c < kColumns; ++c) {
-            const int out_tile = c % kOutTiles;
             const int base = (c / kOutTiles) * out_columns;
-            int column = first_column + out_tile * kTile;
-            const int block_column = column < out_columns ? column : out_columns - 1;
-            column += in_tile;
-            column = base + (column < out_columns ? column : out_columns - 1);
-            weight_rows[c] = p.weight + (static_cast<int64_t>(tile.expert) * p.columns + column) * p.inner;
-            weight_scales[c] = p.weight_scales + (static_cast<int64_t>(tile.expert) * p.column_blocks + (base + block_column) / kScaleBlock) * p.blocks;
-        }
-        const char* value_rows[kRows];
-        const float* row_scales[kRows];
+            const int column = first_column + c % kOutTiles * kTile;
+            weight_scales[c] = p.weight_scales +
+                               (static_cast<int64_t>(tile.expert) * p.column_blocks + (base + (column < out_columns ? column : out_columns - 1)) / kScaleBlock) * p.blocks;
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-            const int in_live = r * kTile + in_tile;
-            const int64_t row = tile.row + (in_live < tile.live ? in_live : tile.live - 1);
-            value_rows[r] = p.values + row * p.value_stride;
-            row_scales[r] = p.scales + row * p.scale_stride;
-        }
-        for (int block = wave; block < p.blocks; block += kWavesPerBlock) {
-            const int at = block * kScaleBlock + group * 16;
-            // the last block may end early: 16 bytes past its end are zeros on both sides
-            const bool low_in = at < p.inner, high_in = at + 64 < p.inner;
-            const int low_at = low_in ? at : 0, high_at = high_in ? at + 64 : 0;
-            const u32x4 zero = {0u, 0u, 0u, 0u};
-            i32x8 rows[kRows];
-            float scale[kRows];
-#pragma unroll
-            for (int r = 0; r < kRows; ++r) {
-                const u32x4 low = *reinterpret_cast<const u32x4*>(value_rows[r] + low_at);
-                const u32x4 high = *reinterpret_cast<const u32x4*>(value_rows[r] + high_at);
-                rows[r] = operand(low_in ? low : zero, high_in ? high : zero);
-                scale[r] = row_scales[r][block];
+            for (int half = 0; half < 2; ++half) {
+                const int row = column + half * 8 + lane / 8;
+                weight_rows[c][half] = weight + static_cast<int64_t>(base + (row < out_columns ? row : out_columns - 1)) * p.inner;
             }
+        }
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int row = r * kTile + half * 8 + lane / 8;
+                value_rows[r][half] = values + (row < tile.live ? row : tile.live - 1) * p.value_stride;
+            }
+        const char* scale_row = scales + (lane < tile.live ? lane : tile.live - 1) * p.scale_stride * 4;
+        const uint32_t ring = lds_address(memory[wave]);
+
+        const auto fetch = [&](int block, int slot) {
+            const int at = block * kScaleBlock + piece * 16;
+            const uint32_t to = ring + slot * kBlockBytes;
+#pragma unroll
+            for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+                    load_to_lds<16>(at < p.inner ? weight_rows[c][half] + at : reinterpret_cast<const char*>(&kZeroPiece),
+                                    to + c * kTileBytes + half * (kTileBytes / 2));
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+                    load_to_lds<16>(at < p.inner ? value_rows[r][half] + at : reinterpret_cast<const char*>(&kZeroPiece),
+                                    to + (kColumns + r) * kTileBytes + half * (kTileBytes / 2));
+            load_to_lds<4>(scale_row + block * 4, to + kScalesAt);
+        };
+        const int turned = in_tile * kScaleBlock + (group ^ (lane & 7)) * 16;
+        const auto multiply = [&](int block, int slot) {
+            const char* from = memory[wave] + slot * kBlockBytes;
+            const auto operand_at = [&](int at) {
+                return operand(*reinterpret_cast<const u32x4*>(from + at + turned), *reinterpret_cast<const u32x4*>(from + at + (turned ^ 64)));
+            };
+            i32x8 weights[kColumns];
+            float weight_scale[kColumns];
 #pragma unroll
             for (int c = 0; c < kColumns; ++c) {
-                const u32x4 low = *reinterpret_cast<const u32x4*>(weight_rows[c] + low_at);
-                const u32x4 high = *reinterpret_cast<const u32x4*>(weight_rows[c] + high_at);
-                const i32x8 weight = operand(low_in ? low : zero, high_in ? high : zero);
-                const float weight_scale = weight_scales[c][block];
+                weights[c] = operand_at(c * kTileBytes);
+                weight_scale[c] = uniform_load(weight_scales[c] + block);
+            }
 #pragma unroll
-                for (int r = 0; r < kRows; ++r) {
-                    const f32x4 product = block_product<kExact>(weight, rows[r]);
-                    const float factor = weight_scale * scale[r];
+            for (int r = 0; r < kRows; ++r) {
+                const i32x8 row = operand_at((kColumns + r) * kTileBytes);
+                const float row_scale = reinterpret_cast<const float*>(from + kScalesAt)[r * kTile + in_tile];
+#pragma unroll
+                for (int c = 0; c < kColumns; ++c) {
+                    const f32x4 product = block_product<kExact>(weights[c], row);
+                    const float factor = weight_scale[c] * row_scale;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         acc[c][r][i] = fmaf(factor, product[i], acc[c][r][i]);
                 }
             }
+        };
+        // this wavefront's blocks: wave, wave + 4, ...
+        const int count = (p.blocks - wave + kWavesPerBlock - 1) / kWavesPerBlock;
+#pragma unroll
+        for (int n = 0; n < kDepth - 1; ++n)
+            if (n < count)
+                fetch(wave + n * kWavesPerBlock, n);
+        int slot = 0;
+        for (int n = 0; n < count; ++n) {
+            // (the slot that is filled is the one the last turn read: its reads are done)
+            if (n + kDepth - 1 < count) {
+                loaded_but_newest<(kDepth - 2) * kLoads>();
+                fetch(wave + (n + kDepth - 1) * kWavesPerBlock, slot == 0 ? kDepth - 1 : slot - 1);
+            } else {
+                loaded_but_newest<0>();
+            }
+            multiply(wave + n * kWavesPerBlock, slot);
+            slot = slot + 1 == kDepth ? 0 : slot + 1;
         }
     }
+    // the ring's memory takes the sums
+    f32x4* const sums = reinterpret_cast<f32x4*>(memory[0]);
+    constexpr int kWaveSums = kWaveBytes / 16;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
     for (int c = 0; c < kColumns; ++c)
 #pragma unroll
         for (int r = 0; r < kRows; ++r)
-            sums[wave][c * kRows + r][lane] = acc[c][r];
+            sums[wave * kWaveSums + (c * kRows + r) * kWave + lane] = acc[c][r];
     __syncthreads();
     for (int item = wave; item < kOutTiles * kRows; item += kWavesPerBlock) {
         const int c = item / kRows, r = item % kRows;
-        f32x4 total = sums[0][c * kRows + r][lane];
+        f32x4 total = sums[(c * kRows + r) * kWave + lane];
 #pragma unroll
         for (int w = 1; w < kWavesPerBlock; ++w)
-            total += sums[w][c * kRows + r][lane];
+            total += sums[w * kWaveSums + (c * kRows + r) * kWave + lane];
         if constexpr (kGated) {
             const int up_at = (c + kOutTiles) * kRows + r;
-            f32x4 up = sums[0][up_at][lane];
+            f32x4 up = sums[up_at * kWave + lane];
 #pragma unroll
             for (int w = 1; w < kWavesPerBlock; ++w)
-                up += sums[w][up_at][lane];
+                up += sums[w * kWaveSums + up_at * kWave + lane];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 total[i] = silu(total[i]) * up[i];
         }
         const int in_size = r * kTile + in_tile;
         const int column = first_column + c * kTile + group * 4;
-        if (in_size >= tile.size || column >= out_columns)
+        if (in_size >= tile.live || column >= out_columns)
             continue;
-        if (in_size >= tile.live)
-            total = {0.0f, 0.0f, 0.0f, 0.0f};
         const int64_t at = (tile.row + in_size) * out_stride + column;
         if constexpr (kGated) {
             *reinterpret_cast<f32x4*>(static_cast<float*>(out) + at) = total;
@@ -255,28 +378,6 @@ __global__ void __launch_bounds__(kBlockThreads) experts_stream_kernel(const Pro
 }
 
 // ------------------------------------------------------------------ many rows an expert
-
-__device__ __forceinline__ uint32_t lds_address(const void* p) {
-    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)(p)));
-}
-
-// Copies 16 (kBytes == 16) or 4 bytes a lane from memory into LDS without registers on the way: lane l's go to
-// `to` + l * kBytes.  `to` and `from` are wave-uniform, `offset` is a lane's own.  Only all_but_newest() waits for it.
-template <int kBytes>
-__device__ __forceinline__ void load_to_lds(const char* from, uint32_t offset, uint32_t to) {
-    if constexpr (kBytes == 16)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(from) : "memory");
-    else
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(from) : "memory");
-}
-
-// The same with a whole address of each lane's own.
-__device__ __forceinline__ void load_to_lds(const char* from, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
-}
-
-// What is read in the place of a piece that lies past its row's end.
-__device__ const u32x4 kZeroPiece = {0u, 0u, 0u, 0u};
 
 // The same number, which the compiler takes for another: what is computed from it is computed where it is
 // needed, and holds no registers over the loops around that place.
@@ -314,7 +415,7 @@ struct TileShape {
 struct Item {
     int expert;
     int row;
-    int live_size;  // live rows, and those that are written, above them (at most 256 each)
+    int live;  // rows, at most the tile's
     int column_tile;
 };
 
@@ -328,14 +429,14 @@ constexpr int kMostSegments = 1 << 14;  // segments whose prefix sums fit the me
 template <int kRows, int kThreads>
 __device__ __forceinline__ int list_tiles(const Product& p, int column_tiles, uint32_t xcd, uint32_t on_xcd, uint32_t xcds, uint32_t unit, int first,
                                           int* before, int* wave_sums, Item* items) {
-    const int segments = p.experts + (p.expert_offsets != nullptr ? 1 : 0);
+    const int segments = p.experts;
     const int each = (segments + kThreads - 1) / kThreads;
     const int from = static_cast<int>(threadIdx.x) * each;
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     int mine = 0;
     for (int e = from; e < from + each && e < segments; ++e) {
         const Segment segment = segment_of(p, e);
-        mine += static_cast<int>((segment.end - segment.begin + kRows - 1) / kRows);
+        mine += static_cast<int>((segment.live + kRows - 1) / kRows);
     }
     int through = mine;
 #pragma unroll
@@ -357,7 +458,7 @@ __device__ __forceinline__ int list_tiles(const Product& p, int column_tiles, ui
     for (int e = from; e < from + each && e < segments; ++e) {
         const Segment segment = segment_of(p, e);
         before[e] = at;
-        at += static_cast<int>((segment.end - segment.begin + kRows - 1) / kRows);
+        at += static_cast<int>((segment.live + kRows - 1) / kRows);
     }
     lds_settled();
     const uint32_t tiles = static_cast<uint32_t>(total) * static_cast<uint32_t>(column_tiles);
@@ -380,14 +481,10 @@ __device__ __forceinline__ int list_tiles(const Product& p, int column_tiles, ui
         }
         const Segment segment = segment_of(p, low);
         const int skipped = (row_tile - before[low]) * kRows;
-        const int size = static_cast<int>(segment.end - segment.begin) - skipped, live = static_cast<int>(segment.live) - skipped;
-        // (a layout whose segments lie over one another may number more tiles than fit an int: no tile then)
-        if (skipped < 0 || size <= 0) {
-            items[i] = {0, 0, 0, 0};
-            continue;
-        }
-        items[i] = {low, static_cast<int>(segment.begin) + skipped, (live < 0 ? 0 : live > kRows ? kRows : live) | (size > kRows ? kRows : size) << 16,
-                    static_cast<int>(in_group / group_rows)};
+        const int live = static_cast<int>(segment.live) - skipped;
+        // (a layout whose segments lie over one another may number more tiles than fit an int: one row then, of some expert's)
+        items[i] = skipped < 0 || live <= 0 ? Item{0, 0, 1, 0}
+                                            : Item{low, static_cast<int>(segment.begin) + skipped, live > kRows ? kRows : live, static_cast<int>(in_group / group_rows)};
     }
     lds_settled();
     const uint64_t start = (static_cast<uint64_t>(first) * xcds + xcd) * unit + on_xcd;
@@ -412,7 +509,7 @@ __device__ __forceinline__ int list_tiles(const Product& p, int column_tiles, ui
 // loads alone 1.36 us: 64 KB that L2 hands out in 64-byte requests, of which a block of all tiles needs about as many
 // clocks as its matrix instructions.  One block's time ahead for the weights, the loads alone took 1.76 us.
 template <int kRowTiles, int kColTiles, int kRowWaves, int kColWaves, bool kGated>
-__global__ void __launch_bounds__(kRowWaves * kColWaves * kWave)
+__global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
     experts_tile_kernel(const Product p, char* __restrict__ out, int64_t out_stride, int column_tiles, XcdMap xcds) {
     using Shape = TileShape<kRowTiles, kColTiles, kRowWaves, kColWaves, kGated>;
     constexpr int kWeightBytes = Shape::kCols * kScaleBlock, kRowBytes = Shape::kRows * kScaleBlock;
@@ -448,21 +545,25 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave)
         const auto item_at = [&](int i) -> Item {
             const Item item = items[i];
             return {__builtin_amdgcn_readfirstlane(item.expert), __builtin_amdgcn_readfirstlane(item.row),
-                    __builtin_amdgcn_readfirstlane(item.live_size), __builtin_amdgcn_readfirstlane(item.column_tile)};
-        };
-        const auto next_live = [&](int i) {
-            while (i < count && (__builtin_amdgcn_readfirstlane(items[i].live_size) & 0xffff) == 0)
-                ++i;
-            return i;
+                    __builtin_amdgcn_readfirstlane(item.live), __builtin_amdgcn_readfirstlane(item.column_tile)};
         };
 
+        // Tiles begin at different blocks and go round.  All of a block's weights are a weight row's length apart, which for a
+        // length like 4096 is on a few of the memory's channels; with all workgroups at the same block, the 256-token decode step
+        // took 279 us, so 228.  Tiles that one XCD works on together share their rows, and so begin together.
+        const auto first_block = [&](const Item& item) {
+            const uint32_t turned = static_cast<uint32_t>(item.expert) * 7 + static_cast<uint32_t>(item.column_tile / kUnitCols) * 5;
+            return static_cast<int>(turned % static_cast<uint32_t>(p.blocks));
+        };
         // the weights' cursor
-        int weight_item = next_live(0), weight_block = 0, weight_slot = 0;
+        int weight_item = 0, weight_block = 0, weight_left = 0, weight_slot = 0;
         const char* weight = nullptr;
         uint32_t weight_offset[Shape::kWeightLoads];
         const auto aim_weights = [&]() {
             const Item item = item_at(weight_item);
             weight = p.weight + static_cast<int64_t>(item.expert) * p.columns * p.inner;
+            weight_block = first_block(item);
+            weight_left = p.blocks;
             const int first_column = item.column_tile * Shape::kOutCols;
             const int row_in_load = afresh(lane) / 8;
 #pragma unroll
@@ -494,13 +595,14 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave)
             } else {
 #pragma unroll
                 for (int i = 0; i < Shape::kWeightLoads; ++i)
-                    load_to_lds(at + piece * 16 < p.inner ? weight + at + weight_offset[i] + piece * 16 : reinterpret_cast<const char*>(&kZeroPiece),
+                    load_to_lds<16>(at + piece * 16 < p.inner ? weight + at + weight_offset[i] + piece * 16 : reinterpret_cast<const char*>(&kZeroPiece),
                                 to + i * kStep);
             }
             weight_slot ^= 1;
-            if (++weight_block == p.blocks) {
+            if (++weight_block == p.blocks)
                 weight_block = 0;
-                weight_item = next_live(weight_item + 1);
+            if (--weight_left == 0) {
+                ++weight_item;
                 if (weight_item < count)
                     aim_weights();
             }
@@ -508,12 +610,14 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave)
         };
 
         // the rows' cursor; rows past the live ones are the last one again, and what they give is not written
-        int row_item = weight_item, row_block = 0, row_slot = 0;
+        int row_item = weight_item, row_block = 0, row_left = 0, row_slot = 0;
         const char *values = nullptr, *scales = nullptr;
         uint32_t row_offset[Shape::kRowLoads], scale_offset = 0;
         const auto aim_rows = [&]() {
             const Item item = item_at(row_item);
-            const int live = item.live_size & 0xffff;
+            const int live = item.live;
+            row_block = first_block(item);
+            row_left = p.blocks;
             values = p.values + static_cast<int64_t>(item.row) * p.value_stride;
             scales = reinterpret_cast<const char*>(p.scales + static_cast<int64_t>(item.row) * p.scale_stride);
             const int row_in_load = afresh(lane) / 8;
@@ -537,15 +641,16 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave)
             } else {
 #pragma unroll
                 for (int i = 0; i < Shape::kRowLoads; ++i)
-                    load_to_lds(at + piece * 16 < p.inner ? values + at + row_offset[i] + piece * 16 : reinterpret_cast<const char*>(&kZeroPiece),
+                    load_to_lds<16>(at + piece * 16 < p.inner ? values + at + row_offset[i] + piece * 16 : reinterpret_cast<const char*>(&kZeroPiece),
                                 to + i * kStep);
             }
             // (where there are more wavefronts than 64 rows, some bring in the same scales)
             load_to_lds<4>(scales + static_cast<int64_t>(row_block) * 4, scale_offset, scales_at + row_slot * Shape::kRows * 4);
             row_slot ^= 1;
-            if (++row_block == p.blocks) {
+            if (++row_block == p.blocks)
                 row_block = 0;
-                row_item = next_live(row_item + 1);
+            if (--row_left == 0) {
+                ++row_item;
                 if (row_item < count)
                     aim_rows();
             }
@@ -595,11 +700,15 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave)
                 read_weights(0, c);
             read_rows(0, 0, 0);
         }
+        // the rows of no expert, while the first operands are on their way
+        if (listed == 0 && p.expert_offsets != nullptr)
+            for (int part = static_cast<int>(blockIdx.x); part < (p.experts + 1) * kGapParts; part += static_cast<int>(gridDim.x))
+                clear_rows<kGated, Shape::kThreads>(out, out_stride, out_columns, gap_part(p, part));
         bool weights_ahead = false;
         bool stored = false;  // the newest accesses are a tile's stores
         for (int i = 0; i < count; ++i) {
             const Item item = item_at(i);
-            const int live = item.live_size & 0xffff, size = item.live_size >> 16;
+            const int live = item.live;
             const int first_column = item.column_tile * Shape::kOutCols;
             f32x4 acc[kColTiles][kRowTiles];
 #pragma unroll
@@ -608,7 +717,7 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave)
                 for (int r = 0; r < kRowTiles; ++r)
                     acc[c][r] = {0.0f, 0.0f, 0.0f, 0.0f};
 
-            if (live > 0) {
+            {
                 // the scales of this wavefront's column tiles: one where they are neighbours within 128 columns
                 constexpr int kScales = kGated ? kColTiles : 1;
                 static_assert(kGated || kScaleBlock % (kColTiles * kTile) == 0);
@@ -621,11 +730,13 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave)
                     int column = first_column + (col_wave * kOutTiles + c % kOutTiles) * kTile;
                     column = (column < out_columns ? column : out_columns - 1) + (c / kOutTiles) * out_columns;
                     weight_scales[c] = p.weight_scales + (static_cast<int64_t>(item.expert) * p.column_blocks + column / kScaleBlock) * p.blocks;
-                    next_scale[c] = uniform_load(weight_scales[c]);
+                    next_scale[c] = uniform_load(weight_scales[c] + first_block(item));
                 }
-                for (int block = 0; block < p.blocks; ++block) {
+                int block = first_block(item);
+                for (int turn = 0; turn < p.blocks; ++turn) {
                     float column_scale[kScales];
-                    const int next_block = block + 1 < p.blocks ? block + 1 : block;
+                    block = block + 1 < p.blocks ? block + 1 : 0;
+                    const int next_block = block;
 #pragma unroll
                     for (int c = 0; c < kScales; ++c) {
                         column_scale[c] = next_scale[c];
@@ -701,7 +812,7 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave)
             const int first_row = row_wave * kRowTiles * kTile + out_lane % kTile;
             constexpr uint32_t kNowhere = 0xffffffffu;
             char* tile_out = out + item.row * out_stride;
-            const __amdgpu_buffer_rsrc_t tile_rows = __builtin_amdgcn_make_buffer_rsrc(tile_out, 0, static_cast<int>(size * out_stride), 0x00020000);
+            const __amdgpu_buffer_rsrc_t tile_rows = __builtin_amdgcn_make_buffer_rsrc(tile_out, 0, static_cast<int>(live * out_stride), 0x00020000);
             if constexpr (!kGated) {
 #pragma unroll
                 for (int r = 0; r < kRowTiles; ++r) {
@@ -710,7 +821,7 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave)
 #pragma unroll
                     for (int c = 0; c < kColTiles; ++c) {
                         const int column = first_column + (col_wave * kColTiles + c) * kTile + in_group * 4;
-                        const f32x4 v = in_rows < live ? acc[c][r] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                        const f32x4 v = acc[c][r];
                         const u32x2 packed = {to_bf16_pair(v[0], v[1]), to_bf16_pair(v[2], v[3])};
                         __builtin_amdgcn_raw_buffer_store_b64(packed, tile_rows, column < out_columns ? row + column * 2 : kNowhere, 0, 0);
                     }
@@ -748,9 +859,9 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave)
                     const GroupScale scale = group_scale(amax);
                     const uint32_t row = static_cast<uint32_t>(in_rows) * static_cast<uint32_t>(out_stride);
                     // the scale, and the record's padding with its last group
-                    if (col_wave == 0 && in_group == 0 && in_rows < size)
+                    if (col_wave == 0 && in_group == 0 && in_rows < live)
                         reinterpret_cast<float*>(tile_out + row + out_columns)[item.column_tile] = scale.scale;
-                    if (item.column_tile == column_tiles - 1 && col_wave == kColWaves - 1 && in_rows < size)
+                    if (item.column_tile == column_tiles - 1 && col_wave == kColWaves - 1 && in_rows < live)
                         for (int word = out_columns / 4 + column_tiles + in_group; word < static_cast<int>(out_stride / 4); word += 4)
                             reinterpret_cast<uint32_t*>(tile_out + row)[word] = 0u;
 #pragma unroll
@@ -837,21 +948,20 @@ int product_of(const void* values, int64_t value_stride, const float* scales, in
     return NANOEP_OK;
 }
 
-// Most tiles of kRows rows that the segments can have: each but the full ones ends in one that is not.
-int64_t most_row_tiles(const Product& p, int rows) {
-    const int64_t segments = p.expert_offsets != nullptr ? p.experts + int64_t{1} : 1;
-    return p.rows / rows + (segments < p.rows ? segments : p.rows);
-}
+// Most tiles of kRows rows that the experts' rows can have: each expert's but the full ones end in one that is not.
+int64_t most_row_tiles(const Product& p, int rows) { return p.rows / rows + (p.experts < p.rows ? p.experts : p.rows); }
 
-template <int kColumns, int kRows, bool kGated, bool kExact>
+template <int kColumns, int kRows, int kDepth, bool kGated, bool kExact>
 int launch_stream(const Product& p, void* out, int64_t out_stride, hipStream_t stream) {
     const int out_columns = kGated ? p.columns / 2 : p.columns;
     constexpr int kOutColumns = (kGated ? kColumns / 2 : kColumns) * kTile;
     const int64_t tiles = most_row_tiles(p, kRows * kTile), column_tiles = (out_columns + kOutColumns - 1) / kOutColumns;
-    if (tiles > 0x7fffffff || column_tiles > 65535)
+    const int64_t gaps = p.expert_offsets != nullptr ? ((p.experts + int64_t{1}) * kGapParts + column_tiles - 1) / column_tiles : 0;
+    if (tiles + gaps > 0x7fffffff || column_tiles > 65535)
         return NANOEP_ERR_INVALID_ARGUMENT;
-    experts_stream_kernel<kColumns, kRows, kGated, kExact>
-        <<<dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(column_tiles)), kBlockThreads, 0, stream>>>(p, out, out_stride);
+    experts_stream_kernel<kColumns, kRows, kDepth, kGated, kExact>
+        <<<dim3(static_cast<unsigned>(tiles + gaps), static_cast<unsigned>(column_tiles)), kBlockThreads, 0, stream>>>(p, out, out_stride,
+                                                                                                                      static_cast<int>(tiles));
     NANOEP_HIP_TRY(hipGetLastError());
     return NANOEP_OK;
 }
@@ -873,32 +983,60 @@ int launch_tiles(const Product& p, void* out, int64_t out_stride, hipStream_t st
     return NANOEP_OK;
 }
 
-// Tiles of 256 rows, of 128 where an expert has fewer rows than that on average.  Of 32 experts, 2048 -> 7168: 115 rows
-// each 136 us with 128-row tiles and 175 with 256-row ones, 230 rows 207 and 202 (gated, 7168 -> 2048: 580 and 626), 460 rows 355
-// and 338 (gated 973 and 891).
-template <bool kGated>
-int launch_tiles_by_rows(const Product& p, void* out, int64_t out_stride, hipStream_t stream) {
-    if (p.rows / p.experts > 256)
-        return launch_tiles<8, 4, 2, 4, kGated>(p, out, out_stride, stream);
-    return launch_tiles<4, 4, 2, 4, kGated>(p, out, out_stride, stream);
-}
-
-// Whether the tile kernel takes a product: enough rows an expert, no more experts than its list of tiles is made from, and an
-// expert's weight and a tile's rows, in and out, within the 32-bit offsets it addresses them with.
-bool takes_tiles(int64_t rows, int64_t experts, int inner, int columns, int64_t value_stride, int64_t scale_stride) {
+// Rows of the tile kernel's tiles for a product, 0 for the stream kernel.
+//   The tile follows the rows an expert has on average.  Of 32 experts, 2048 -> 7168: 58 rows each 127 us with 64-row tiles and 128 with
+//   128-row ones (gated, 7168 -> 2048: 261 and 281), 115 rows 158, 136 and, with 256-row tiles, 175 us, 230 rows 207 (128) and 202 us
+//   (256; gated 580 and 626), 460 rows 355 and 338 us (gated 973 and 891).
+//   Smaller tiles, where the larger ones do not go round the compute units.
+//   The stream kernel, whose wavefronts share out the inner columns, where the smallest do not either: one token's eight experts,
+//   gated, 7168 -> 2048, 47 us against 93; 115 rows of 128 experts, 768 -> 2048, 42 us against 29 with 64-row tiles.
+//   And for addresses beyond the tile kernel's: an expert's weight and a tile's rows, in and out, lie within 32-bit offsets, its list
+//   of tiles is made from at most kMostSegments experts.
+int tile_rows(int64_t rows, int64_t experts, int inner, int columns, int out_columns_each, int out_columns, int64_t value_stride, int64_t scale_stride) {
     constexpr int64_t kMost = int64_t{1} << 32;
-    return rows / experts > 64 && experts < kMostSegments && columns <= 1 << 21 && static_cast<int64_t>(columns) * inner <= kMost &&
-           value_stride <= kMost / 256 && scale_stride <= kMost / 1024;
+    if (experts >= kMostSegments || columns > 1 << 21 || static_cast<int64_t>(columns) * inner > kMost || value_stride > kMost / 256 ||
+        scale_stride > kMost / 1024)
+        return 0;
+    const Tuning tuning = current_tuning();
+    if (tuning.experts_tile != 0)
+        return tuning.experts_tile == 64 || tuning.experts_tile == 128 || tuning.experts_tile == 256 ? tuning.experts_tile : 0;
+    const int64_t cus = current_topology(tuning).cus;
+    const int64_t each = rows / experts, column_tiles = (out_columns + out_columns_each - 1) / out_columns_each;
+    const int64_t owners = experts < rows ? experts : rows;
+    for (const int tile : {256, 128, 64}) {
+        const bool suits = tile == 64 || each > tile;
+        if (suits && (rows / tile > owners ? rows / tile : owners) * column_tiles >= cus)
+            return tile;
+    }
+    return 0;
 }
 
+template <bool kGated>
+int launch_product(const Product& p, void* out, int64_t out_stride, int tile, hipStream_t stream) {
+    if (tile == 256)
+        return launch_tiles<8, 4, 2, 4, kGated>(p, out, out_stride, stream);
+    if (tile == 128)
+        return launch_tiles<4, 4, 2, 4, kGated>(p, out, out_stride, stream);
+    return launch_tiles<2, 4, 2, 4, kGated>(p, out, out_stride, stream);
+}
+
+// `out_stride` in values: bf16 ones, or a gated product's fp32 ones.
 template <bool kGated, bool kExact>
-int launch_product(const Product& p, void* out, int64_t out_stride, hipStream_t stream) {
-    const int64_t rows_each = p.rows / p.experts;
-    if (rows_each <= 16)
-        return launch_stream<2, 1, kGated, kExact>(p, out, out_stride, stream);
-    if (rows_each <= 32)
-        return launch_stream<2, 2, kGated, kExact>(p, out, out_stride, stream);
-    return launch_stream<4, 4, kGated, kExact>(p, out, out_stride, stream);
+int launch_streams(const Product& p, void* out, int64_t out_stride, hipStream_t stream) {
+    if (p.rows / p.experts <= 16)
+        return launch_stream<2, 1, 3, kGated, kExact>(p, out, out_stride, stream);
+    return launch_stream<2, 4, 2, kGated, kExact>(p, out, out_stride, stream);
+}
+
+int linear_tile_rows(const Product& p) {
+    // up to 64 inner columns the 16-bit instructions take no longer than the one 128-wide 8-bit one
+    if (p.inner <= kScaleBlock / 2)
+        return 0;
+    return tile_rows(p.rows, p.experts, p.inner, p.columns, TileShape<8, 4, 2, 4, false>::kOutCols, p.columns, p.value_stride, p.scale_stride);
+}
+
+int gated_tile_rows(int64_t rows, int64_t experts, int inner, int columns, int64_t value_stride, int64_t scale_stride) {
+    return tile_rows(rows, experts, inner, columns, TileShape<8, 4, 2, 4, true>::kOutCols, columns / 2, value_stride, scale_stride);
 }
 
 }  // namespace
@@ -917,18 +1055,16 @@ int nanoep_experts_linear(const void* values, int64_t value_stride, const float*
         return status;
     if (out == nullptr || !aligned16(out))
         return NANOEP_ERR_INVALID_ARGUMENT;
-    // up to 64 inner columns the 16-bit instructions take no longer than the one 128-wide 8-bit one
-    if (inner > kScaleBlock / 2 && takes_tiles(rows, experts, inner, columns, value_stride, scale_stride))
-        return launch_tiles_by_rows<false>(p, out, static_cast<int64_t>(columns) * 2, static_cast<hipStream_t>(stream));
-    if (inner <= kScaleBlock / 2)
-        return launch_product<false, true>(p, out, columns, static_cast<hipStream_t>(stream));
-    return launch_product<false, false>(p, out, columns, static_cast<hipStream_t>(stream));
+    const auto on = static_cast<hipStream_t>(stream);
+    if (const int tile = linear_tile_rows(p))
+        return launch_product<false>(p, out, static_cast<int64_t>(columns) * 2, tile, on);
+    return inner <= kScaleBlock / 2 ? launch_streams<false, true>(p, out, columns, on) : launch_streams<false, false>(p, out, columns, on);
 }
 
 size_t nanoep_experts_gated_workspace_bytes(int64_t rows, int64_t experts, int inner, int columns, int64_t value_stride,
                                             int64_t scale_stride) {
     if (rows <= 0 || experts <= 0 || inner <= 0 || columns <= 0 ||
-        nanoep::takes_tiles(rows, experts, inner, columns, value_stride, scale_stride))
+        nanoep::gated_tile_rows(rows, experts, inner, columns, value_stride, scale_stride) != 0)
         return 0;
     return static_cast<size_t>(rows) * static_cast<size_t>(columns / 2) * sizeof(float);
 }
@@ -950,9 +1086,9 @@ int nanoep_experts_gated(const void* values, int64_t value_stride, const float* 
     if (needed > 0 && (workspace == nullptr || !aligned16(workspace)))
         return NANOEP_ERR_INVALID_ARGUMENT;
     const auto on = static_cast<hipStream_t>(stream);
-    if (takes_tiles(rows, experts, inner, columns, value_stride, scale_stride))
-        return launch_tiles_by_rows<true>(p, records, record_bytes_of(columns / 2), on);
-    const int launched = launch_product<true, true>(p, workspace, columns / 2, on);
+    if (const int tile = gated_tile_rows(rows, experts, inner, columns, value_stride, scale_stride))
+        return launch_product<true>(p, records, record_bytes_of(columns / 2), tile, on);
+    const int launched = launch_streams<true, true>(p, workspace, columns / 2, on);
     if (launched != NANOEP_OK)
         return launched;
     const unsigned blocks = static_cast<unsigned>((rows + kWavesPerBlock - 1) / kWavesPerBlock);

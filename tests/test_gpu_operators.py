@@ -128,25 +128,33 @@ def on(device, weight):
     return ep.Fp8Weight(weight.values.to(device), weight.scales.to(device))
 
 
+# the kernel by the product's size, and each one whatever its size
+KERNELS = [0, 1, 64, 128, 256]
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("inner,columns", SIZES)
 @pytest.mark.parametrize("segments", SEGMENTS)
-def test_experts_linear(device, segments, inner, columns):
+def test_experts_linear(device, tuning, segments, inner, columns, kernel):
+    tuning("EXPERTS_TILE", kernel)
     columns -= 8 if inner == 144 else 0  # a tile of columns that ends early
     values, scales, weight, offsets, counts = make_product(segments, inner, columns, inner + columns)
     z, slack = oracle.experts(values, scales, weight.values, weight.scales, offsets, counts)
-    print("experts_linear", segments, inner, columns, flush=True)
+    print("experts_linear", segments, inner, columns, kernel, flush=True)
     got = ep.experts_linear(records_of(values, scales, device), on(device, weight), offsets.to(device), counts.to(device))
     close(got, z, slack)
     loose = ep.Fp8Rows(values.to(device), scales.to(device))
     assert torch.equal(ep.experts_linear(loose, on(device, weight), offsets.to(device), counts.to(device)), got)
 
 
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("inner,columns", SIZES)
 @pytest.mark.parametrize("segments", SEGMENTS)
-def test_experts_gated(device, segments, inner, columns):
+def test_experts_gated(device, tuning, segments, inner, columns, kernel):
+    tuning("EXPERTS_TILE", kernel)
     values, scales, weight, offsets, counts = make_product(segments, inner, columns, inner + columns)
     act, slack = oracle.gated(*oracle.experts(values, scales, weight.values, weight.scales, offsets, counts))
-    print("experts_gated", segments, inner, columns, flush=True)
+    print("experts_gated", segments, inner, columns, kernel, flush=True)
     got = ep.experts_gated(records_of(values, scales, device), on(device, weight), offsets.to(device), counts.to(device))
     oracle.check_eight_bits(got.values.cpu(), got.scales.cpu(), act, slack)
     width = columns // 2
@@ -156,7 +164,9 @@ def test_experts_gated(device, segments, inner, columns):
 
 
 @pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 31, 33, 64, 65, 100, 129, 300])
-def test_products_without_a_layout_are_one_experts(device, rows):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_products_without_a_layout_are_one_experts(device, rows, tuning, kernel):
+    tuning("EXPERTS_TILE", kernel)
     inner, columns = 272, 320
     values, scales = oracle.quantize_rows(randn(rows, rows, inner))
     weight = ep.quantize_weight(randn(rows + 1, 1, columns, inner))
@@ -168,7 +178,9 @@ def test_products_without_a_layout_are_one_experts(device, rows):
     oracle.check_eight_bits(got.values.cpu(), got.scales.cpu(), *oracle.gated(z, slack))
 
 
-def test_products_follow_strides_of_their_own(device):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_products_follow_strides_of_their_own(device, tuning, kernel):
+    tuning("EXPERTS_TILE", kernel)
     values, scales, weight, offsets, counts = make_product("uneven", 256, 128, 9)
     z, slack = oracle.experts(values, scales, weight.values, weight.scales, offsets, counts)
     rows = values.shape[0]
@@ -181,7 +193,9 @@ def test_products_follow_strides_of_their_own(device):
     close(got, z, slack)
 
 
-def test_products_keep_a_nan_to_its_row_and_its_expert(device):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_products_keep_a_nan_to_its_row_and_its_expert(device, tuning, kernel):
+    tuning("EXPERTS_TILE", kernel)
     values, scales, weight, offsets, counts = make_product("uneven", 256, 256, 4)
     values.view(torch.uint8)[10, 77] = NAN_BYTE
     weight.values.view(torch.uint8)[3, 20, 100] = NAN_BYTE
@@ -195,7 +209,9 @@ def test_products_keep_a_nan_to_its_row_and_its_expert(device):
     assert torch.equal(got.scales.cpu()[:, 0].isnan(), reached.any(1))
 
 
-def test_products_stay_within_the_rows_whatever_the_layout_says(device):
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_products_stay_within_the_rows_whatever_the_layout_says(device, tuning, kernel):
+    tuning("EXPERTS_TILE", kernel)
     values, scales = oracle.quantize_rows(randn(3, 64, 128))
     weight = ep.quantize_weight(randn(4, 3, 64, 128))
     rows = ep.Fp8Rows(values.to(device), scales.to(device))
