@@ -11,8 +11,10 @@ constexpr int kMostNormVectors = 8;  // 16-byte vectors of a row that a lane hol
 // One workgroup a row: s = x + residual, r = 1 / sqrt(mean(s^2) + eps), n = s * r * gamma; then, for every 128
 // columns, scale = max |n| / 448 and the values n / scale, rounded to e4m3.  The row stays in registers
 // between its sum of squares and its output (kVectors 16-byte vectors a lane, 8 columns each), so that every
-// input byte is read once; s and n are fp32 throughout, and each output is rounded from them once.  16
-// neighbouring lanes hold the 128 columns of a scale.
+// input byte is read once, all of them ahead of anything else; s and n are fp32 throughout, and each output is rounded from them once.  16
+// neighbouring lanes hold the 128 columns of a scale.  HBM-bound: 4096 x 7168 with both bf16 outputs 48.3 us, 5.5 TB/s (outputs
+// with plain stores and gamma read behind the sum: 54.0), 8192 x 2048 24.7 us, 6.1 TB/s; nontemporal loads of the inputs take 44.9
+// and 27.2 us, but would pass over inputs that the last kernel left in the caches.
 template <int kVectors>
 __global__ void __launch_bounds__(kMostNormThreads) rms_norm_fp8_kernel(const u32x4* __restrict__ x,         // [T][vectors]
                                                                        const u32x4* __restrict__ residual,  // [T][vectors] or null
@@ -33,6 +35,14 @@ __global__ void __launch_bounds__(kMostNormThreads) rms_norm_fp8_kernel(const u3
 
     float s[kVectors][8];
     float squares = 0.0f;
+    u32x4 others[kVectors];
+    if (residual != nullptr) {
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            const int at = threadIdx.x + v * threads;
+            others[v] = at < vectors ? row_residual[at] : u32x4{0u, 0u, 0u, 0u};
+        }
+    }
 #pragma unroll
     for (int v = 0; v < kVectors; ++v) {
         const int at = threadIdx.x + v * threads;
@@ -45,14 +55,13 @@ __global__ void __launch_bounds__(kMostNormThreads) rms_norm_fp8_kernel(const u3
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
             const int at = threadIdx.x + v * threads;
-            float other[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-            if (at < vectors)
-                unpack_bf16(row_residual[at], other);
+            float other[8];
+            unpack_bf16(others[v], other);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 s[v][i] += other[i];
             if (at < vectors)
-                residual_out[row * vectors + at] = pack_bf16(s[v]);
+                store_vec<true>(residual_out + row * vectors + at, pack_bf16(s[v]));
         }
     }
 #pragma unroll
@@ -60,6 +69,12 @@ __global__ void __launch_bounds__(kMostNormThreads) rms_norm_fp8_kernel(const u3
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             squares = fmaf(s[v][i], s[v][i], squares);
+    u32x4 gammas[kVectors];
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v) {
+        const int at = threadIdx.x + v * threads;
+        gammas[v] = at < vectors ? gamma[at] : u32x4{0u, 0u, 0u, 0u};
+    }
     squares = wave_sum(squares);
     if (threadIdx.x % kWave == 0)
         wave_sums[threadIdx.x / kWave] = squares;
@@ -74,9 +89,8 @@ __global__ void __launch_bounds__(kMostNormThreads) rms_norm_fp8_kernel(const u3
 #pragma unroll
     for (int v = 0; v < kVectors; ++v) {
         const int at = threadIdx.x + v * threads;
-        float weight[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (at < vectors)
-            unpack_bf16(gamma[at], weight);
+        float weight[8];
+        unpack_bf16(gammas[v], weight);
         uint32_t amax = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -85,7 +99,7 @@ __global__ void __launch_bounds__(kMostNormThreads) rms_norm_fp8_kernel(const u3
             amax = larger(amax, magnitude_bits(s[v][i]));
         }
         if (normalized != nullptr && at < vectors)
-            normalized[row * vectors + at] = pack_bf16(s[v]);
+            store_vec<true>(normalized + row * vectors + at, pack_bf16(s[v]));
         const GroupScale group = group_scale(largest_of_16(amax));
         if (at < vectors) {
             uint2 packed;
@@ -122,8 +136,9 @@ int nanoep_rms_norm_fp8(const void* x, const void* residual, const void* gamma, 
         !aligned16(records) || !aligned16(residual_out) || !aligned16(normalized))
         return NANOEP_ERR_INVALID_ARGUMENT;
     const int vectors = hidden / 8;
-    // one vector a lane up to 1024 lanes while there are few rows; more a lane when the rows alone fill the device
-    const int wanted = num_tokens >= 1024 ? 4 : 1;
+    // one vector a lane up to 1024 lanes while there are few rows; two when the rows alone fill the device (4096 x 7168: one 47.6
+    // us, two 48.3, four 49.2; 8192 x 2048: 26.7, 24.7, 27.0)
+    const int wanted = num_tokens >= 1024 ? 2 : 1;
     int held = 1;
     while (held < kMostNormVectors && (vectors + held - 1) / held > (held < wanted ? kWave : kMostNormThreads))
         held *= 2;

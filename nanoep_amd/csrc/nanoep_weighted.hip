@@ -66,22 +66,53 @@ __global__ void __launch_bounds__(kBlockThreads) combine_weighted_kernel(const u
     }
 }
 
+// Zeros in a part of the rows of grad_y that no choice refers to: behind every expert's rows, and behind the last expert's
+// segment, each in kGapParts parts.
+constexpr int kGapParts = 8;
+constexpr int64_t kGapBytesApart = int64_t{32} << 20;
+__device__ __forceinline__ void clear_gap(const int64_t* expert_offsets, const int64_t* expert_counts, u32x4* rows, int64_t num_rows,
+                                          int64_t num_experts, int vectors, int64_t part) {
+    const int64_t expert = part / kGapParts;
+    int64_t begin = expert_offsets[expert], end = num_rows;
+    if (expert < num_experts) {
+        begin += expert_counts[expert];
+        end = expert_offsets[expert + 1];
+    }
+    begin = begin < 0 ? 0 : begin;
+    end = end > num_rows ? num_rows : end;
+    if (begin >= end)
+        return;
+    const int64_t gap = (end - begin) * vectors, each = (gap + kGapParts - 1) / kGapParts;
+    const int64_t from = part % kGapParts * each, to = from + each < gap ? from + each : gap;
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    for (int64_t at = from + threadIdx.x; at < to; at += kBlockThreads)
+        store_vec<true>(rows + begin * vectors + at, zero);
+}
+
 // The gradient: grad_y[slot[t][k]] = weights[t][k] * grad[t], grad_weights[t][k] = <y[slot[t][k]], grad[t]>.
 // One wavefront a (token, choice) walks the row once: it reads both rows, writes the third and keeps the product's
 // sum in its lanes, which are added in a fixed order at the end.  A token's choices are neighbours, so that its
-// gradient row comes from the caches for all but one of them.
+// gradient row comes from the caches for all but one of them.  Workgroups ahead of theirs clear the rows of no expert.
 __global__ void __launch_bounds__(kBlockThreads) combine_weighted_backward_kernel(const u32x4* __restrict__ grad,  // [T][vectors]
                                                                                   const u32x4* __restrict__ y,     // [C][vectors]
                                                                                   const int32_t* __restrict__ token_slots,
                                                                                   const float* __restrict__ weights,
                                                                                   u32x4* __restrict__ grad_y,
                                                                                   float* __restrict__ grad_weights,
+                                                                                  const int64_t* __restrict__ expert_offsets,  // null: all cleared before
+                                                                                  const int64_t* __restrict__ expert_counts,
+                                                                                  int64_t num_experts,
                                                                                   int64_t y_rows,
                                                                                   int64_t pairs,
+                                                                                  uint32_t gap_blocks,
                                                                                   int vectors,
                                                                                   int num_topk) {
+    if (blockIdx.x < gap_blocks) {
+        clear_gap(expert_offsets, expert_counts, grad_y, y_rows, num_experts, vectors, blockIdx.x);
+        return;
+    }
     const int lane = threadIdx.x % kWave;
-    const int64_t pair = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int64_t pair = static_cast<int64_t>(blockIdx.x - gap_blocks) * kWavesPerBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if (pair >= pairs)
         return;
     const int64_t slot = token_slots[pair];
@@ -110,27 +141,6 @@ __global__ void __launch_bounds__(kBlockThreads) combine_weighted_backward_kerne
     product = wave_sum(product);
     if (lane == 0)
         grad_weights[pair] = product;
-}
-
-// Zeros in the rows of grad_y that no choice refers to: behind every expert's rows, and behind the last expert's segment.
-__global__ void __launch_bounds__(kBlockThreads) zero_gaps_kernel(const int64_t* __restrict__ expert_offsets,
-                                                                  const int64_t* __restrict__ expert_counts,
-                                                                  u32x4* __restrict__ rows,
-                                                                  int64_t num_rows,
-                                                                  int64_t num_experts,
-                                                                  int vectors) {
-    const int64_t expert = blockIdx.x;
-    int64_t begin = expert_offsets[expert], end = num_rows;
-    if (expert < num_experts) {
-        begin += expert_counts[expert];
-        end = expert_offsets[expert + 1];
-    }
-    begin = begin < 0 ? 0 : begin;
-    end = end > num_rows ? num_rows : end;
-    const u32x4 zero = {0u, 0u, 0u, 0u};
-    for (int64_t at = begin * vectors + static_cast<int64_t>(blockIdx.y) * kBlockThreads + threadIdx.x; at < end * vectors;
-         at += static_cast<int64_t>(gridDim.y) * kBlockThreads)
-        store_vec<true>(rows + at, zero);
 }
 
 __global__ void __launch_bounds__(kBlockThreads) zero_rows_kernel(u32x4* __restrict__ rows, int64_t vectors) {
@@ -187,23 +197,28 @@ int nanoep_combine_weighted_backward(const void* grad, const void* y, int64_t y_
         return NANOEP_ERR_INVALID_ARGUMENT;
     const int vectors = hidden / 8;
     const auto on = static_cast<hipStream_t>(stream);
-    if (y_rows > 0) {
-        if (expert_offsets != nullptr) {
-            zero_gaps_kernel<<<dim3(static_cast<unsigned>(num_local_experts + 1), 8), kBlockThreads, 0, on>>>(
-                expert_offsets, expert_counts, static_cast<u32x4*>(grad_y), y_rows, num_local_experts, vectors);
-        } else {
-            zero_rows_kernel<<<2048, kBlockThreads, 0, on>>>(static_cast<u32x4*>(grad_y), y_rows * vectors);
-        }
+    if (y_rows > 0 && expert_offsets == nullptr) {
+        zero_rows_kernel<<<2048, kBlockThreads, 0, on>>>(static_cast<u32x4*>(grad_y), y_rows * vectors);
         NANOEP_HIP_TRY(hipGetLastError());
     }
-    if (num_tokens > 0) {
-        const int64_t pairs = num_tokens * num_topk;
-        const unsigned blocks = static_cast<unsigned>((pairs + kWavesPerBlock - 1) / kWavesPerBlock);
-        combine_weighted_backward_kernel<<<blocks, kBlockThreads, 0, on>>>(
-            static_cast<const u32x4*>(grad), static_cast<const u32x4*>(y), token_slots, weights, static_cast<u32x4*>(grad_y), grad_weights,
-            y_rows, pairs, vectors, num_topk);
-        NANOEP_HIP_TRY(hipGetLastError());
-    }
+    const int64_t pairs = num_tokens * num_topk, pair_blocks = (pairs + kWavesPerBlock - 1) / kWavesPerBlock;
+    const int64_t gap_blocks = y_rows > 0 && expert_offsets != nullptr ? (num_local_experts + 1) * kGapParts : 0;
+    if (pair_blocks + gap_blocks > 0x7fffffff)
+        return NANOEP_ERR_INVALID_ARGUMENT;
+    // Few rows to clear ride in the gradient's launch (9222 choices, 450 padding rows of 2816: 23.0 us, in a launch of their own
+    // 28.8); many have one ahead of it, because writes alone and the gradient's mix go faster one after the other (29500
+    // choices, 16200 padding rows of 7168: 197 us, beside one another 204).
+    const bool apart = (y_rows - pairs) * hidden * 2 > kGapBytesApart;
+    const auto launch = [&](int64_t gaps, int64_t blocks) {
+        if (blocks > 0)
+            combine_weighted_backward_kernel<<<static_cast<unsigned>(blocks), kBlockThreads, 0, on>>>(
+                static_cast<const u32x4*>(grad), static_cast<const u32x4*>(y), token_slots, weights, static_cast<u32x4*>(grad_y), grad_weights,
+                expert_offsets, expert_counts, num_local_experts, y_rows, pairs, static_cast<uint32_t>(gaps), vectors, num_topk);
+    };
+    if (apart)
+        launch(gap_blocks, gap_blocks);
+    launch(apart ? 0 : gap_blocks, (apart ? 0 : gap_blocks) + pair_blocks);
+    NANOEP_HIP_TRY(hipGetLastError());
     return NANOEP_OK;
 }
 
