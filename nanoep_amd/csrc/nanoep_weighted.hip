@@ -195,6 +195,8 @@ int nanoep_combine_weighted_backward(const void* grad, const void* y, int64_t y_
         return NANOEP_ERR_INVALID_ARGUMENT;
     if (num_tokens > 0 && (grad == nullptr || token_slots == nullptr || weights == nullptr || grad_weights == nullptr))
         return NANOEP_ERR_INVALID_ARGUMENT;
+    if (num_tokens == 0 && y_rows == 0)
+        return NANOEP_OK;
     const int vectors = hidden / 8;
     const auto on = static_cast<hipStream_t>(stream);
     if (y_rows > 0 && expert_offsets == nullptr) {
