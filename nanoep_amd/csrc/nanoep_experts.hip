@@ -406,6 +406,8 @@ struct TileShape {
     static constexpr int kOutCols = kGated ? kCols / 2 : kCols;
     static constexpr int kRowLoads = kRows / 8 / kWaves;     // loads of a wavefront that bring in a block of the rows
     static constexpr int kWeightLoads = kCols / 8 / kWaves;  // ... and of the weights
+    // blocks in LDS: as many as fit beside the lists
+    static constexpr int kStages = (kRows + kCols) * kScaleBlock * 3 <= (148 << 10) ? 3 : 2;
     // stores of a wavefront that write a tile's output
     static constexpr int kStores = kGated ? kRowTiles * kColTiles / 2 : kRowTiles * kColTiles;
     static_assert(kRows % (8 * kWaves) == 0 && kCols % (8 * kWaves) == 0 && kRows % kWave == 0);
@@ -512,10 +514,14 @@ template <int kRowTiles, int kColTiles, int kRowWaves, int kColWaves, bool kGate
 __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
     experts_tile_kernel(const Product p, char* __restrict__ out, int64_t out_stride, int column_tiles, XcdMap xcds) {
     using Shape = TileShape<kRowTiles, kColTiles, kRowWaves, kColWaves, kGated>;
+    constexpr int kStages = Shape::kStages;
     constexpr int kWeightBytes = Shape::kCols * kScaleBlock, kRowBytes = Shape::kRows * kScaleBlock;
-    __shared__ __attribute__((aligned(1024))) char weight_blocks[2][kWeightBytes];
-    __shared__ __attribute__((aligned(1024))) char row_blocks[2][kRowBytes];
-    __shared__ float row_scales[2][Shape::kRows];
+    // accesses of a wavefront that are newer than the next block's operands when it asks for those
+    constexpr int kNewer = (kStages - 1) * Shape::kWeightLoads + (kStages - 2) * (Shape::kRowLoads + 1);
+    const auto after = [](int slot) { return slot + 1 == kStages ? 0 : slot + 1; };
+    __shared__ __attribute__((aligned(1024))) char weight_blocks[kStages][kWeightBytes];
+    __shared__ __attribute__((aligned(1024))) char row_blocks[kStages][kRowBytes];
+    __shared__ float row_scales[kStages][Shape::kRows];
     __shared__ uint32_t group_amax[kGated ? Shape::kRows : 1][kColWaves];
     __shared__ int wave_sums[Shape::kWaves];
     __shared__ Item items[kMostItems];
@@ -598,7 +604,7 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                     load_to_lds<16>(at + piece * 16 < p.inner ? weight + at + weight_offset[i] + piece * 16 : reinterpret_cast<const char*>(&kZeroPiece),
                                 to + i * kStep);
             }
-            weight_slot ^= 1;
+            weight_slot = after(weight_slot);
             if (++weight_block == p.blocks)
                 weight_block = 0;
             if (--weight_left == 0) {
@@ -646,7 +652,7 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
             }
             // (where there are more wavefronts than 64 rows, some bring in the same scales)
             load_to_lds<4>(scales + static_cast<int64_t>(row_block) * 4, scale_offset, scales_at + row_slot * Shape::kRows * 4);
-            row_slot ^= 1;
+            row_slot = after(row_slot);
             if (++row_block == p.blocks)
                 row_block = 0;
             if (--row_left == 0) {
@@ -687,14 +693,19 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
             rows[to][1] = row_piece(in_slot, r, 1);
             scale[to] = row_scales[in_slot][scale_at + r * kTile];
         };
+        bool weights_ahead = false;  // whether the newest fetch of weights was one
         if (weight_item < count) {
             aim_weights();
             aim_rows();
-            fetch_weights();
-            fetch_rows();
-            all_but_newest<0>();
-            fetch_weights();
-            fetch_rows();
+#pragma unroll
+            for (int stage = 0; stage < kStages; ++stage) {
+                weights_ahead = fetch_weights();
+                fetch_rows();
+            }
+            if (weights_ahead)
+                all_but_newest<(kStages - 1) * (Shape::kWeightLoads + Shape::kRowLoads + 1)>();
+            else
+                all_but_newest<0>();
 #pragma unroll
             for (int c = 0; c < kColTiles; ++c)
                 read_weights(0, c);
@@ -704,8 +715,7 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
         if (listed == 0 && p.expert_offsets != nullptr)
             for (int part = static_cast<int>(blockIdx.x); part < (p.experts + 1) * kGapParts; part += static_cast<int>(gridDim.x))
                 clear_rows<kGated, Shape::kThreads>(out, out_stride, out_columns, gap_part(p, part));
-        bool weights_ahead = false;
-        bool stored = false;  // the newest accesses are a tile's stores
+        int stored = 0;  // blocks whose operands are older than the last tile's stores
         for (int i = 0; i < count; ++i) {
             const Item item = item_at(i);
             const int live = item.live;
@@ -757,13 +767,13 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                             // matrix instructions of that tile hide the first reads of the next block.
                             if (!weights_ahead)
                                 all_but_newest<0>();
-                            else if (stored)
-                                all_but_newest<Shape::kWeightLoads + Shape::kStores>();
+                            else if (stored > 0)
+                                all_but_newest<kNewer + Shape::kStores>();
                             else
-                                all_but_newest<Shape::kWeightLoads>();
-                            stored = false;
+                                all_but_newest<kNewer>();
+                            --stored;
                             fetch_rows();
-                            read_rows(slot ^ 1, 0, 0);
+                            read_rows(after(slot), 0, 0);
                         }
                         f32x4 product[kColTiles];
 #pragma unroll
@@ -788,7 +798,7 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                             for (int c = 0; c < kColTiles; ++c)
-                                read_weights(slot ^ 1, c);
+                                read_weights(after(slot), c);
                             __builtin_amdgcn_sched_barrier(0);
                         }
 #pragma unroll
@@ -802,7 +812,7 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                         static_assert(kColTiles == 4);
                         asm volatile("" : "+v"(acc[0][r]), "+v"(acc[1][r]), "+v"(acc[2][r]), "+v"(acc[3][r]));
                     }
-                    slot ^= 1;
+                    slot = after(slot);
                 }
             }
 
@@ -881,7 +891,7 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                     }
                 }
             }
-            stored = true;
+            stored = kStages - 1;
         }
         // (the list's memory is the weights': nothing may still be on its way there)
         if (count < kMostItems)
