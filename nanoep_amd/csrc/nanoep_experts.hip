@@ -775,6 +775,9 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                             fetch_rows();
                             read_rows(after(slot), 0, 0);
                         }
+                        float linear_factor = 0.0f;  // (a gated product has no registers for its four ahead of their use)
+                        if constexpr (!kGated)
+                            linear_factor = column_scale[0] * scale[r & 1];
                         f32x4 product[kColTiles];
 #pragma unroll
                         for (int c = 0; c < kColTiles; ++c)
@@ -803,7 +806,7 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                         }
 #pragma unroll
                         for (int c = 0; c < kColTiles; ++c) {
-                            const float factor = column_scale[c % kScales] * scale[r & 1];
+                            const float factor = kGated ? column_scale[c % kScales] * scale[r & 1] : linear_factor;
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
                                 acc[c][r][j] = fmaf(factor, product[c][j], acc[c][r][j]);
