@@ -192,6 +192,12 @@ __device__ __forceinline__ void load_to_lds(const char* from, uint32_t to) {
 // What is read in the place of a piece that lies past its row's end.
 __device__ const u32x4 kZeroPiece = {0u, 0u, 0u, 0u};
 
+// The odd groups of 16 lanes of `a` and the even ones of `b` change places.
+__device__ __forceinline__ u32x2 swapped(uint32_t a, uint32_t b) {
+    const auto both = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    return {both[0], both[1]};
+}
+
 // Waits until all but the newest kNewer of this wavefront's loads are done, and its reads of LDS.
 template <int kNewer>
 __device__ __forceinline__ void loaded_but_newest() {
@@ -409,7 +415,7 @@ struct TileShape {
     // blocks in LDS: as many as fit beside the lists
     static constexpr int kStages = (kRows + kCols) * kScaleBlock * 3 <= (148 << 10) ? 3 : 2;
     // stores of a wavefront that write a tile's output
-    static constexpr int kStores = kGated ? kRowTiles * kColTiles / 2 : kRowTiles * kColTiles;
+    static constexpr int kStores = kGated ? kRowTiles * kColTiles / 4 : kRowTiles * kColTiles / 2;
     static_assert(kRows % (8 * kWaves) == 0 && kCols % (8 * kWaves) == 0 && kRows % kWave == 0);
 };
 
@@ -506,7 +512,10 @@ __device__ __forceinline__ int list_tiles(const Product& p, int column_tiles, ui
 // time for it.  Rows mostly come from L2 and have one block's.  The two cursors run on into the next tile, whose first
 // operands so arrive while this one's output is written.
 //
-// Measured (32 experts, 29500 rows): 2048 -> 7168 590 us, 1.47 PFLOP/s; gated 7168 -> 2 x 2048 1690 us, 1.02 PFLOP/s (its bf16
+// A lane's four columns of a tile are 8 bytes of bf16: neighbouring column tiles swap halves first, so that half as many
+// stores write twice as much each (2048 -> 7168 557 us against 597, 64 rows an expert 102 against 108).
+//
+// Measured (32 experts, 29500 rows): 2048 -> 7168 557 us, 1.55 PFLOP/s; gated 7168 -> 2 x 2048 1650 us, 1.05 PFLOP/s (its bf16
 // instructions have half the rate).  A block of a tile takes 2.0 us; its matrix instructions alone take 0.98 us, its
 // loads alone 1.36 us: 64 KB that L2 hands out in 64-byte requests, of which a block of all tiles needs about as many
 // clocks as its matrix instructions.  One block's time ahead for the weights, the loads alone took 1.76 us.
@@ -832,11 +841,14 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                     const int in_rows = first_row + r * kTile;
                     const uint32_t row = static_cast<uint32_t>(in_rows) * static_cast<uint32_t>(out_stride);
 #pragma unroll
-                    for (int c = 0; c < kColTiles; ++c) {
-                        const int column = first_column + (col_wave * kColTiles + c) * kTile + in_group * 4;
-                        const f32x4 v = acc[c][r];
-                        const u32x2 packed = {to_bf16_pair(v[0], v[1]), to_bf16_pair(v[2], v[3])};
-                        __builtin_amdgcn_raw_buffer_store_b64(packed, tile_rows, column < out_columns ? row + column * 2 : kNowhere, 0, 0);
+                    for (int c = 0; c < kColTiles; c += 2) {
+                        // two neighbouring column tiles: lanes of even groups get eight columns of the first, of odd ones of the second
+                        const f32x4 v = acc[c][r], w = acc[c + 1][r];
+                        const u32x2 low = swapped(to_bf16_pair(v[0], v[1]), to_bf16_pair(w[0], w[1]));
+                        const u32x2 high = swapped(to_bf16_pair(v[2], v[3]), to_bf16_pair(w[2], w[3]));
+                        const int column = first_column + (col_wave * kColTiles + c + in_group % 2) * kTile + in_group / 2 * 8;
+                        __builtin_amdgcn_raw_buffer_store_b128(u32x4{low.x, high.x, low.y, high.y}, tile_rows,
+                                                               column < out_columns ? row + column * 2 : kNowhere, 0, 0);
                     }
                 }
             } else {
@@ -886,11 +898,13 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
 #pragma unroll
                 for (int r = 0; r < kRowTiles; ++r) {
                     const uint32_t row = static_cast<uint32_t>(first_row + r * kTile) * static_cast<uint32_t>(out_stride);
+                    static_assert(kOutTiles % 2 == 0 || !kGated);
 #pragma unroll
-                    for (int c = 0; c < kOutTiles; ++c) {
-                        const int column = first_column + (col_wave * kOutTiles + c) * kTile + in_group * 4;
-                        __builtin_amdgcn_raw_buffer_store_b32(to_fp8_quad(acc[c][r][0], acc[c][r][1], acc[c][r][2], acc[c][r][3]), tile_rows,
-                                                              column < out_columns ? row + column : kNowhere, 0, 0);
+                    for (int c = 0; c < kOutTiles; c += 2) {
+                        const u32x2 both = swapped(to_fp8_quad(acc[c][r][0], acc[c][r][1], acc[c][r][2], acc[c][r][3]),
+                                                   to_fp8_quad(acc[c + 1][r][0], acc[c + 1][r][1], acc[c + 1][r][2], acc[c + 1][r][3]));
+                        const int column = first_column + (col_wave * kOutTiles + c + in_group % 2) * kTile + in_group / 2 * 8;
+                        __builtin_amdgcn_raw_buffer_store_b64(both, tile_rows, column < out_columns ? row + column : kNowhere, 0, 0);
                     }
                 }
             }
