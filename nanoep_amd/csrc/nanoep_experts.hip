@@ -513,7 +513,7 @@ __device__ __forceinline__ int list_tiles(const Product& p, int column_tiles, ui
 // operands so arrive while this one's output is written.
 //
 // A lane's four columns of a tile are 8 bytes of bf16: neighbouring column tiles swap halves first, so that half as many
-// stores write twice as much each (2048 -> 7168 557 us against 597, 64 rows an expert 102 against 108).
+// stores write twice as much each (2048 -> 7168 557 us against 597).
 //
 // Measured (32 experts, 29500 rows): 2048 -> 7168 557 us, 1.55 PFLOP/s; gated 7168 -> 2 x 2048 1650 us, 1.05 PFLOP/s (its bf16
 // instructions have half the rate).  A block of a tile takes 2.0 us; its matrix instructions alone take 0.98 us, its
@@ -524,6 +524,8 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
     experts_tile_kernel(const Product p, char* __restrict__ out, int64_t out_stride, int column_tiles, XcdMap xcds) {
     using Shape = TileShape<kRowTiles, kColTiles, kRowWaves, kColWaves, kGated>;
     constexpr int kStages = Shape::kStages;
+    constexpr bool kSkips = kGated && kRowTiles <= 4;
+    constexpr int kRowStep = kRowWaves * kTile;  // the row wavefronts' row tiles alternate
     constexpr int kWeightBytes = Shape::kCols * kScaleBlock, kRowBytes = Shape::kRows * kScaleBlock;
     // accesses of a wavefront that are newer than the next block's operands when it asks for those
     constexpr int kNewer = (kStages - 1) * Shape::kWeightLoads + (kStages - 2) * (Shape::kRowLoads + 1);
@@ -673,14 +675,14 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
 
         int slot = 0;
         const int turned = (group ^ (lane & 7)) * 16;
-        const int weight_at = (col_wave * kColTiles * kTile + in_tile) * kScaleBlock, row_at = (row_wave * kRowTiles * kTile + in_tile) * kScaleBlock;
-        const int scale_at = row_wave * kRowTiles * kTile + in_tile;
+        const int weight_at = (col_wave * kColTiles * kTile + in_tile) * kScaleBlock, row_at = (row_wave * kTile + in_tile) * kScaleBlock;
+        const int scale_at = row_wave * kTile + in_tile;
         // a lane's two pieces of a row: columns group * 16 on of the block, and 64 further
         const auto weight_piece = [&](int in_slot, int c, int half) {
             return *reinterpret_cast<const u32x4*>(weight_blocks[in_slot] + weight_at + c * kTile * kScaleBlock + (turned ^ half * 64));
         };
         const auto row_piece = [&](int in_slot, int r, int half) {
-            return *reinterpret_cast<const u32x4*>(row_blocks[in_slot] + row_at + r * kTile * kScaleBlock + (turned ^ half * 64));
+            return *reinterpret_cast<const u32x4*>(row_blocks[in_slot] + row_at + r * kRowStep * kScaleBlock + (turned ^ half * 64));
         };
         i32x8 weights[kGated ? 1 : kColTiles];
         bf16x8 wide_weights[kGated ? kColTiles : 1][4];
@@ -700,7 +702,7 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
         const auto read_rows = [&](int in_slot, int r, int to) {
             rows[to][0] = row_piece(in_slot, r, 0);
             rows[to][1] = row_piece(in_slot, r, 1);
-            scale[to] = row_scales[in_slot][scale_at + r * kTile];
+            scale[to] = row_scales[in_slot][scale_at + r * kRowStep];
         };
         bool weights_ahead = false;  // whether the newest fetch of weights was one
         if (weight_item < count) {
@@ -751,6 +753,10 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                     weight_scales[c] = p.weight_scales + (static_cast<int64_t>(item.expert) * p.column_blocks + column / kScaleBlock) * p.blocks;
                     next_scale[c] = uniform_load(weight_scales[c] + first_block(item));
                 }
+                // Row tiles without a live row are left out of a gated product's small tiles, whose few rows an expert its
+                // 16-bit instructions take longer with than the weights' way from memory (32 experts of 16 rows 188 us against
+                // 238).  A linear product gains nothing by it, and the 256-row tile has no registers for the branches.
+                const int live_tiles = kSkips ? __builtin_amdgcn_readfirstlane((static_cast<int>(live) - row_wave * kTile + kRowStep - 1) / kRowStep) : kRowTiles;
                 int block = first_block(item);
                 for (int turn = 0; turn < p.blocks; ++turn) {
                     float column_scale[kScales];
@@ -791,7 +797,8 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
 #pragma unroll
                         for (int c = 0; c < kColTiles; ++c)
                             product[c] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        if constexpr (kGated) {
+                        if (kSkips && r >= live_tiles) {
+                        } else if constexpr (kGated) {
 #pragma unroll
                             for (int part = 0; part < 4; ++part) {
                                 const u32x4 raw = rows[r & 1][part / 2];
@@ -813,12 +820,14 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                                 read_weights(after(slot), c);
                             __builtin_amdgcn_sched_barrier(0);
                         }
+                        if (!kSkips || r < live_tiles) {
 #pragma unroll
-                        for (int c = 0; c < kColTiles; ++c) {
-                            const float factor = kGated ? column_scale[c % kScales] * scale[r & 1] : linear_factor;
+                            for (int c = 0; c < kColTiles; ++c) {
+                                const float factor = kGated ? column_scale[c % kScales] * scale[r & 1] : linear_factor;
 #pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                acc[c][r][j] = fmaf(factor, product[c][j], acc[c][r][j]);
+                                for (int j = 0; j < 4; ++j)
+                                    acc[c][r][j] = fmaf(factor, product[c][j], acc[c][r][j]);
+                            }
                         }
                         // (done here, not where the sums are next used, with all products kept until then)
                         static_assert(kColTiles == 4);
@@ -831,14 +840,14 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
             // Stores past the tile's rows or columns are dropped by the buffer's bounds, not branched around: a wavefront's
             // number of them is always the same, which the count of newest accesses above relies on.
             const int out_lane = afresh(lane), in_group = out_lane / kTile;
-            const int first_row = row_wave * kRowTiles * kTile + out_lane % kTile;
+            const int first_row = row_wave * kTile + out_lane % kTile;
             constexpr uint32_t kNowhere = 0xffffffffu;
             char* tile_out = out + item.row * out_stride;
             const __amdgpu_buffer_rsrc_t tile_rows = __builtin_amdgcn_make_buffer_rsrc(tile_out, 0, static_cast<int>(live * out_stride), 0x00020000);
             if constexpr (!kGated) {
 #pragma unroll
                 for (int r = 0; r < kRowTiles; ++r) {
-                    const int in_rows = first_row + r * kTile;
+                    const int in_rows = first_row + r * kRowStep;
                     const uint32_t row = static_cast<uint32_t>(in_rows) * static_cast<uint32_t>(out_stride);
 #pragma unroll
                     for (int c = 0; c < kColTiles; c += 2) {
@@ -857,7 +866,7 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
 #pragma unroll
                 for (int r = 0; r < kRowTiles; ++r) {
                     uint32_t amax = 0;
-                    const bool is_live = first_row + r * kTile < live;
+                    const bool is_live = first_row + r * kRowStep < live;
 #pragma unroll
                     for (int c = 0; c < kOutTiles; ++c) {
                         const int column = first_column + (col_wave * kOutTiles + c) * kTile + in_group * 4;
@@ -871,12 +880,12 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                     amax = larger(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 16, kWave)));
                     amax = larger(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 32, kWave)));
                     if (in_group == 0)
-                        group_amax[first_row + r * kTile][col_wave] = amax;
+                        group_amax[first_row + r * kRowStep][col_wave] = amax;
                 }
                 lds_settled();
 #pragma unroll
                 for (int r = 0; r < kRowTiles; ++r) {
-                    const int in_rows = first_row + r * kTile;
+                    const int in_rows = first_row + r * kRowStep;
                     uint32_t amax = group_amax[in_rows][0];
 #pragma unroll
                     for (int w = 1; w < kColWaves; ++w)
@@ -897,7 +906,7 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                 }
 #pragma unroll
                 for (int r = 0; r < kRowTiles; ++r) {
-                    const uint32_t row = static_cast<uint32_t>(first_row + r * kTile) * static_cast<uint32_t>(out_stride);
+                    const uint32_t row = static_cast<uint32_t>(first_row + r * kRowStep) * static_cast<uint32_t>(out_stride);
                     static_assert(kOutTiles % 2 == 0 || !kGated);
 #pragma unroll
                     for (int c = 0; c < kOutTiles; c += 2) {
@@ -1011,9 +1020,12 @@ int launch_tiles(const Product& p, void* out, int64_t out_stride, hipStream_t st
 }
 
 // Rows of the tile kernel's tiles for a product, 0 for the stream kernel.
-//   The tile follows the rows an expert has on average.  Of 32 experts, 2048 -> 7168: 58 rows each 127 us with 64-row tiles and 128 with
-//   128-row ones (gated, 7168 -> 2048: 261 and 281), 115 rows 158, 136 and, with 256-row tiles, 175 us, 230 rows 207 (128) and 202 us
-//   (256; gated 580 and 626), 460 rows 355 and 338 us (gated 973 and 891).
+//   The tile follows the rows an expert has on average.  Of 32 experts, 2048 -> 7168 (gated, 7168 -> 2 x 2048):
+//       rows each                   43         58        115        130        172         460
+//       64-row tiles, us     101 (192)  113 (274)  147 (428)                       457 (1403)
+//       128-row tiles        107 (210)  112 (229)  124 (370)  152 (500)  180 (530)  328 (1042)
+//       256-row tiles                   151 (445)  155 (457)  155 (458)  160 (457)   303 (895)
+//   With most rows at a few experts the two larger ones change order a little later: 172 rows each, 178 (619) and 188 us (617).
 //   Smaller tiles, where the larger ones do not go round the compute units.
 //   The stream kernel, whose wavefronts share out the inner columns, where the smallest do not either: one token's eight experts,
 //   gated, 7168 -> 2048, 47 us against 93; 115 rows of 128 experts, 768 -> 2048, 42 us against 29 with 64-row tiles.
@@ -1031,7 +1043,7 @@ int tile_rows(int64_t rows, int64_t experts, int inner, int columns, int out_col
     const int64_t each = rows / experts, column_tiles = (out_columns + out_columns_each - 1) / out_columns_each;
     const int64_t owners = experts < rows ? experts : rows;
     for (const int tile : {256, 128, 64}) {
-        const bool suits = tile == 64 || each > tile;
+        const bool suits = tile == 64 || each > (tile == 256 ? 128 : 48);
         if (suits && (rows / tile > owners ? rows / tile : owners) * column_tiles >= cus)
             return tile;
     }
