@@ -210,8 +210,13 @@ __device__ __forceinline__ void loaded_but_newest() {
 // kRows * 16 rows; its four wavefronts take every fourth block of 128 inner columns, sum the blocks' products, each
 // times its two scales, in fp32 registers, and add their sums through LDS.  Each wavefront has a ring of kDepth blocks' operands in
 // LDS of its own, filled straight from memory, whole 128-byte lines at a time, and needs no barrier to read it: kDepth - 1
-// blocks are on their way.  (Two blocks' operands in registers, loaded there in their layout, took the same time on one token's
-// eight experts; what is left there is the workgroups' start, their sums and the scales' launch.)  A gated product takes half of its column tiles from the gate and half from the up weights.
+// blocks are on their way.  A gated product takes half of its column tiles from the gate and half from the up weights,
+// and leaves fp32 rows to quantize_rows_kernel, since no workgroup has the 128 columns of a scale.
+//
+// Measured: one token's eight experts, gated, 7168 -> 2 x 2048 (223 MB of weights): 40 to 47 us, 5.0 TB/s, and 4 for the
+// scales' launch.  What is left is the workgroups' start and their sums.  Two blocks' operands in registers, loaded there in
+// their layout, took the same time; eight wavefronts that have a whole group's columns and need no second launch 53 us
+// against 50 for both, and up to 2.8 times as long at smaller sizes.
 template <int kColumns, int kRows, int kDepth, bool kGated, bool kExact>
 __global__ void __launch_bounds__(kBlockThreads) experts_stream_kernel(const Product p, void* __restrict__ out, int64_t out_stride, int row_tiles) {
     constexpr int kTileBytes = kTile * kScaleBlock;
@@ -515,10 +520,12 @@ __device__ __forceinline__ int list_tiles(const Product& p, int column_tiles, ui
 // A lane's four columns of a tile are 8 bytes of bf16: neighbouring column tiles swap halves first, so that half as many
 // stores write twice as much each (2048 -> 7168 557 us against 597).
 //
-// Measured (32 experts, 29500 rows): 2048 -> 7168 557 us, 1.55 PFLOP/s; gated 7168 -> 2 x 2048 1650 us, 1.05 PFLOP/s (its bf16
-// instructions have half the rate).  A block of a tile takes 2.0 us; its matrix instructions alone take 0.98 us, its
-// loads alone 1.36 us: 64 KB that L2 hands out in 64-byte requests, of which a block of all tiles needs about as many
-// clocks as its matrix instructions.  One block's time ahead for the weights, the loads alone took 1.76 us.
+// Measured (32 experts, 29500 rows): 2048 -> 7168 547 to 557 us, 1.55 PFLOP/s, matrix instructions busy for 40 % of the clocks, which
+// are down to 1.83 GHz; gated 7168 -> 2 x 2048 1650 to 1690 us, 1.04 PFLOP/s, 47 % at 1.99 GHz (its bf16 instructions have half the
+// rate); 64 experts of 28 rows, gated, 4096 -> 2 x 2048, 64-row tiles: 202 us, 5.4 TB/s.  With 8 bytes a store a block of a 256-row
+// tile took 2.0 us; its matrix instructions alone take 0.98 us, its loads alone 1.36 us: 64 KB that L2 hands out in
+// 64-byte requests, of which a block of all tiles needs about as many clocks as its matrix instructions.  One block's time
+// ahead for the weights, the loads alone took 1.76 us.
 template <int kRowTiles, int kColTiles, int kRowWaves, int kColWaves, bool kGated>
 __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
     experts_tile_kernel(const Product p, char* __restrict__ out, int64_t out_stride, int column_tiles, XcdMap xcds) {
@@ -926,7 +933,8 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
     }
 }
 
-// fp32 rows in 8 bits with a scale for every 128 columns: a wavefront a row, 16 lanes a group of 128 columns.
+// fp32 rows in 8 bits with a scale for every 128 columns: a wavefront a row, 16 lanes a group of 128 columns.  Few rows
+// behind a product of few rows, so that its time is a launch's: eight rows of 2048 4.1 us.
 __global__ void __launch_bounds__(kBlockThreads) quantize_rows_kernel(const float* __restrict__ rows,
                                                                       char* __restrict__ records,
                                                                       int64_t num_rows,

@@ -11,10 +11,11 @@ constexpr int kMostNormVectors = 8;  // 16-byte vectors of a row that a lane hol
 // One workgroup a row: s = x + residual, r = 1 / sqrt(mean(s^2) + eps), n = s * r * gamma; then, for every 128
 // columns, scale = max |n| / 448 and the values n / scale, rounded to e4m3.  The row stays in registers
 // between its sum of squares and its output (kVectors 16-byte vectors a lane, 8 columns each), so that every
-// input byte is read once, all of them ahead of anything else; s and n are fp32 throughout, and each output is rounded from them once.  16
-// neighbouring lanes hold the 128 columns of a scale.  HBM-bound: 4096 x 7168 with both bf16 outputs 48.3 us, 5.5 TB/s (outputs
-// with plain stores and gamma read behind the sum: 54.0), 8192 x 2048 24.7 us, 6.1 TB/s; nontemporal loads of the inputs take 44.9
-// and 27.2 us, but would pass over inputs that the last kernel left in the caches.
+// input byte is read once, all of them ahead of anything else; s and n are fp32 throughout, and each output is rounded
+// from them once.  16 neighbouring lanes hold the 128 columns of a scale.  HBM-bound: 4096 x 7168 with both bf16 outputs
+// (265 MB) 40 to 42 us, 6.3 TB/s, 44.7 a call among others; one token 2.6.  Side by side, back to back: 48.3 us (with plain stores and
+// gamma read behind the sum 54.0), 8192 x 2048 24.7; nontemporal loads of the inputs take 44.9 and 27.2 there, but would pass
+// over inputs that the last kernel left in the caches.
 template <int kVectors>
 __global__ void __launch_bounds__(kMostNormThreads) rms_norm_fp8_kernel(const u32x4* __restrict__ x,         // [T][vectors]
                                                                        const u32x4* __restrict__ residual,  // [T][vectors] or null
