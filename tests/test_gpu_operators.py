@@ -163,6 +163,22 @@ def test_experts_gated(device, tuning, segments, inner, columns, kernel):
     assert torch.equal(again.payload.view(torch.int16), got.payload.view(torch.int16))
 
 
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("alignment", [1, 16])
+def test_products_of_counts_around_every_row_tile(device, tuning, monkeypatch, alignment, kernel):
+    """A matrix instruction has 16 rows; tiles leave out those of their row tiles that hold no row."""
+    tuning("EXPERTS_TILE", kernel)
+    counts = [16 * tiles + more for tiles in range(9) for more in (-1, 0, 1) if 16 * tiles + more > 0]
+    monkeypatch.setitem(SEGMENTS, "edges", (counts, alignment, 5))
+    values, scales, weight, offsets, counts = make_product("edges", 272, 288, 31 + alignment)
+    z, slack = oracle.experts(values, scales, weight.values, weight.scales, offsets, counts)
+    rows, weight, layout = records_of(values, scales, device), on(device, weight), (offsets.to(device), counts.to(device))
+    print("counts around row tiles", alignment, kernel, flush=True)
+    close(ep.experts_linear(rows, weight, *layout), z, slack)
+    got = ep.experts_gated(rows, weight, *layout)
+    oracle.check_eight_bits(got.values.cpu(), got.scales.cpu(), *oracle.gated(z, slack))
+
+
 @pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 31, 33, 64, 65, 100, 129, 300])
 @pytest.mark.parametrize("kernel", KERNELS)
 def test_products_without_a_layout_are_one_experts(device, rows, tuning, kernel):
