@@ -531,7 +531,7 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
     experts_tile_kernel(const Product p, char* __restrict__ out, int64_t out_stride, int column_tiles, XcdMap xcds) {
     using Shape = TileShape<kRowTiles, kColTiles, kRowWaves, kColWaves, kGated>;
     constexpr int kStages = Shape::kStages;
-    constexpr bool kSkips = kGated && kRowTiles <= 4;
+    constexpr bool kSkips = kGated && kRowTiles <= 4, kHalves = !kGated && kRowTiles > 4;
     constexpr int kRowStep = kRowWaves * kTile;  // the row wavefronts' row tiles alternate
     constexpr int kWeightBytes = Shape::kCols * kScaleBlock, kRowBytes = Shape::kRows * kScaleBlock;
     // accesses of a wavefront that are newer than the next block's operands when it asks for those
@@ -762,8 +762,12 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                 }
                 // Row tiles without a live row are left out of a gated product's small tiles, whose few rows an expert its
                 // 16-bit instructions take longer with than the weights' way from memory (32 experts of 16 rows 188 us against
-                // 238).  A linear product gains nothing by it, and the 256-row tile has no registers for the branches.
+                // 238); small linear ones gain nothing by it.  A linear 256-row tile that is at most half full leaves out most
+                // of its other half in one branch: 32 experts of 130 rows 145 us against 156, 60 of 154 94.5 against 98,
+                // 32 of 920 560 against 582 (a branch a row tile: 150, 97.3, 587).  A gated one has no registers for either
+                // (1690 us would be 2000).
                 const int live_tiles = kSkips ? __builtin_amdgcn_readfirstlane((static_cast<int>(live) - row_wave * kTile + kRowStep - 1) / kRowStep) : kRowTiles;
+                const bool half_full = kHalves && __builtin_amdgcn_readfirstlane(static_cast<int>(live)) <= kRowTiles / 2 * kRowStep;
                 int block = first_block(item);
                 for (int turn = 0; turn < p.blocks; ++turn) {
                     float column_scale[kScales];
@@ -776,6 +780,9 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                     }
 #pragma unroll
                     for (int r = 0; r < kRowTiles; ++r) {
+                        // (the last one's step has the way to the next block in it: it works on rows of the one before, whose sums nobody stores)
+                        if (kHalves && r >= kRowTiles / 2 && r + 1 < kRowTiles && half_full)
+                            continue;
                         __builtin_amdgcn_sched_barrier(0);
                         if (r == kRefill) {
                             // every wavefront has read the block's weights: the next but one's may come
