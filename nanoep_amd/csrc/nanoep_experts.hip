@@ -520,8 +520,8 @@ __device__ __forceinline__ int list_tiles(const Product& p, int column_tiles, ui
 // A lane's four columns of a tile are 8 bytes of bf16: neighbouring column tiles swap halves first, so that half as many
 // stores write twice as much each (2048 -> 7168 557 us against 597).
 //
-// Measured (32 experts, 29500 rows): 2048 -> 7168 547 to 557 us, 1.55 PFLOP/s, matrix instructions busy for 40 % of the clocks, which
-// are down to 1.83 GHz; gated 7168 -> 2 x 2048 1650 to 1690 us, 1.04 PFLOP/s, 47 % at 1.99 GHz (its bf16 instructions have half the
+// Measured (32 experts, 29500 rows): 2048 -> 7168 547 to 565 us, 1.55 PFLOP/s, matrix instructions busy for 38 % of the clocks, which
+// are down to 1.85 GHz; gated 7168 -> 2 x 2048 1650 to 1690 us, 1.04 PFLOP/s, 47 % at 1.99 GHz (its bf16 instructions have half the
 // rate); 64 experts of 28 rows, gated, 4096 -> 2 x 2048, 64-row tiles: 202 us, 5.4 TB/s.  With 8 bytes a store a block of a 256-row
 // tile took 2.0 us; its matrix instructions alone take 0.98 us, its loads alone 1.36 us: 64 KB that L2 hands out in
 // 64-byte requests, of which a block of all tiles needs about as many clocks as its matrix instructions.  One block's time
