@@ -145,23 +145,16 @@ __device__ __forceinline__ bf16x8 widened(int low, int high) {
 // and of activation row l % 16 and gets the products of weight rows 4 * (l / 16) .. + 3 with activation row l % 16.
 // Which of the block's columns a lane holds does not matter as long as both operands agree.
 //
-// The 8-bit matrix instruction adds its products with some 14 bits below the largest of them: on normal
-// inputs the sum of a block is off by 1.5e-5 of its deviation, without a bias, however many blocks follow.  Under the bf16
-// rounding of a linear product's output (1.7e-3) that does not show.  A gated product's scales are fp32 outputs, where it
-// would be the largest error there is, so kExact widens the operands to bf16, whose products and sums the 16-bit
-// instruction takes in fp32 (1e-7), at half the rate.
-template <bool kExact>
+// The operands are widened to bf16, whose products and sums the 16-bit instruction takes in fp32 (off by 1e-7 of a block's
+// deviation).  The 8-bit instruction has twice the rate, but adds its products with some 14 bits below the largest of them:
+// 1.5e-5 on normal inputs, and where large products cancel, small ones beside them are lost.
 __device__ __forceinline__ f32x4 block_product(const i32x8 weight, const i32x8 row) {
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (kExact) {
 #pragma unroll
-        for (int part = 0; part < 4; ++part)
-            sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widened(weight[2 * part], weight[2 * part + 1]),
-                                                          widened(row[2 * part], row[2 * part + 1]), sum, 0, 0, 0);
-        return sum;
-    } else {
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(weight, row, sum, 0, 0, 0, 0, 0, 0);
-    }
+    for (int part = 0; part < 4; ++part)
+        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widened(weight[2 * part], weight[2 * part + 1]),
+                                                      widened(row[2 * part], row[2 * part + 1]), sum, 0, 0, 0);
+    return sum;
 }
 
 __device__ __forceinline__ float silu(float v) { return v / (1.0f + __expf(-v)); }
@@ -217,7 +210,7 @@ __device__ __forceinline__ void loaded_but_newest() {
 // scales' launch.  What is left is the workgroups' start and their sums.  Two blocks' operands in registers, loaded there in
 // their layout, took the same time; eight wavefronts that have a whole group's columns and need no second launch 53 us
 // against 50 for both, and up to 2.8 times as long at smaller sizes.
-template <int kColumns, int kRows, int kDepth, bool kGated, bool kExact>
+template <int kColumns, int kRows, int kDepth, bool kGated>
 __global__ void __launch_bounds__(kBlockThreads) experts_stream_kernel(const Product p, void* __restrict__ out, int64_t out_stride, int row_tiles) {
     constexpr int kTileBytes = kTile * kScaleBlock;
     constexpr int kScalesAt = (kColumns + kRows) * kTileBytes, kBlockBytes = kScalesAt + kWave * 4;
@@ -319,7 +312,7 @@ __global__ void __launch_bounds__(kBlockThreads) experts_stream_kernel(const Pro
                 const float row_scale = reinterpret_cast<const float*>(from + kScalesAt)[r * kTile + in_tile];
 #pragma unroll
                 for (int c = 0; c < kColumns; ++c) {
-                    const f32x4 product = block_product<kExact>(weights[c], row);
+                    const f32x4 product = block_product(weights[c], row);
                     const float factor = weight_scale[c] * row_scale;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -518,20 +511,18 @@ __device__ __forceinline__ int list_tiles(const Product& p, int column_tiles, ui
 // operands so arrive while this one's output is written.
 //
 // A lane's four columns of a tile are 8 bytes of bf16: neighbouring column tiles swap halves first, so that half as many
-// stores write twice as much each (2048 -> 7168 557 us against 597).
+// stores write twice as much each (60 experts, 1424 -> 2816: 140 us against 149).
 //
-// Measured (32 experts, 29500 rows): 2048 -> 7168 547 to 565 us, 1.55 PFLOP/s, matrix instructions busy for 38 % of the clocks, which
-// are down to 1.85 GHz; gated 7168 -> 2 x 2048 1650 to 1690 us, 1.04 PFLOP/s, 47 % at 1.99 GHz (its bf16 instructions have half the
-// rate); 64 experts of 28 rows, gated, 4096 -> 2 x 2048, 64-row tiles: 202 us, 5.4 TB/s.  With 8 bytes a store a block of a 256-row
-// tile took 2.0 us; its matrix instructions alone take 0.98 us, its loads alone 1.36 us: 64 KB that L2 hands out in
-// 64-byte requests, of which a block of all tiles needs about as many clocks as its matrix instructions.  One block's time
-// ahead for the weights, the loads alone took 1.76 us.
+// Measured (32 experts, 29500 rows): 2048 -> 7168 828 to 852 us, 1.03 PFLOP/s; gated 7168 -> 2 x 2048 1650 to 1690 us, 1.04 PFLOP/s:
+// 81 % of what a large library product reaches in bf16.  64 experts of 28 rows, gated, 4096 -> 2 x 2048, 64-row tiles: 202 us, 5.4
+// TB/s.  The loads of a 256-row tile's block alone take 1.36 us of its 3.0: 64 KB that L2 hands out in 64-byte requests; with one
+// block's time ahead for the weights they took 1.76 us.
 template <int kRowTiles, int kColTiles, int kRowWaves, int kColWaves, bool kGated>
 __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
     experts_tile_kernel(const Product p, char* __restrict__ out, int64_t out_stride, int column_tiles, XcdMap xcds) {
     using Shape = TileShape<kRowTiles, kColTiles, kRowWaves, kColWaves, kGated>;
     constexpr int kStages = Shape::kStages;
-    constexpr bool kSkips = kGated && kRowTiles <= 4, kHalves = !kGated && kRowTiles > 4;
+    constexpr bool kSkips = kRowTiles <= 4;
     constexpr int kRowStep = kRowWaves * kTile;  // the row wavefronts' row tiles alternate
     constexpr int kWeightBytes = Shape::kCols * kScaleBlock, kRowBytes = Shape::kRows * kScaleBlock;
     // accesses of a wavefront that are newer than the next block's operands when it asks for those
@@ -619,7 +610,7 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
             } else {
 #pragma unroll
                 for (int i = 0; i < Shape::kWeightLoads; ++i)
-                    load_to_lds<16>(at + piece * 16 < p.inner ? weight + at + weight_offset[i] + piece * 16 : reinterpret_cast<const char*>(&kZeroPiece),
+                    load_to_lds<16>(at + piece * 16 < p.inner ? weight + at + static_cast<uint32_t>(afresh(static_cast<int>(weight_offset[i]))) + piece * 16 : reinterpret_cast<const char*>(&kZeroPiece),
                                 to + i * kStep);
             }
             weight_slot = after(weight_slot);
@@ -665,7 +656,7 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
             } else {
 #pragma unroll
                 for (int i = 0; i < Shape::kRowLoads; ++i)
-                    load_to_lds<16>(at + piece * 16 < p.inner ? values + at + row_offset[i] + piece * 16 : reinterpret_cast<const char*>(&kZeroPiece),
+                    load_to_lds<16>(at + piece * 16 < p.inner ? values + at + static_cast<uint32_t>(afresh(static_cast<int>(row_offset[i]))) + piece * 16 : reinterpret_cast<const char*>(&kZeroPiece),
                                 to + i * kStep);
             }
             // (where there are more wavefronts than 64 rows, some bring in the same scales)
@@ -691,18 +682,13 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
         const auto row_piece = [&](int in_slot, int r, int half) {
             return *reinterpret_cast<const u32x4*>(row_blocks[in_slot] + row_at + r * kRowStep * kScaleBlock + (turned ^ half * 64));
         };
-        i32x8 weights[kGated ? 1 : kColTiles];
-        bf16x8 wide_weights[kGated ? kColTiles : 1][4];
+        bf16x8 wide_weights[kColTiles][4];
         const auto read_weights = [&](int in_slot, int c) {
             const u32x4 low = weight_piece(in_slot, c, 0), high = weight_piece(in_slot, c, 1);
-            if constexpr (kGated) {
-                wide_weights[c][0] = widened(low.x, low.y);
-                wide_weights[c][1] = widened(low.z, low.w);
-                wide_weights[c][2] = widened(high.x, high.y);
-                wide_weights[c][3] = widened(high.z, high.w);
-            } else {
-                weights[c] = operand(low, high);
-            }
+            wide_weights[c][0] = widened(low.x, low.y);
+            wide_weights[c][1] = widened(low.z, low.w);
+            wide_weights[c][2] = widened(high.x, high.y);
+            wide_weights[c][3] = widened(high.z, high.w);
         };
         u32x4 rows[2][2];
         float scale[2];
@@ -760,14 +746,11 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                     weight_scales[c] = p.weight_scales + (static_cast<int64_t>(item.expert) * p.column_blocks + column / kScaleBlock) * p.blocks;
                     next_scale[c] = uniform_load(weight_scales[c] + first_block(item));
                 }
-                // Row tiles without a live row are left out of a gated product's small tiles, whose few rows an expert its
-                // 16-bit instructions take longer with than the weights' way from memory (32 experts of 16 rows 188 us against
-                // 238); small linear ones gain nothing by it.  A linear 256-row tile that is at most half full leaves out most
-                // of its other half in one branch: 32 experts of 130 rows 145 us against 156, 60 of 154 94.5 against 98,
-                // 32 of 920 560 against 582 (a branch a row tile: 150, 97.3, 587).  A gated one has no registers for either
-                // (1690 us would be 2000).
+                // Row tiles without a live row are left out of small tiles, whose few rows an expert the matrix instructions take
+                // longer with than the weights' way from memory: gated, 32 experts of 16 rows 188 us against 238; linear,
+                // 128 experts of 1 row 30.6 against 35.7.  A 256-row tile has no registers for it (gated 1690 us would be 2000), nor
+                // for one branch over its other half where it is half full (linear, 2048 -> 7168 828 us would be 982).
                 const int live_tiles = kSkips ? __builtin_amdgcn_readfirstlane((static_cast<int>(live) - row_wave * kTile + kRowStep - 1) / kRowStep) : kRowTiles;
-                const bool half_full = kHalves && __builtin_amdgcn_readfirstlane(static_cast<int>(live)) <= kRowTiles / 2 * kRowStep;
                 int block = first_block(item);
                 for (int turn = 0; turn < p.blocks; ++turn) {
                     float column_scale[kScales];
@@ -780,9 +763,6 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                     }
 #pragma unroll
                     for (int r = 0; r < kRowTiles; ++r) {
-                        // (the last one's step has the way to the next block in it: it works on rows of the one before, whose sums nobody stores)
-                        if (kHalves && r >= kRowTiles / 2 && r + 1 < kRowTiles && half_full)
-                            continue;
                         __builtin_amdgcn_sched_barrier(0);
                         if (r == kRefill) {
                             // every wavefront has read the block's weights: the next but one's may come
@@ -811,8 +791,7 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
 #pragma unroll
                         for (int c = 0; c < kColTiles; ++c)
                             product[c] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        if (kSkips && r >= live_tiles) {
-                        } else if constexpr (kGated) {
+                        if (!kSkips || r < live_tiles) {
 #pragma unroll
                             for (int part = 0; part < 4; ++part) {
                                 const u32x4 raw = rows[r & 1][part / 2];
@@ -821,11 +800,6 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                                 for (int c = 0; c < kColTiles; ++c)
                                     product[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wide_weights[c][part], wide, product[c], 0, 0, 0);
                             }
-                        } else {
-                            const i32x8 row = operand(rows[r & 1][0], rows[r & 1][1]);
-#pragma unroll
-                            for (int c = 0; c < kColTiles; ++c)
-                                product[c] = block_product<false>(weights[c], row);
                         }
                         if (r + 1 == kRowTiles) {
                             __builtin_amdgcn_sched_barrier(0);
@@ -1002,7 +976,7 @@ int product_of(const void* values, int64_t value_stride, const float* scales, in
 // Most tiles of kRows rows that the experts' rows can have: each expert's but the full ones end in one that is not.
 int64_t most_row_tiles(const Product& p, int rows) { return p.rows / rows + (p.experts < p.rows ? p.experts : p.rows); }
 
-template <int kColumns, int kRows, int kDepth, bool kGated, bool kExact>
+template <int kColumns, int kRows, int kDepth, bool kGated>
 int launch_stream(const Product& p, void* out, int64_t out_stride, hipStream_t stream) {
     const int out_columns = kGated ? p.columns / 2 : p.columns;
     constexpr int kOutColumns = (kGated ? kColumns / 2 : kColumns) * kTile;
@@ -1010,7 +984,7 @@ int launch_stream(const Product& p, void* out, int64_t out_stride, hipStream_t s
     const int64_t gaps = p.expert_offsets != nullptr ? ((p.experts + int64_t{1}) * kGapParts + column_tiles - 1) / column_tiles : 0;
     if (tiles + gaps > 0x7fffffff || column_tiles > 65535)
         return NANOEP_ERR_INVALID_ARGUMENT;
-    experts_stream_kernel<kColumns, kRows, kDepth, kGated, kExact>
+    experts_stream_kernel<kColumns, kRows, kDepth, kGated>
         <<<dim3(static_cast<unsigned>(tiles + gaps), static_cast<unsigned>(column_tiles)), kBlockThreads, 0, stream>>>(p, out, out_stride,
                                                                                                                       static_cast<int>(tiles));
     NANOEP_HIP_TRY(hipGetLastError());
@@ -1037,13 +1011,13 @@ int launch_tiles(const Product& p, void* out, int64_t out_stride, hipStream_t st
 // Rows of the tile kernel's tiles for a product, 0 for the stream kernel.
 //   The tile follows the rows an expert has on average.  Of 32 experts, 2048 -> 7168 (gated, 7168 -> 2 x 2048):
 //       rows each                   43         58        115        130        172         460
-//       64-row tiles, us     101 (192)  113 (274)  147 (428)                       457 (1403)
-//       128-row tiles        107 (210)  112 (229)  124 (370)  152 (500)  180 (530)  328 (1042)
-//       256-row tiles                   151 (445)  155 (457)  155 (458)  160 (457)   303 (895)
-//   With most rows at a few experts the two larger ones change order a little later: 172 rows each, 178 (619) and 188 us (617).
+//       64-row tiles, us     107 (192)  129 (274)  193 (428)  233        260        663 (1403)
+//       128-row tiles        116 (210)  122 (229)  153 (370)  202 (500)  246 (530)  491 (1042)
+//       256-row tiles        225        225 (445)  228 (457)  230 (458)  234 (457)  428 (895)
+//   With most rows at a few experts the two larger ones change order a little later: 172 rows each, 266 (619) and 287 us (617).
 //   Smaller tiles, where the larger ones do not go round the compute units.
 //   The stream kernel, whose wavefronts share out the inner columns, where the smallest do not either: one token's eight experts,
-//   gated, 7168 -> 2048, 47 us against 93; 115 rows of 128 experts, 768 -> 2048, 42 us against 29 with 64-row tiles.
+//   gated, 7168 -> 2048, 47 us against 93; 768 -> 2048, 7.4 us against 15.1; 115 rows of 128 experts of these 43 us, 31 with 64-row tiles.
 //   And for addresses beyond the tile kernel's: an expert's weight and a tile's rows, in and out, lie within 32-bit offsets, its list
 //   of tiles is made from at most kMostSegments experts.
 int tile_rows(int64_t rows, int64_t experts, int inner, int columns, int out_columns_each, int out_columns, int64_t value_stride, int64_t scale_stride) {
@@ -1075,17 +1049,14 @@ int launch_product(const Product& p, void* out, int64_t out_stride, int tile, hi
 }
 
 // `out_stride` in values: bf16 ones, or a gated product's fp32 ones.
-template <bool kGated, bool kExact>
+template <bool kGated>
 int launch_streams(const Product& p, void* out, int64_t out_stride, hipStream_t stream) {
     if (p.rows / p.experts <= 16)
-        return launch_stream<2, 1, 3, kGated, kExact>(p, out, out_stride, stream);
-    return launch_stream<2, 4, 2, kGated, kExact>(p, out, out_stride, stream);
+        return launch_stream<2, 1, 3, kGated>(p, out, out_stride, stream);
+    return launch_stream<2, 4, 2, kGated>(p, out, out_stride, stream);
 }
 
 int linear_tile_rows(const Product& p) {
-    // up to 64 inner columns the 16-bit instructions take no longer than the one 128-wide 8-bit one
-    if (p.inner <= kScaleBlock / 2)
-        return 0;
     return tile_rows(p.rows, p.experts, p.inner, p.columns, TileShape<8, 4, 2, 4, false>::kOutCols, p.columns, p.value_stride, p.scale_stride);
 }
 
@@ -1112,7 +1083,7 @@ int nanoep_experts_linear(const void* values, int64_t value_stride, const float*
     const auto on = static_cast<hipStream_t>(stream);
     if (const int tile = linear_tile_rows(p))
         return launch_product<false>(p, out, static_cast<int64_t>(columns) * 2, tile, on);
-    return inner <= kScaleBlock / 2 ? launch_streams<false, true>(p, out, columns, on) : launch_streams<false, false>(p, out, columns, on);
+    return launch_streams<false>(p, out, columns, on);
 }
 
 size_t nanoep_experts_gated_workspace_bytes(int64_t rows, int64_t experts, int inner, int columns, int64_t value_stride,
@@ -1142,7 +1113,7 @@ int nanoep_experts_gated(const void* values, int64_t value_stride, const float* 
     const auto on = static_cast<hipStream_t>(stream);
     if (const int tile = gated_tile_rows(rows, experts, inner, columns, value_stride, scale_stride))
         return launch_product<true>(p, records, record_bytes_of(columns / 2), tile, on);
-    const int launched = launch_streams<true, true>(p, workspace, columns / 2, on);
+    const int launched = launch_streams<true>(p, workspace, columns / 2, on);
     if (launched != NANOEP_OK)
         return launched;
     const unsigned blocks = static_cast<unsigned>((rows + kWavesPerBlock - 1) / kWavesPerBlock);
