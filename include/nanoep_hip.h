@@ -320,7 +320,7 @@ int nanoep_rms_norm_fp8(const void* x, const void* residual, const void* gamma, 
  * and [E], as nanoep_layout writes them); the rows up to expert_offsets[e + 1], and those behind the last segment, are no
  * expert's: their outputs are zero and their inputs are not looked at.  Both NULL: one expert, all rows.
  * Values and scales that point outside the rows are never followed.
- *   linear : out[s] = z[s], bf16 [rows, columns]; columns % 8 == 0
+ *   linear : out[s] = z[s], bf16 [rows, columns]; columns % 8 == 0, columns <= 2^24 (a gated product's as well)
  *   gated  : records of silu(z[s][n]) * z[s][columns / 2 + n], n < columns / 2; columns % 32 == 0; needs
  *            nanoep_experts_gated_workspace_bytes of device scratch (may be 0)
  * values: rows value_stride bytes apart (a multiple of 16, at least inner); scales: rows scale_stride floats apart;

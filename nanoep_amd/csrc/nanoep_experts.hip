@@ -211,7 +211,8 @@ __device__ __forceinline__ void loaded_but_newest() {
 // their layout, took the same time; eight wavefronts that have a whole group's columns and need no second launch 53 us
 // against 50 for both, and up to 2.8 times as long at smaller sizes.
 template <int kColumns, int kRows, int kDepth, bool kGated>
-__global__ void __launch_bounds__(kBlockThreads) experts_stream_kernel(const Product p, void* __restrict__ out, int64_t out_stride, int row_tiles) {
+__global__ void __launch_bounds__(kBlockThreads)
+    experts_stream_kernel(const Product p, void* __restrict__ out, int64_t out_stride, int row_tiles, int first_column_tile) {
     constexpr int kTileBytes = kTile * kScaleBlock;
     constexpr int kScalesAt = (kColumns + kRows) * kTileBytes, kBlockBytes = kScalesAt + kWave * 4;
     constexpr int kLoads = 2 * (kColumns + kRows) + 1;  // of a block
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(kBlockThreads) experts_stream_kernel(const Pro
     const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int group = lane / kTile, in_tile = lane % kTile;
-    const int first_column = static_cast<int>(blockIdx.y) * kOutTiles * kTile;
+    const int first_column = (first_column_tile + static_cast<int>(blockIdx.y)) * kOutTiles * kTile;
 
     f32x4 acc[kColumns][kRows];
 #pragma unroll
@@ -954,11 +955,13 @@ __global__ void __launch_bounds__(kBlockThreads) quantize_rows_kernel(const floa
         reinterpret_cast<uint32_t*>(record)[word] = 0u;
 }
 
+constexpr int kMostColumns = 1 << 24;
+
 int product_of(const void* values, int64_t value_stride, const float* scales, int64_t scale_stride, const void* weight,
                const float* weight_scales, const int64_t* expert_offsets, const int64_t* expert_counts, int64_t rows, int64_t experts,
                int inner, int columns, int column_multiple, Product& p) {
     if (rows < 0 || rows > 0x7fffffff || experts <= 0 || experts >= (int64_t{1} << 30) || inner <= 0 || inner % 16 != 0 || columns <= 0 ||
-        columns % column_multiple != 0 || (expert_offsets == nullptr) != (expert_counts == nullptr))
+        columns > kMostColumns || columns % column_multiple != 0 || (expert_offsets == nullptr) != (expert_counts == nullptr))
         return NANOEP_ERR_INVALID_ARGUMENT;
     if (expert_offsets == nullptr && experts != 1)
         return NANOEP_ERR_INVALID_ARGUMENT;
@@ -976,18 +979,24 @@ int product_of(const void* values, int64_t value_stride, const float* scales, in
 // Most tiles of kRows rows that the experts' rows can have: each expert's but the full ones end in one that is not.
 int64_t most_row_tiles(const Product& p, int rows) { return p.rows / rows + (p.experts < p.rows ? p.experts : p.rows); }
 
+constexpr int kMostGridSteps = 65535;  // of a launch's second axis
+
 template <int kColumns, int kRows, int kDepth, bool kGated>
 int launch_stream(const Product& p, void* out, int64_t out_stride, hipStream_t stream) {
     const int out_columns = kGated ? p.columns / 2 : p.columns;
     constexpr int kOutColumns = (kGated ? kColumns / 2 : kColumns) * kTile;
     const int64_t tiles = most_row_tiles(p, kRows * kTile), column_tiles = (out_columns + kOutColumns - 1) / kOutColumns;
-    const int64_t gaps = p.expert_offsets != nullptr ? ((p.experts + int64_t{1}) * kGapParts + column_tiles - 1) / column_tiles : 0;
-    if (tiles + gaps > 0x7fffffff || column_tiles > 65535)
-        return NANOEP_ERR_INVALID_ARGUMENT;
-    experts_stream_kernel<kColumns, kRows, kDepth, kGated>
-        <<<dim3(static_cast<unsigned>(tiles + gaps), static_cast<unsigned>(column_tiles)), kBlockThreads, 0, stream>>>(p, out, out_stride,
-                                                                                                                      static_cast<int>(tiles));
-    NANOEP_HIP_TRY(hipGetLastError());
+    // as many columns at a time as an axis of a grid has steps; the first launch clears the rows of no expert
+    for (int64_t first = 0; first < column_tiles; first += kMostGridSteps) {
+        const int64_t columns = std::min<int64_t>(column_tiles - first, kMostGridSteps);
+        const int64_t gaps = p.expert_offsets != nullptr && first == 0 ? ((p.experts + int64_t{1}) * kGapParts + columns - 1) / columns : 0;
+        if (tiles + gaps > 0x7fffffff)
+            return NANOEP_ERR_INVALID_ARGUMENT;
+        experts_stream_kernel<kColumns, kRows, kDepth, kGated>
+            <<<dim3(static_cast<unsigned>(tiles + gaps), static_cast<unsigned>(columns)), kBlockThreads, 0, stream>>>(
+                p, out, out_stride, static_cast<int>(tiles), static_cast<int>(first));
+        NANOEP_HIP_TRY(hipGetLastError());
+    }
     return NANOEP_OK;
 }
 

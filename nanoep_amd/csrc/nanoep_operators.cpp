@@ -170,7 +170,7 @@ ProductArguments require_product(const char* what, const torch::Tensor& values, 
         refuse(what, " weight must be [experts, columns, inner]");
     const int64_t experts = weight.size(0), columns = weight.size(1);
     if (experts <= 0 || experts >= (1 << 30) || columns <= 0 || columns % column_multiple != 0 || columns > (1 << 24))
-        refuse(what, " weight must have at least one expert and a positive multiple of ", column_multiple, " columns");
+        refuse(what, " weight must have at least one expert and a positive multiple of ", column_multiple, " columns, at most 2^24");
     require(weight, device, at::kFloat8_e4m3fn, {experts, columns, inner}, what, "weight");
     require(weight_scales, device, at::kFloat, {experts, (columns + kScaleBlock - 1) / kScaleBlock, groups}, what, "weight scales");
     require_aligned(values, what, "values");

@@ -140,7 +140,7 @@ def experts_linear(
 
     Expert e has the rows [expert_offsets[e], expert_offsets[e] + expert_counts[e]), as a handle's layout says (int64 [E + 1]
     from 0 on, and [E]); rows of no expert are zero, and what they hold is not looked at.  Without the two, all rows are the only
-    expert's.  inner is a multiple of 16, columns one of 8."""
+    expert's.  inner is a multiple of 16, columns one of 8, both at most 2^24."""
     return load_extension().experts_linear(rows.values, rows.scales, weight.values, weight.scales, expert_offsets, expert_counts)
 
 

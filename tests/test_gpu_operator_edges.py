@@ -40,3 +40,21 @@ def test_products_of_terms_that_cancel(device, tuning, inner, kernel):
     close(ep.experts_linear(on_device, on(device, weight), *layout), z, slack)
     got = ep.experts_gated(on_device, on(device, weight), *layout)
     oracle.check_eight_bits(got.values.cpu(), got.scales.cpu(), *oracle.gated(z, slack))
+
+
+@pytest.mark.parametrize("columns", [(1 << 21) + 32, 1 << 24])
+def test_products_of_more_columns_than_a_grid_axis_has_steps(device, columns):
+    """Whole numbers: every product and sum is exact.  A row behind the expert's, and one behind the last segment."""
+    generator = torch.Generator().manual_seed(columns)
+    inner, rows = 16, 5
+    layout = torch.tensor([0, 4], device=device), torch.tensor([3], device=device)
+    values = torch.randint(-4, 5, (rows, inner), generator=generator).float()
+    weight = torch.randint(-4, 5, (1, columns, inner), generator=generator, dtype=torch.int8).float()
+    rows_on = ep.Fp8Rows(values.to(torch.float8_e4m3fn).to(device), torch.ones(rows, 1, device=device))
+    weight_on = ep.Fp8Weight(weight.to(torch.float8_e4m3fn).to(device), torch.ones(1, oracle.groups(columns), 1, device=device))
+    z = values @ weight[0].T
+    z[3:] = 0
+    print("columns", columns, flush=True)
+    assert torch.equal(ep.experts_linear(rows_on, weight_on, *layout).cpu(), z.to(torch.bfloat16))
+    got = ep.experts_gated(rows_on, weight_on, *layout)
+    oracle.check_eight_bits(got.values.cpu(), got.scales.cpu(), *oracle.gated(z.double(), torch.zeros_like(z).double()))
