@@ -101,10 +101,8 @@ struct RowRange {
     int64_t begin;
     int64_t end;
 };
-__device__ __forceinline__ RowRange gap_part(const Product& p, int part) {
-    if (part >= (p.experts + 1) * kGapParts)
-        return {0, 0};
-    const Segment segment = segment_of(p, part / kGapParts);
+__device__ __forceinline__ RowRange gap_part(const Product& p, int64_t part) {
+    const Segment segment = segment_of(p, static_cast<int>(part / kGapParts));
     const int64_t begin = segment.begin + segment.live, rows = segment.end - begin;
     return {begin + rows * (part % kGapParts) / kGapParts, begin + rows * (part % kGapParts + 1) / kGapParts};
 }
@@ -212,7 +210,7 @@ __device__ __forceinline__ void loaded_but_newest() {
 // against 50 for both, and up to 2.8 times as long at smaller sizes.
 template <int kColumns, int kRows, int kDepth, bool kGated>
 __global__ void __launch_bounds__(kBlockThreads)
-    experts_stream_kernel(const Product p, void* __restrict__ out, int64_t out_stride, int row_tiles, int first_column_tile) {
+    experts_stream_kernel(const Product p, void* __restrict__ out, int64_t out_stride, int first_row_tile, int row_tiles, int first_column_tile) {
     constexpr int kTileBytes = kTile * kScaleBlock;
     constexpr int kScalesAt = (kColumns + kRows) * kTileBytes, kBlockBytes = kScalesAt + kWave * 4;
     constexpr int kLoads = 2 * (kColumns + kRows) + 1;  // of a block
@@ -225,11 +223,13 @@ __global__ void __launch_bounds__(kBlockThreads)
     if (static_cast<int>(blockIdx.x) >= row_tiles) {
         // workgroups of their own for the rows of no expert
         constexpr int kValueBytes = kGated ? 4 : 2;
-        clear_rows<false, kBlockThreads, kValueBytes>(static_cast<char*>(out), out_stride * kValueBytes, out_columns,
-                                                      gap_part(p, static_cast<int>((blockIdx.x - row_tiles) * gridDim.y + blockIdx.y)));
+        const int64_t workgroups = static_cast<int64_t>(gridDim.x - row_tiles) * gridDim.y;
+        for (int64_t part = static_cast<int64_t>(blockIdx.x - row_tiles) * gridDim.y + blockIdx.y; part < (p.experts + int64_t{1}) * kGapParts;
+             part += workgroups)
+            clear_rows<false, kBlockThreads, kValueBytes>(static_cast<char*>(out), out_stride * kValueBytes, out_columns, gap_part(p, part));
         return;
     }
-    const RowTile tile = find_row_tile<kRows * kTile>(p, static_cast<int>(blockIdx.x));
+    const RowTile tile = find_row_tile<kRows * kTile>(p, first_row_tile + static_cast<int>(blockIdx.x));
     if (tile.expert < 0)
         return;
     const int lane = threadIdx.x % kWave;
@@ -924,7 +924,7 @@ __global__ void __launch_bounds__(kBlockThreads) quantize_rows_kernel(const floa
                                                                       int columns,
                                                                       int groups) {
     const int lane = threadIdx.x % kWave;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + threadIdx.x / kWave;
+    const int64_t row = workgroup_number() * kWavesPerBlock + threadIdx.x / kWave;
     if (row >= num_rows)
         return;
     const float* from = rows + row * columns;
@@ -986,17 +986,17 @@ int launch_stream(const Product& p, void* out, int64_t out_stride, hipStream_t s
     const int out_columns = kGated ? p.columns / 2 : p.columns;
     constexpr int kOutColumns = (kGated ? kColumns / 2 : kColumns) * kTile;
     const int64_t tiles = most_row_tiles(p, kRows * kTile), column_tiles = (out_columns + kOutColumns - 1) / kOutColumns;
-    // as many columns at a time as an axis of a grid has steps; the first launch clears the rows of no expert
-    for (int64_t first = 0; first < column_tiles; first += kMostGridSteps) {
-        const int64_t columns = std::min<int64_t>(column_tiles - first, kMostGridSteps);
-        const int64_t gaps = p.expert_offsets != nullptr && first == 0 ? ((p.experts + int64_t{1}) * kGapParts + columns - 1) / columns : 0;
-        if (tiles + gaps > 0x7fffffff)
-            return NANOEP_ERR_INVALID_ARGUMENT;
-        experts_stream_kernel<kColumns, kRows, kDepth, kGated>
-            <<<dim3(static_cast<unsigned>(tiles + gaps), static_cast<unsigned>(columns)), kBlockThreads, 0, stream>>>(
-                p, out, out_stride, static_cast<int>(tiles), static_cast<int>(first));
-        NANOEP_HIP_TRY(hipGetLastError());
-    }
+    // as many rows and columns at a time as the axes of a grid have steps; the first launch clears the rows of no expert
+    for (int64_t first_row = 0; first_row < tiles; first_row += kMostOnAxis)
+        for (int64_t first = 0; first < column_tiles; first += kMostGridSteps) {
+            const int64_t rows = std::min(tiles - first_row, kMostOnAxis), columns = std::min<int64_t>(column_tiles - first, kMostGridSteps);
+            const bool clears = p.expert_offsets != nullptr && first_row == 0 && first == 0;
+            const int64_t gaps = clears ? std::min(((p.experts + int64_t{1}) * kGapParts + columns - 1) / columns, kMostOnAxis) : 0;
+            experts_stream_kernel<kColumns, kRows, kDepth, kGated>
+                <<<dim3(static_cast<unsigned>(rows + gaps), static_cast<unsigned>(columns)), kBlockThreads, 0, stream>>>(
+                    p, out, out_stride, static_cast<int>(first_row), static_cast<int>(rows), static_cast<int>(first));
+            NANOEP_HIP_TRY(hipGetLastError());
+        }
     return NANOEP_OK;
 }
 
@@ -1125,8 +1125,7 @@ int nanoep_experts_gated(const void* values, int64_t value_stride, const float* 
     const int launched = launch_streams<true>(p, workspace, columns / 2, on);
     if (launched != NANOEP_OK)
         return launched;
-    const unsigned blocks = static_cast<unsigned>((rows + kWavesPerBlock - 1) / kWavesPerBlock);
-    quantize_rows_kernel<<<blocks, kBlockThreads, 0, on>>>(static_cast<const float*>(workspace), static_cast<char*>(records), rows,
+    quantize_rows_kernel<<<grid_of((rows + kWavesPerBlock - 1) / kWavesPerBlock), kBlockThreads, 0, on>>>(static_cast<const float*>(workspace), static_cast<char*>(records), rows,
                                                            record_bytes_of(columns / 2), columns / 2, static_cast<int>(scale_groups(columns / 2)));
     NANOEP_HIP_TRY(hipGetLastError());
     return NANOEP_OK;

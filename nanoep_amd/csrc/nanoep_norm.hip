@@ -23,13 +23,16 @@ __global__ void __launch_bounds__(kMostNormThreads) rms_norm_fp8_kernel(const u3
                                                                        char* __restrict__ records,
                                                                        u32x4* __restrict__ residual_out,  // [T][vectors] or null
                                                                        u32x4* __restrict__ normalized,    // [T][vectors] or null
+                                                                       int64_t rows,
                                                                        int vectors,
                                                                        int groups,
                                                                        int64_t record_bytes,
                                                                        float columns,
                                                                        float eps) {
     __shared__ float wave_sums[kMostNormThreads / kWave];
-    const int64_t row = blockIdx.x;
+    const int64_t row = workgroup_number();
+    if (row >= rows)
+        return;
     const int threads = blockDim.x;
     const u32x4* row_x = x + row * vectors;
     const u32x4* row_residual = residual + row * vectors;
@@ -144,11 +147,11 @@ int nanoep_rms_norm_fp8(const void* x, const void* residual, const void* gamma, 
     while (held < kMostNormVectors && (vectors + held - 1) / held > (held < wanted ? kWave : kMostNormThreads))
         held *= 2;
     const int threads = static_cast<int>(align_up(static_cast<size_t>((vectors + held - 1) / held), kWave));
-    const dim3 grid(static_cast<unsigned>(num_tokens));
+    const dim3 grid = grid_of(num_tokens);
 #define NANOEP_LAUNCH_NORM(HELD)                                                                                                        \
     rms_norm_fp8_kernel<HELD><<<grid, threads, 0, static_cast<hipStream_t>(stream)>>>(                                                  \
         static_cast<const u32x4*>(x), static_cast<const u32x4*>(residual), static_cast<const u32x4*>(gamma), static_cast<char*>(records), \
-        static_cast<u32x4*>(residual_out), static_cast<u32x4*>(normalized), vectors, static_cast<int>(scale_groups(hidden)),            \
+        static_cast<u32x4*>(residual_out), static_cast<u32x4*>(normalized), num_tokens, vectors, static_cast<int>(scale_groups(hidden)), \
         record_bytes_of(hidden), static_cast<float>(hidden), eps)
     if (held == 1)
         NANOEP_LAUNCH_NORM(1);

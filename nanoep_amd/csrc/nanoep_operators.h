@@ -22,6 +22,16 @@ inline int64_t record_bytes_of(int64_t columns) {
     return static_cast<int64_t>(align_up(static_cast<size_t>(columns + 4 * scale_groups(columns)), kRecordAlignment));
 }
 
+// A launch of any number of workgroups: an axis of a grid has fewer than 2^32 threads, so more go over two.  The last
+// row of such a grid may have workgroups too many, which return.
+constexpr int64_t kMostOnAxis = int64_t{1} << 21;  // workgroups, of 1024 threads at most
+inline dim3 grid_of(int64_t workgroups) {
+    if (workgroups <= kMostOnAxis)
+        return dim3(static_cast<unsigned>(workgroups));
+    return dim3(static_cast<unsigned>(kMostOnAxis), static_cast<unsigned>((workgroups + kMostOnAxis - 1) / kMostOnAxis));
+}
+__device__ __forceinline__ int64_t workgroup_number() { return static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x; }
+
 __device__ __forceinline__ float from_bf16_low(uint32_t packed) { return __uint_as_float(packed << 16); }
 __device__ __forceinline__ float from_bf16_high(uint32_t packed) { return __uint_as_float(packed & 0xffff0000u); }
 

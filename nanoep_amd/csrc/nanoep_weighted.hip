@@ -1,5 +1,7 @@
 // Combine with the gate weights applied, and its gradient.
 
+#include <algorithm>
+
 #include "nanoep_operators.h"
 
 namespace nanoep {
@@ -24,7 +26,7 @@ __global__ void __launch_bounds__(kBlockThreads) combine_weighted_kernel(const u
                                                                          int chunks,
                                                                          int num_topk) {
     const int lane = threadIdx.x % kWave;
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int64_t item = workgroup_number() * kWavesPerBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if (item >= work_items)
         return;
     const int64_t token = item / chunks;
@@ -70,8 +72,9 @@ __global__ void __launch_bounds__(kBlockThreads) combine_weighted_kernel(const u
 }
 
 // Zeros in a part of the rows of grad_y that no choice refers to: behind every expert's rows, and behind the last expert's
-// segment, each in kGapParts parts.
+// segment, each in kGapParts parts, at most kMostGapBlocks at a time.
 constexpr int kGapParts = 8;
+constexpr int64_t kMostGapBlocks = int64_t{1} << 20;
 constexpr int64_t kGapBytesApart = int64_t{32} << 20;
 __device__ __forceinline__ void clear_gap(const int64_t* expert_offsets, const int64_t* expert_counts, u32x4* rows, int64_t num_rows,
                                           int64_t num_experts, int vectors, int64_t part) {
@@ -109,15 +112,17 @@ __global__ void __launch_bounds__(kBlockThreads) combine_weighted_backward_kerne
                                                                                   int64_t num_experts,
                                                                                   int64_t y_rows,
                                                                                   int64_t pairs,
-                                                                                  uint32_t gap_blocks,
+                                                                                  int64_t gap_blocks,
                                                                                   int vectors,
                                                                                   int num_topk) {
-    if (blockIdx.x < gap_blocks) {
-        clear_gap(expert_offsets, expert_counts, grad_y, y_rows, num_experts, vectors, blockIdx.x);
+    const int64_t block = workgroup_number();
+    if (block < gap_blocks) {
+        for (int64_t part = block; part < (num_experts + 1) * kGapParts; part += gap_blocks)
+            clear_gap(expert_offsets, expert_counts, grad_y, y_rows, num_experts, vectors, part);
         return;
     }
     const int lane = threadIdx.x % kWave;
-    const int64_t pair = static_cast<int64_t>(blockIdx.x - gap_blocks) * kWavesPerBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int64_t pair = (block - gap_blocks) * kWavesPerBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if (pair >= pairs)
         return;
     const int64_t slot = token_slots[pair];
@@ -179,9 +184,7 @@ int nanoep_combine_weighted(const void* y, int64_t y_rows, const int32_t* token_
     const int chunks = (vectors + kWave - 1) / kWave;
     const int64_t items = num_tokens * chunks;
     const int64_t blocks = (items + kWavesPerBlock - 1) / kWavesPerBlock;
-    if (blocks > 0x7fffffff)
-        return NANOEP_ERR_INVALID_ARGUMENT;
-    combine_weighted_kernel<<<dim3(static_cast<unsigned>(blocks)), kBlockThreads, 0, static_cast<hipStream_t>(stream)>>>(
+    combine_weighted_kernel<<<grid_of(blocks), kBlockThreads, 0, static_cast<hipStream_t>(stream)>>>(
         static_cast<const u32x4*>(y), token_slots, weights, static_cast<const u32x4*>(bias), static_cast<u32x4*>(out), y_rows, items, vectors,
         chunks, num_topk);
     NANOEP_HIP_TRY(hipGetLastError());
@@ -209,18 +212,16 @@ int nanoep_combine_weighted_backward(const void* grad, const void* y, int64_t y_
         NANOEP_HIP_TRY(hipGetLastError());
     }
     const int64_t pairs = num_tokens * num_topk, pair_blocks = (pairs + kWavesPerBlock - 1) / kWavesPerBlock;
-    const int64_t gap_blocks = y_rows > 0 && expert_offsets != nullptr ? (num_local_experts + 1) * kGapParts : 0;
-    if (pair_blocks + gap_blocks > 0x7fffffff)
-        return NANOEP_ERR_INVALID_ARGUMENT;
+    const int64_t gap_blocks = y_rows > 0 && expert_offsets != nullptr ? std::min((num_local_experts + 1) * kGapParts, kMostGapBlocks) : 0;
     // Few rows to clear ride in the gradient's launch (9222 choices, 450 padding rows of 2816: 23.0 us, in a launch of their own
     // 28.8); many have one ahead of it, because writes alone and the gradient's mix go faster one after the other (29500
     // choices, 16200 padding rows of 7168: 197 us, beside one another 204).
     const bool apart = (y_rows - pairs) * hidden * 2 > kGapBytesApart;
     const auto launch = [&](int64_t gaps, int64_t blocks) {
         if (blocks > 0)
-            combine_weighted_backward_kernel<<<static_cast<unsigned>(blocks), kBlockThreads, 0, on>>>(
+            combine_weighted_backward_kernel<<<grid_of(blocks), kBlockThreads, 0, on>>>(
                 static_cast<const u32x4*>(grad), static_cast<const u32x4*>(y), token_slots, weights, static_cast<u32x4*>(grad_y), grad_weights,
-                expert_offsets, expert_counts, num_local_experts, y_rows, pairs, static_cast<uint32_t>(gaps), vectors, num_topk);
+                expert_offsets, expert_counts, num_local_experts, y_rows, pairs, gaps, vectors, num_topk);
     };
     if (apart)
         launch(gap_blocks, gap_blocks);

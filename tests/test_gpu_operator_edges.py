@@ -58,3 +58,70 @@ def test_products_of_more_columns_than_a_grid_axis_has_steps(device, columns):
     assert torch.equal(ep.experts_linear(rows_on, weight_on, *layout).cpu(), z.to(torch.bfloat16))
     got = ep.experts_gated(rows_on, weight_on, *layout)
     oracle.check_eight_bits(got.values.cpu(), got.scales.cpu(), *oracle.gated(z.double(), torch.zeros_like(z).double()))
+
+
+def test_products_of_more_row_tiles_than_a_grid_axis_has_threads_for(device, tuning):
+    """2^24 tiles of 64 rows, of 256 threads each; the same whole numbers over and over, in a period that no grid has."""
+    tuning("EXPERTS_TILE", 1)
+    period, inner, columns = 4_000_037, 16, 8
+    rows = (1 << 30) + 70
+    whole = torch.randint(-4, 5, (period, inner), device=device).float()
+    weight = torch.randint(-4, 5, (1, columns, inner), generator=torch.Generator().manual_seed(6)).float()
+    values = torch.empty(rows, inner, dtype=torch.float8_e4m3fn, device=device)
+    for part in range(0, rows, period):
+        values[part : part + period] = whole[: rows - part].to(torch.float8_e4m3fn)
+    scales = torch.ones(rows, 1, device=device)
+    want = (whole @ weight[0].T.to(device)).to(torch.bfloat16)
+    layout = torch.tensor([0, rows - 3], device=device), torch.tensor([rows - 5], device=device)
+    print("row tiles", rows, flush=True)
+    got = ep.experts_linear(ep.Fp8Rows(values, scales), ep.Fp8Weight(weight.to(torch.float8_e4m3fn).to(device), torch.ones(1, 1, 1, device=device)), *layout)
+    assert not got[rows - 5 :].any()
+    for part in range(0, rows - 5, period):
+        assert torch.equal(got[part : min(part + period, rows - 5)], want[: rows - 5 - part])
+
+
+# ------------------------------------------------------------------ norm and combine
+
+
+def test_rms_norm_of_more_rows_than_a_grid_axis_has_threads_for(device):
+    """2^26 rows, of 64 threads each."""
+    period, tokens = 4_000_037, (1 << 26) + 5
+    few = torch.randn(period, 16, device=device).to(torch.bfloat16)
+    x = torch.empty(tokens, 16, dtype=torch.bfloat16, device=device)
+    for part in range(0, tokens, period):
+        x[part : part + period] = few[: tokens - part]
+    gamma = torch.ones(16, dtype=torch.bfloat16, device=device)
+    print("rms_norm_fp8", tokens, flush=True)
+    got, want = ep.rms_norm_fp8(x, gamma).rows.payload.view(torch.int32), ep.rms_norm_fp8(few, gamma).rows.payload.view(torch.int32)
+    for part in range(0, tokens, period):
+        assert torch.equal(got[part : part + period], want[: tokens - part])
+
+
+def test_combines_of_more_rows_than_a_grid_axis_has_threads_for(device):
+    """2^24 workgroups of 256 threads: four tokens each, four choices each of the gradient."""
+    generator = torch.Generator(device=device).manual_seed(7)
+    tokens = (1 << 26) - 1
+    y = torch.randn(1000, 8, device=device, generator=generator).to(torch.bfloat16)
+    slots = torch.randint(-1, 1000, (tokens, 1), dtype=torch.int32, device=device, generator=generator)
+    weights = torch.rand(tokens, 1, device=device, generator=generator)
+    print("combine_weighted", tokens, flush=True)
+    got = ep.combine_weighted(y, slots, weights)
+    for part in range(0, tokens, 1 << 22):
+        at = slice(part, part + (1 << 22))
+        want = torch.where(slots[at] >= 0, y[slots[at, 0].clamp(min=0).long()].float() * weights[at], 0.0)
+        assert torch.equal(got[at], want.to(torch.bfloat16))
+
+    tokens, topk = (1 << 23) + 1, 8
+    rows = tokens * topk
+    y = torch.randn(rows, 8, device=device, generator=generator).to(torch.bfloat16)
+    slots = torch.randperm(rows, device=device, generator=generator).to(torch.int32).reshape(tokens, topk)
+    weights = torch.rand(tokens, topk, device=device, generator=generator)
+    grad = torch.randn(tokens, 8, device=device, generator=generator).to(torch.bfloat16)
+    print("combine_weighted_backward", tokens, flush=True)
+    grad_y, grad_weights = ep.combine_weighted_backward(grad, y, slots, weights)
+    for part in range(0, tokens, 1 << 20):
+        at = slice(part, part + (1 << 20))
+        g = grad[at, None].float()
+        assert torch.equal(grad_y[slots[at].long()], (weights[at, :, None] * g).to(torch.bfloat16))
+        terms = y[slots[at].long()].double() * g
+        assert ((grad_weights[at].double() - terms.sum(2)).abs() <= terms.abs().sum(2) * oracle.FP32 * 8).all()
