@@ -153,6 +153,13 @@ def experts_gated(
     return Fp8Rows(values, scales, payload)
 
 
+def _dense(grad: torch.Tensor) -> torch.Tensor:
+    """A gradient as the kernels take one: contiguous, from a multiple of 16 bytes on (a part of a concatenation's is a
+    contiguous view that starts anywhere)."""
+    grad = grad.contiguous()
+    return grad if grad.data_ptr() % 16 == 0 else grad.clone()
+
+
 class _CombineWeighted(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, token_slots, weights, bias, expert_offsets, expert_counts):
@@ -165,7 +172,7 @@ class _CombineWeighted(torch.autograd.Function):
         y, token_slots, weights, expert_offsets, expert_counts = ctx.saved_tensors
         grad_y = grad_weights = None
         if ctx.needs_input_grad[0] or ctx.needs_input_grad[2]:
-            grad_y, grad_weights = combine_weighted_backward(grad.contiguous(), y, token_slots, weights, expert_offsets, expert_counts)
+            grad_y, grad_weights = combine_weighted_backward(_dense(grad), y, token_slots, weights, expert_offsets, expert_counts)
         return grad_y, None, grad_weights, grad if ctx.needs_input_grad[3] else None, None, None
 
 
@@ -213,7 +220,7 @@ class _DispatchRows(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        return ctx.buffer.combine(grad.contiguous(), ctx.handle).x, None, None
+        return ctx.buffer.combine(_dense(grad), ctx.handle).x, None, None
 
 
 def dispatch_rows(buffer, x: torch.Tensor, handle) -> torch.Tensor:

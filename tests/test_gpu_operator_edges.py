@@ -6,7 +6,7 @@ import torch
 
 import nanoep_amd as ep
 import operator_oracle as oracle
-from test_gpu_operators import KERNELS, close, on
+from test_gpu_operators import KERNELS, close, on, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -125,3 +125,33 @@ def test_combines_of_more_rows_than_a_grid_axis_has_threads_for(device):
         assert torch.equal(grad_y[slots[at].long()], (weights[at, :, None] * g).to(torch.bfloat16))
         terms = y[slots[at].long()].double() * g
         assert ((grad_weights[at].double() - terms.sum(2)).abs() <= terms.abs().sum(2) * oracle.FP32 * 8).all()
+
+
+# ------------------------------------------------------------------ gradients
+
+
+def test_gradients_that_arrive_off_their_alignment(device):
+    """The gradient of a part of a concatenation is a contiguous view that starts anywhere."""
+    tokens, topk, hidden, experts = 33, 2, 256, 4
+    idx = torch.rand(tokens, experts, generator=torch.Generator().manual_seed(3)).topk(topk, dim=1).indices.to(device)
+    x, weights = randn(1, tokens, hidden).to(torch.bfloat16).to(device), torch.rand(tokens, topk, device=device)
+    bias = randn(2, tokens, hidden).to(torch.bfloat16).to(device)
+    few = torch.zeros(3, dtype=torch.bfloat16, device=device)
+    with ep.Buffer(None, ep.EPConfig(experts, topk, hidden, tokens)) as buffer:
+        handle = buffer.dispatch(x, topk_idx=idx, do_expand=True, alignment=8).handle
+        rows = ep.dispatch_rows(buffer, x, handle)
+        grad = randn(4, 3 + tokens * hidden).to(torch.bfloat16).to(device)
+        aligned = grad[3:].clone().view(tokens, hidden)
+
+        leaves = [t.clone().requires_grad_() for t in (rows, weights, bias)]
+        out = ep.combine_weighted(leaves[0], handle.token_slots, leaves[1], bias=leaves[2])
+        torch.cat([few, out.flatten()]).backward(grad)
+        want = ep.combine_weighted_backward(aligned, rows, handle.token_slots, weights)
+        for leaf, gradient in zip(leaves, (*want, aligned)):
+            assert torch.equal(leaf.grad, gradient)
+
+        source = x.clone().requires_grad_()
+        moved = ep.dispatch_rows(buffer, source, handle)
+        grad = randn(5, 3 + moved.numel()).to(torch.bfloat16).to(device)
+        torch.cat([few, moved.flatten()]).backward(grad)
+        assert torch.equal(source.grad, buffer.combine(grad[3:].clone().view(moved.shape), handle).x)
