@@ -8,6 +8,7 @@
 #include <ATen/hip/HIPContext.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 
 #include <initializer_list>
 #include <optional>
@@ -83,7 +84,16 @@ void require_aligned(const torch::Tensor& tensor, const char* what, const char* 
         refuse(what, " ", name, " must start at a multiple of 16 bytes");
 }
 
+// Forward mode goes by the tensors alone: torch.no_grad() leaves it on.
+void require_no_tangent(const char* what, std::initializer_list<const torch::Tensor*> tensors) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        return;
+    for (const torch::Tensor* tensor : tensors)
+        TORCH_CHECK(tensor == nullptr || !tensor->_fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative");
+}
+
 void require_no_gradient(const char* what, std::initializer_list<const torch::Tensor*> tensors) {
+    require_no_tangent(what, tensors);
     if (!at::GradMode::is_enabled())
         return;
     for (const torch::Tensor* tensor : tensors)
@@ -266,6 +276,7 @@ torch::Tensor combine_weighted(const torch::Tensor& y, const torch::Tensor& toke
         require(*bias, device, at::kBFloat16, {a.tokens, a.hidden}, what, "bias");
         require_aligned(*bias, what, "bias");
     }
+    require_no_tangent(what, {&y, &weights, bias.has_value() ? &*bias : nullptr});
     const DeviceGuard guard(device);
     torch::Tensor out = make({a.tokens, a.hidden}, at::kBFloat16, device);
     check(nanoep_combine_weighted(y.data_ptr(), y.size(0), static_cast<const int32_t*>(token_slots.data_ptr()),
@@ -294,6 +305,7 @@ std::tuple<torch::Tensor, torch::Tensor> combine_weighted_backward(const torch::
         require(*expert_counts, device, at::kLong, {experts}, what, "expert_counts");
         require(*expert_offsets, device, at::kLong, {experts + 1}, what, "expert_offsets");
     }
+    require_no_tangent(what, {&grad, &y, &weights});
     const DeviceGuard guard(device);
     torch::Tensor grad_y = make({y.size(0), a.hidden}, at::kBFloat16, device);
     torch::Tensor grad_weights = make({a.tokens, a.topk}, at::kFloat, device);

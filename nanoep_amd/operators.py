@@ -14,7 +14,8 @@ A row in 8 bits is a record: its e4m3 values, then one fp32 scale for every 128 
 The buffer that dispatches records is one whose `hidden` is `fp8_payload_width(hidden)`.
 
 Calls run on the caller's current stream; nothing is copied to the host.  `ValueError` for misuse of arguments, as
-`Buffer` has it.  None of this has a counterpart in the reference, whose experts are the caller's.
+`Buffer` has it; `RuntimeError` where a derivative is asked for that an operator does not have; in forward mode none has one.
+None of this has a counterpart in the reference, whose experts are the caller's.
 """
 
 from __future__ import annotations

@@ -3,6 +3,7 @@ gradients that arrive in unusual tensors, derivatives that do not exist."""
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import nanoep_amd as ep
 import operator_oracle as oracle
@@ -155,3 +156,46 @@ def test_gradients_that_arrive_off_their_alignment(device):
         grad = randn(5, 3 + moved.numel()).to(torch.bfloat16).to(device)
         torch.cat([few, moved.flatten()]).backward(grad)
         assert torch.equal(source.grad, buffer.combine(grad[3:].clone().view(moved.shape), handle).x)
+
+
+# ------------------------------------------------------------------ derivatives that the operators do not have
+
+
+def calls_of_every_operator(device):
+    """Name, call and its floating inputs."""
+    y, slots, weights = torch.zeros(4, 256, dtype=torch.bfloat16, device=device), torch.arange(4, dtype=torch.int32, device=device)[:, None], torch.ones(4, 1, device=device)
+    gamma = torch.ones(256, dtype=torch.bfloat16, device=device)
+    rows, weight = ep.rms_norm_fp8(y, gamma).rows, on(device, ep.quantize_weight(randn(1, 1, 64, 256)))
+    scales = rows.scales.contiguous()
+    return [
+        ("rms_norm_fp8", lambda x, g, r: ep.rms_norm_fp8(x, g, residual=r), (y, gamma, y.clone())),
+        ("experts_linear", lambda s, w: ep.experts_linear(ep.Fp8Rows(rows.values, s), ep.Fp8Weight(weight.values, w)), (scales, weight.scales)),
+        ("experts_gated", lambda s, w: ep.experts_gated(ep.Fp8Rows(rows.values, s), ep.Fp8Weight(weight.values, w)), (scales, weight.scales)),
+        ("combine_weighted", lambda v, w, b: ep.combine_weighted(v, slots, w, bias=b), (y, weights, y.clone())),
+        ("combine_weighted_backward", lambda g, v, w: ep.combine_weighted_backward(g, v, slots, w), (y, y.clone(), weights)),
+    ]
+
+
+def test_forward_mode_derivatives_are_refused(device):
+    """A result without its tangent would pass for one that does not depend on the input."""
+    for name, call, inputs in calls_of_every_operator(device):
+        for which in range(len(inputs)):
+            print("forward mode", name, which, flush=True)
+            with forward_ad.dual_level():
+                dual = forward_ad.make_dual(inputs[which], torch.ones_like(inputs[which]))
+                arguments = [*inputs[:which], dual, *inputs[which + 1 :]]
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*arguments)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*arguments)
+                call(*inputs)
+    # beside an input that reverse mode follows, and through the functions that torch.autograd knows
+    x = torch.zeros(4, 256, dtype=torch.bfloat16, device=device)
+    idx = torch.arange(4, device=device)[:, None]
+    with ep.Buffer(None, ep.EPConfig(4, 1, 256, 4)) as buffer, forward_ad.dual_level():
+        handle = buffer.dispatch(x, topk_idx=idx, do_expand=True).handle
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError):
+            ep.dispatch_rows(buffer, dual, handle)
+        with pytest.raises(RuntimeError):
+            ep.combine_weighted(dual, handle.token_slots, torch.ones(4, 1, device=device, requires_grad=True))
