@@ -305,7 +305,7 @@ std::tuple<torch::Tensor, torch::Tensor> combine_weighted_backward(const torch::
         require(*expert_counts, device, at::kLong, {experts}, what, "expert_counts");
         require(*expert_offsets, device, at::kLong, {experts + 1}, what, "expert_offsets");
     }
-    require_no_tangent(what, {&grad, &y, &weights});
+    require_no_gradient(what, {&grad, &y, &weights});
     const DeviceGuard guard(device);
     torch::Tensor grad_y = make({y.size(0), a.hidden}, at::kBFloat16, device);
     torch::Tensor grad_weights = make({a.tokens, a.topk}, at::kFloat, device);

@@ -208,7 +208,7 @@ def combine_weighted_backward(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """The gradients (grad_y bf16 [rows, hidden], grad_weights float32 [tokens, topk]) of `combine_weighted`:
     grad_y[token_slots[t, k]] = weights[t, k] * grad[t], grad_weights[t, k] = <y[token_slots[t, k]], grad[t]>, zero where masked.
-    No two choices name the same row."""
+    No two choices name the same row.  Without a gradient of its own."""
     return load_extension().combine_weighted_backward(grad, y, token_slots, weights, expert_offsets, expert_counts)
 
 

@@ -199,3 +199,13 @@ def test_forward_mode_derivatives_are_refused(device):
             ep.dispatch_rows(buffer, dual, handle)
         with pytest.raises(RuntimeError):
             ep.combine_weighted(dual, handle.token_slots, torch.ones(4, 1, device=device, requires_grad=True))
+
+
+def test_the_gradients_own_gradient_is_refused(device):
+    name, call, inputs = calls_of_every_operator(device)[-1]
+    for which in range(len(inputs)):
+        arguments = [*inputs[:which], inputs[which].clone().requires_grad_(), *inputs[which + 1 :]]
+        with pytest.raises(RuntimeError, match="has no gradient"):
+            call(*arguments)
+        with torch.no_grad():
+            call(*arguments)
