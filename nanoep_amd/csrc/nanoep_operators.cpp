@@ -267,11 +267,29 @@ WeightedArguments require_weighted(const char* what, const torch::Tensor& y, con
     return {tokens, topk, hidden};
 }
 
+// The experts of a layout, 0 without one.
+int64_t require_layout(const char* what, const Device& device, const std::optional<torch::Tensor>& expert_offsets,
+                       const std::optional<torch::Tensor>& expert_counts) {
+    if (expert_offsets.has_value() != expert_counts.has_value())
+        refuse(what, " takes expert_offsets and expert_counts together");
+    if (!expert_counts.has_value())
+        return 0;
+    const int64_t experts = expert_counts->numel();
+    if (experts <= 0 || experts >= (1 << 30))
+        refuse(what, " expert_counts must name at least one expert");
+    require(*expert_counts, device, at::kLong, {experts}, what, "expert_counts");
+    require(*expert_offsets, device, at::kLong, {experts + 1}, what, "expert_offsets");
+    return experts;
+}
+
+// (the layout is for the gradient; what is wrong with it is said here)
 torch::Tensor combine_weighted(const torch::Tensor& y, const torch::Tensor& token_slots, const torch::Tensor& weights,
-                               const std::optional<torch::Tensor>& bias) {
+                               const std::optional<torch::Tensor>& bias, const std::optional<torch::Tensor>& expert_offsets,
+                               const std::optional<torch::Tensor>& expert_counts) {
     const char* what = "combine_weighted";
     const WeightedArguments a = require_weighted(what, y, token_slots, weights);
     const Device device = y.device();
+    require_layout(what, device, expert_offsets, expert_counts);
     if (bias.has_value()) {
         require(*bias, device, at::kBFloat16, {a.tokens, a.hidden}, what, "bias");
         require_aligned(*bias, what, "bias");
@@ -295,16 +313,7 @@ std::tuple<torch::Tensor, torch::Tensor> combine_weighted_backward(const torch::
     const Device device = y.device();
     require(grad, device, at::kBFloat16, {a.tokens, a.hidden}, what, "grad");
     require_aligned(grad, what, "grad");
-    if (expert_offsets.has_value() != expert_counts.has_value())
-        refuse(what, " takes expert_offsets and expert_counts together");
-    int64_t experts = 0;
-    if (expert_counts.has_value()) {
-        experts = expert_counts->numel();
-        if (experts <= 0 || experts >= (1 << 30))
-            refuse(what, " expert_counts must name at least one expert");
-        require(*expert_counts, device, at::kLong, {experts}, what, "expert_counts");
-        require(*expert_offsets, device, at::kLong, {experts + 1}, what, "expert_offsets");
-    }
+    const int64_t experts = require_layout(what, device, expert_offsets, expert_counts);
     require_no_gradient(what, {&grad, &y, &weights});
     const DeviceGuard guard(device);
     torch::Tensor grad_y = make({y.size(0), a.hidden}, at::kBFloat16, device);
@@ -330,7 +339,7 @@ void bind_operators(py::module_& module) {
     module.def("experts_gated", &experts_gated, py::arg("values"), py::arg("scales"), py::arg("weight"), py::arg("weight_scales"),
                py::arg("expert_offsets"), py::arg("expert_counts"), py::call_guard<py::gil_scoped_release>());
     module.def("combine_weighted", &combine_weighted, py::arg("y"), py::arg("token_slots"), py::arg("weights"), py::arg("bias"),
-               py::call_guard<py::gil_scoped_release>());
+               py::arg("expert_offsets"), py::arg("expert_counts"), py::call_guard<py::gil_scoped_release>());
     module.def("combine_weighted_backward", &combine_weighted_backward, py::arg("grad"), py::arg("y"), py::arg("token_slots"),
                py::arg("weights"), py::arg("expert_offsets"), py::arg("expert_counts"), py::call_guard<py::gil_scoped_release>());
 }

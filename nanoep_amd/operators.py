@@ -165,7 +165,7 @@ class _CombineWeighted(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, token_slots, weights, bias, expert_offsets, expert_counts):
         ctx.save_for_backward(y, token_slots, weights, expert_offsets, expert_counts)
-        return load_extension().combine_weighted(y, token_slots, weights, bias)
+        return load_extension().combine_weighted(y, token_slots, weights, bias, expert_offsets, expert_counts)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -195,7 +195,7 @@ def combine_weighted(
     tracked = y.requires_grad or weights.requires_grad or (bias is not None and bias.requires_grad)
     if tracked and torch.is_grad_enabled():
         return _CombineWeighted.apply(y, token_slots, weights, bias, expert_offsets, expert_counts)
-    return load_extension().combine_weighted(y, token_slots, weights, bias)
+    return load_extension().combine_weighted(y, token_slots, weights, bias, expert_offsets, expert_counts)
 
 
 def combine_weighted_backward(

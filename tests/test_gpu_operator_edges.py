@@ -158,6 +158,18 @@ def test_gradients_that_arrive_off_their_alignment(device):
         assert torch.equal(source.grad, buffer.combine(grad[3:].clone().view(moved.shape), handle).x)
 
 
+def test_layouts_are_checked_ahead_of_the_combine(device):
+    """Not in the backward pass, or never."""
+    y, slots, weights = torch.zeros(4, 256, dtype=torch.bfloat16, device=device), torch.zeros(4, 1, dtype=torch.int32, device=device), torch.ones(4, 1, device=device)
+    offsets, counts = torch.tensor([0, 2, 4], device=device), torch.tensor([2, 2], device=device)
+    ep.combine_weighted(y, slots, weights, expert_offsets=offsets, expert_counts=counts)
+    for layout in ((offsets, None), (None, counts), (offsets, counts[:1]), (offsets[:2], counts), (offsets.int(), counts), (offsets, counts.cpu()),
+                   (offsets[:1], counts[:0])):
+        for needed in (False, True):
+            with pytest.raises(ValueError):
+                ep.combine_weighted(y, slots, weights.clone().requires_grad_(needed), expert_offsets=layout[0], expert_counts=layout[1])
+
+
 # ------------------------------------------------------------------ derivatives that the operators do not have
 
 
