@@ -161,24 +161,30 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
     return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)(p)));
 }
 
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 // Copies 16 (kBytes == 16) or 4 bytes a lane from memory into LDS without registers on the way: lane l's go to
 // `to` + l * kBytes.  `to` and `from` are wave-uniform, `offset` is a lane's own.  Waits are the caller's, by counting.
+// m0 is named as overwritten, so that the compiler takes nothing it has put there to be there still; that it warns of a
+// register of its own on that list is switched off.
 template <int kBytes>
 __device__ __forceinline__ void load_to_lds(const char* from, uint32_t offset, uint32_t to) {
     if constexpr (kBytes == 16)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(from) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(from) : "m0", "memory");
     else
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(from) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(from) : "m0", "memory");
 }
 
 // The same with a whole address of each lane's own.
 template <int kBytes>
 __device__ __forceinline__ void load_to_lds(const char* from, uint32_t to) {
     if constexpr (kBytes == 16)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "m0", "memory");
     else
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "m0", "memory");
 }
+
+#pragma clang diagnostic pop
 
 // What is read in the place of a piece that lies past its row's end.
 __device__ const u32x4 kZeroPiece = {0u, 0u, 0u, 0u};

@@ -1,7 +1,10 @@
 """What of the operators' edges needs no GPU."""
 
+import re
+
 import pytest
 
+from nanoep_amd.build import CSRC
 from test_operators_host import library
 
 
@@ -10,3 +13,14 @@ def test_more_columns_than_the_products_take_are_refused(columns):
     lib, null = library(), None
     assert lib.nanoep_experts_linear(64, 128, 64, 1, 64, 64, null, null, 1, 1, 128, columns, 64, null) == 1
     assert lib.nanoep_experts_gated(64, 128, 64, 1, 64, 64, null, null, 1, 1, 128, columns, 64, 64, 1 << 40, null) == 1
+
+
+def test_statements_that_write_m0_say_so():
+    """An assembly statement whose clobbers leave out a register that it writes is right only while nobody else uses it."""
+    found = 0
+    for source in sorted(CSRC.glob("*")):
+        for statement in re.findall(r"\basm\b[^;]*?;", re.sub(r"//[^\n]*", "", source.read_text()), re.S):
+            if re.search(r"\bm0\s*,", statement.split(":")[0]):
+                found += 1
+                assert '"m0"' in statement.split(":")[-1], f"{source.name}: {statement}"
+    assert found == 4
