@@ -331,7 +331,6 @@ std::tuple<torch::Tensor, torch::Tensor> combine_weighted_backward(const torch::
 }  // namespace
 
 void bind_operators(py::module_& module) {
-    module.def("fp8_record_bytes", &nanoep_fp8_record_bytes, py::arg("columns"));
     module.def("rms_norm_fp8", &rms_norm_fp8, py::arg("x"), py::arg("gamma"), py::arg("residual"), py::arg("eps"), py::arg("normalized"),
                py::call_guard<py::gil_scoped_release>());
     module.def("experts_linear", &experts_linear, py::arg("values"), py::arg("scales"), py::arg("weight"), py::arg("weight_scales"),

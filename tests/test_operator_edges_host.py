@@ -1,9 +1,11 @@
 """What of the operators' edges needs no GPU."""
 
+import inspect
 import re
 
 import pytest
 
+from nanoep_amd import operators
 from nanoep_amd.build import CSRC
 from test_operators_host import library
 
@@ -24,3 +26,9 @@ def test_statements_that_write_m0_say_so():
                 found += 1
                 assert '"m0"' in statement.split(":")[-1], f"{source.name}: {statement}"
     assert found == 4
+
+
+def test_every_function_that_the_operators_bind_is_called():
+    bound = set(re.findall(r'module\.def\("(\w+)"', (CSRC / "nanoep_operators.cpp").read_text()))
+    called = set(re.findall(r"load_extension\(\)\.(\w+)\(", inspect.getsource(operators)))
+    assert bound == called
