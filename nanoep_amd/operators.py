@@ -79,6 +79,8 @@ class Fp8Rows:
         width = fp8_payload_width(hidden)
         if payload.dtype != torch.bfloat16 or payload.dim() != 2 or payload.shape[1] != width or not payload.is_contiguous():
             raise ValueError(f"payload must be contiguous bfloat16 [rows, {width}]")
+        if payload.storage_offset() % 2:
+            raise ValueError("payload must start at a whole fp32 of its storage, as its scales do")
         first = hidden // 4
         scales = payload.view(torch.float32)[:, first : first + -(-hidden // SCALE_BLOCK)]
         return cls(payload.view(torch.float8_e4m3fn)[:, :hidden], scales, payload)

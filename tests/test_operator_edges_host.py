@@ -4,7 +4,9 @@ import inspect
 import re
 
 import pytest
+import torch
 
+import nanoep_amd as ep
 from nanoep_amd import operators
 from nanoep_amd.build import CSRC
 from test_operators_host import library
@@ -32,3 +34,11 @@ def test_every_function_that_the_operators_bind_is_called():
     bound = set(re.findall(r'module\.def\("(\w+)"', (CSRC / "nanoep_operators.cpp").read_text()))
     called = set(re.findall(r"load_extension\(\)\.(\w+)\(", inspect.getsource(operators)))
     assert bound == called
+
+
+def test_records_that_start_between_two_scales_are_refused():
+    width = ep.fp8_payload_width(256)
+    storage = torch.zeros(3 * width + 2, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        ep.Fp8Rows.of_payload(storage[1 : 1 + 3 * width].view(3, width), 256)
+    assert ep.Fp8Rows.of_payload(storage[2:].view(3, width), 256).scales.shape == (3, 2)
