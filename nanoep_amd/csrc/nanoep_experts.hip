@@ -467,7 +467,9 @@ __device__ __forceinline__ int list_tiles(const Product& p, int column_tiles, ui
         at += w < wave ? wave_sums[w] : 0;
         total += wave_sums[w];
     }
-    total = __builtin_amdgcn_readfirstlane(total);
+    // no more than segments behind one another can have: a layout whose segments lie over one another ends as soon
+    const int most = static_cast<int>(p.rows / kRows) + static_cast<int>(p.experts < p.rows ? p.experts : p.rows);
+    total = __builtin_amdgcn_readfirstlane(total < 0 || total > most ? most : total);
     for (int e = from; e < from + each && e < segments; ++e) {
         const Segment segment = segment_of(p, e);
         before[e] = at;
@@ -495,7 +497,7 @@ __device__ __forceinline__ int list_tiles(const Product& p, int column_tiles, ui
         const Segment segment = segment_of(p, low);
         const int skipped = (row_tile - before[low]) * kRows;
         const int live = static_cast<int>(segment.live) - skipped;
-        // (a layout whose segments lie over one another may number more tiles than fit an int: one row then, of some expert's)
+        // (segments that lie over one another may have more tiles than fit an int: one row then, of some expert's)
         items[i] = skipped < 0 || live <= 0 ? Item{0, 0, 1, 0}
                                             : Item{low, static_cast<int>(segment.begin) + skipped, live > kRows ? kRows : live, static_cast<int>(in_group / group_rows)};
     }

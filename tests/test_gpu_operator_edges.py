@@ -81,6 +81,24 @@ def test_products_of_more_row_tiles_than_a_grid_axis_has_threads_for(device, tun
         assert torch.equal(got[part : min(part + period, rows - 5)], want[: rows - 5 - part])
 
 
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_products_of_segments_that_lie_over_one_another(device, tuning, kernel):
+    """Every other segment is all rows, which have tiles for two of them; the experts' weights are the same."""
+    tuning("EXPERTS_TILE", kernel)
+    experts, rows = 2000, 1000
+    values, scales = oracle.quantize_rows(randn(3, rows, 128))
+    weight = ep.quantize_weight(randn(4, 1, 64, 128))
+    weight = ep.Fp8Weight(weight.values.expand(experts, -1, -1).contiguous(), weight.scales.expand(experts, -1, -1).contiguous())
+    offsets = torch.tensor([0, rows] * (experts // 2) + [rows], device=device)
+    counts = torch.full((experts,), rows, device=device)
+    z, slack = oracle.experts(values, scales, weight.values[:1], weight.scales[:1], None, None)
+    rows_on, weight = ep.Fp8Rows(values.to(device), scales.to(device)), on(device, weight)
+    print("segments over one another", kernel, flush=True)
+    close(ep.experts_linear(rows_on, weight, offsets, counts), z, slack)
+    got = ep.experts_gated(rows_on, weight, offsets, counts)
+    oracle.check_eight_bits(got.values.cpu(), got.scales.cpu(), *oracle.gated(z, slack))
+
+
 # ------------------------------------------------------------------ norm and combine
 
 
