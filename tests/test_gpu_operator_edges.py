@@ -7,7 +7,7 @@ from torch.autograd import forward_ad
 
 import nanoep_amd as ep
 import operator_oracle as oracle
-from test_gpu_operators import KERNELS, close, on, randn
+from test_gpu_operators import KERNELS, NAN_BYTE, close, make_product, on, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -99,6 +99,119 @@ def test_products_of_segments_that_lie_over_one_another(device, tuning, kernel):
     oracle.check_eight_bits(got.values.cpu(), got.scales.cpu(), *oracle.gated(z, slack))
 
 
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_gated_products_follow_strides_of_their_own(device, tuning, kernel):
+    tuning("EXPERTS_TILE", kernel)
+    values, scales, weight, offsets, counts = make_product("uneven", 272, 160, 9)
+    rows = values.shape[0]
+    wide = torch.full((rows, 272 + 48), NAN_BYTE, dtype=torch.uint8, device=device)
+    wide[:, 16:288] = values.view(torch.uint8).to(device)
+    wide_scales = torch.full((rows, 7), float("nan"), device=device)
+    wide_scales[:, 2:5] = scales.to(device)
+    print("gated strides", kernel, flush=True)
+    got = ep.experts_gated(ep.Fp8Rows(wide[:, 16:288].view(torch.float8_e4m3fn), wide_scales[:, 2:5]), on(device, weight), offsets.to(device),
+                           counts.to(device))
+    z = oracle.experts(values, scales, weight.values, weight.scales, offsets, counts)
+    oracle.check_eight_bits(got.values.cpu(), got.scales.cpu(), *oracle.gated(*z))
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_gated_products_stay_within_the_rows_whatever_the_layout_says(device, tuning, kernel):
+    tuning("EXPERTS_TILE", kernel)
+    values, scales = oracle.quantize_rows(randn(3, 64, 128))
+    weight = ep.quantize_weight(randn(4, 3, 64, 128))
+    # an expert's count reaches past its segment, the last segment past the rows
+    offsets, counts = torch.tensor([0, 20, 40, 90], device=device), torch.tensor([25, 20, 1 << 40], device=device)
+    z = oracle.experts(values, scales, weight.values, weight.scales, torch.tensor([0, 20, 40]), torch.tensor([20, 20, 24]))
+    print("gated layout", kernel, flush=True)
+    got = ep.experts_gated(ep.Fp8Rows(values.to(device), scales.to(device)), on(device, weight), offsets, counts)
+    oracle.check_eight_bits(got.values.cpu(), got.scales.cpu(), *oracle.gated(*z))
+
+
+def test_gated_products_of_rows_beyond_32_bit_offsets(device):
+    rows, inner, columns = 600_000, 4096, 64
+    values = torch.randint(0, 0x70, (rows, inner), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+    scales = torch.rand(rows, inner // 128, device=device) * 1e-3
+    weight = ep.quantize_weight(randn(6, 2, columns, inner))
+    layout = torch.tensor([0, rows - 100, rows], device=device), torch.tensor([rows - 100, 100], device=device)
+    got = ep.experts_gated(ep.Fp8Rows(values, scales), on(device, weight), *layout)
+    for e, part in ((0, slice(0, 40)), (0, slice(rows - 140, rows - 100)), (1, slice(rows - 100, rows))):
+        z = oracle.experts(values[part].cpu(), scales[part].cpu(), weight.values[e : e + 1], weight.scales[e : e + 1], None, None)
+        oracle.check_eight_bits(got.values[part].cpu(), got.scales[part].cpu(), *oracle.gated(*z))
+
+
+def test_gated_products_of_more_tiles_than_a_workgroup_lists(device, tuning):
+    """66000 tiles of 256 rows; whole numbers, whose sums are exact."""
+    tuning("EXPERTS_TILE", 256)
+    rows, inner, columns = 66_000 * 256 + 17, 16, 32
+    whole = torch.randint(-4, 5, (rows, inner), dtype=torch.int8, device=device)
+    scales = 2.0 ** torch.randint(-3, 4, (rows, 1), device=device)
+    weight = torch.randint(-4, 5, (1, columns, inner), generator=torch.Generator().manual_seed(6)).float()
+    weight_on = ep.Fp8Weight(weight.to(torch.float8_e4m3fn).to(device), torch.ones(1, 1, 1, device=device))
+    print("gated tiles", rows, flush=True)
+    got = ep.experts_gated(ep.Fp8Rows(whole.to(torch.float8_e4m3fn), scales), weight_on)
+    for part in range(0, rows, 1 << 20):
+        at = slice(part, part + (1 << 20))
+        z = ((whole[at].float() @ weight[0].T.to(device)) * scales[at]).double()
+        oracle.check_eight_bits(got.values[at], got.scales[at], *oracle.gated(z, torch.zeros_like(z)))
+
+
+def test_products_with_an_experts_weight_beyond_32_bit_offsets(device):
+    inner, columns, rows = 4112, (1 << 20) + 256, 3
+    assert inner * columns > 1 << 32
+    values, scales = oracle.quantize_rows(randn(1, rows, inner))
+    weight = torch.randint(0, 0x70, (1, columns, inner), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+    weight_scales = torch.rand(1, oracle.groups(columns), oracle.groups(inner), device=device) * 1e-3
+    rows_on, weight_on = ep.Fp8Rows(values.to(device), scales.to(device)), ep.Fp8Weight(weight, weight_scales)
+    print("weight beyond 32 bits", flush=True)
+    linear, gated = ep.experts_linear(rows_on, weight_on), ep.experts_gated(rows_on, weight_on)
+
+    def z_of(part):
+        blocks = slice(part.start // 128, part.stop // 128)
+        return oracle.experts(values, scales, weight[:, part].cpu(), weight_scales[:, blocks].cpu(), None, None)
+
+    half = columns // 2
+    for begin in (0, half - 128 * 5, half - 128):
+        part, above = slice(begin, begin + 128), slice(half + begin, half + begin + 128)
+        (gate, gate_slack), (up, up_slack) = z_of(part), z_of(above)
+        close(linear[:, part], gate, gate_slack)
+        close(linear[:, above], up, up_slack)
+        act = oracle.gated(torch.cat([gate, up], 1), torch.cat([gate_slack, up_slack], 1))
+        oracle.check_eight_bits(gated.values[:, part].cpu(), gated.scales[:, begin // 128 : begin // 128 + 1].cpu(), *act)
+
+
+def test_products_of_more_experts_than_a_tile_list_takes(device):
+    experts, inner, columns = (1 << 14) + 3, 32, 64
+    counts = torch.randint(0, 3, (experts,), generator=torch.Generator().manual_seed(2))
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), ((counts + 3) // 4 * 4).cumsum(0)])
+    rows = int(offsets[-1]) + 2
+    values, scales = oracle.quantize_rows(randn(3, rows, inner))
+    weight = randn(4, experts, columns, inner).clamp(-4, 4).mul(100).to(torch.float8_e4m3fn)
+    weight_scales = torch.rand(experts, 1, 1) * 1e-2
+    z = oracle.experts(values, scales, weight, weight_scales, offsets, counts)
+    rows_on, weight_on = ep.Fp8Rows(values.to(device), scales.to(device)), on(device, ep.Fp8Weight(weight, weight_scales))
+    print("experts", experts, flush=True)
+    close(ep.experts_linear(rows_on, weight_on, offsets.to(device), counts.to(device)), *z)
+    got = ep.experts_gated(rows_on, weight_on, offsets.to(device), counts.to(device))
+    oracle.check_eight_bits(got.values.cpu(), got.scales.cpu(), *oracle.gated(*z))
+
+
+@pytest.mark.parametrize("value_stride,scale_stride", [((1 << 24) + 16, 3), (272, (1 << 22) + 1)])
+def test_products_of_rows_far_apart(device, value_stride, scale_stride):
+    rows, inner, columns = 70, 272, 96
+    values, scales = oracle.quantize_rows(randn(5, rows, inner))
+    weight = ep.quantize_weight(randn(6, 1, columns, inner))
+    far = torch.full((rows * value_stride,), NAN_BYTE, dtype=torch.uint8, device=device).view(rows, value_stride)[:, :inner].view(torch.float8_e4m3fn)
+    far.view(torch.uint8).copy_(values.view(torch.uint8))
+    far_scales = torch.full((rows * scale_stride,), float("nan"), device=device).view(rows, scale_stride)[:, :3]
+    far_scales.copy_(scales)
+    z = oracle.experts(values, scales, weight.values, weight.scales, None, None)
+    print("rows apart", value_stride, scale_stride, flush=True)
+    close(ep.experts_linear(ep.Fp8Rows(far, far_scales), on(device, weight)), *z)
+    got = ep.experts_gated(ep.Fp8Rows(far, far_scales), on(device, weight))
+    oracle.check_eight_bits(got.values.cpu(), got.scales.cpu(), *oracle.gated(*z))
+
+
 # ------------------------------------------------------------------ norm and combine
 
 
@@ -174,6 +287,28 @@ def test_gradients_that_arrive_off_their_alignment(device):
         grad = randn(5, 3 + moved.numel()).to(torch.bfloat16).to(device)
         torch.cat([few, moved.flatten()]).backward(grad)
         assert torch.equal(source.grad, buffer.combine(grad[3:].clone().view(moved.shape), handle).x)
+
+
+def test_many_rows_of_no_expert_are_cleared_ahead_of_the_gradient(device):
+    """More than 32 MiB of them have a launch of their own."""
+    tokens, topk, hidden, experts = 50, 4, 2816, 128
+    idx = torch.rand(tokens, experts, generator=torch.Generator().manual_seed(1)).topk(topk, dim=1).indices
+    idx[idx % 7 == 0] = -1
+    with ep.Buffer(None, ep.EPConfig(experts, topk, 256, tokens)) as buffer:
+        handle = buffer.dispatch(torch.zeros(tokens, 256, dtype=torch.bfloat16, device=device), topk_idx=idx.to(device), do_expand=True,
+                                 alignment=128).handle
+    rows = handle.layout.expanded_capacity + 3
+    assert (rows - tokens * topk) * hidden * 2 > 32 << 20
+    y, grad = randn(2, rows, hidden).to(torch.bfloat16), randn(3, tokens, hidden).to(torch.bfloat16)
+    weights = torch.rand(tokens, topk)
+    want_y, want_weights, slack = oracle.combine_backward(grad, y, handle.token_slots.cpu(), weights)
+    inputs = grad.to(device), y.to(device), handle.token_slots, weights.to(device)
+    torch.full((rows, hidden), float("nan"), dtype=torch.bfloat16, device=device)  # what a new tensor's memory may hold
+    got = ep.combine_weighted_backward(*inputs, handle.layout.expert_offsets, handle.layout.expert_counts)
+    close(got[0], want_y, want_y.abs() * oracle.FP32)
+    assert ((got[1].cpu().double() - want_weights).abs() <= slack).all()
+    again = ep.combine_weighted_backward(*inputs)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
 
 
 def test_layouts_are_checked_ahead_of_the_combine(device):
