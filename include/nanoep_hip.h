@@ -341,8 +341,9 @@ int nanoep_experts_gated(const void* values, int64_t value_stride, const float* 
  * (+ f32(bias[t])) ), for the slot table of an expanded handle; a slot outside [0, y_rows) counts as masked, and its weight is not
  * looked at.  y: bf16 [y_rows, hidden], weights: fp32 [T, K], bias: bf16 [T, hidden] or NULL; hidden % 8 == 0, K <= 32.
  * The gradient: grad_y[slot[t][k]] = weights[t][k] * grad[t], grad_weights[t][k] = <y[slot[t][k]], grad[t]>, 0 where masked; no two
- * choices may name one row.  Rows that no choice names get zero: with expert_offsets (int64 [L + 1]) and expert_counts (int64
- * [L]) only the rows that are no expert's are cleared, without (both NULL) all of them are, ahead of the gradient.
+ * choices may name one row.  Rows that no choice names get zero: all rows are cleared ahead of the gradient.  With expert_offsets
+ * (int64 [L + 1]) and expert_counts (int64 [L]; both NULL: as above) only the rows that are no expert's are cleared, and every
+ * expert's row has to be named by a choice.
  */
 int nanoep_combine_weighted(const void* y, int64_t y_rows, const int32_t* token_slots, const float* weights, const void* bias,
                             int64_t num_tokens, int hidden, int num_topk, void* out, void* stream);

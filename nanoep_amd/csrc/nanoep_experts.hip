@@ -522,10 +522,11 @@ __device__ __forceinline__ int list_tiles(const Product& p, int column_tiles, ui
 // A lane's four columns of a tile are 8 bytes of bf16: neighbouring column tiles swap halves first, so that half as many
 // stores write twice as much each (60 experts, 1424 -> 2816: 140 us against 149).
 //
-// Measured (32 experts, 29500 rows): 2048 -> 7168 828 to 852 us, 1.03 PFLOP/s; gated 7168 -> 2 x 2048 1650 to 1690 us, 1.04 PFLOP/s:
-// 81 % of what a large library product reaches in bf16.  64 experts of 28 rows, gated, 4096 -> 2 x 2048, 64-row tiles: 202 us, 5.4
-// TB/s.  The loads of a 256-row tile's block alone take 1.36 us of its 3.0: 64 KB that L2 hands out in 64-byte requests; with one
-// block's time ahead for the weights they took 1.76 us.
+// Measured (32 experts, 29500 rows): 2048 -> 7168 812 to 836 us, 1.04 PFLOP/s; gated 7168 -> 2 x 2048 1650 to 1710 us, 1.04 PFLOP/s:
+// 81 % of what a large library product reaches in bf16, matrix instructions busy for 49 and 48 % of the clocks at 2.35 GHz.
+// 64 experts of 28 rows, gated, 4096 -> 2 x 2048, 64-row tiles: 200 us, 5.4 TB/s.  The loads of a block of a 256-row tile
+// alone take 1.36 us (64 KB that L2 hands out in 64-byte requests), the whole block 3.5; with one block's time ahead for the
+// weights the loads alone took 1.76 us.  The 256-row tile spills 19 registers, outside its loop over the blocks.
 template <int kRowTiles, int kColTiles, int kRowWaves, int kColWaves, bool kGated>
 __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
     experts_tile_kernel(const Product p, char* __restrict__ out, int64_t out_stride, int column_tiles, XcdMap xcds) {

@@ -13,7 +13,7 @@ constexpr int kMostNormVectors = 8;  // 16-byte vectors of a row that a lane hol
 // between its sum of squares and its output (kVectors 16-byte vectors a lane, 8 columns each), so that every
 // input byte is read once, all of them ahead of anything else; s and n are fp32 throughout, and each output is rounded
 // from them once.  16 neighbouring lanes hold the 128 columns of a scale.  HBM-bound: 4096 x 7168 with both bf16 outputs
-// (265 MB) 40 to 42 us, 6.3 TB/s, 44.7 a call among others; one token 2.6.  Side by side, back to back: 48.3 us (with plain stores and
+// (265 MB) 40 to 42 us, 6.5 TB/s, 45.1 a call among others; one token 2.7.  Side by side, back to back: 48.3 us (with plain stores and
 // gamma read behind the sum 54.0), 8192 x 2048 24.7; nontemporal loads of the inputs take 44.9 and 27.2 there, but would pass
 // over inputs that the last kernel left in the caches.
 template <int kVectors>

@@ -100,7 +100,7 @@ __device__ __forceinline__ void clear_gap(const int64_t* expert_offsets, const i
 // sum in its lanes, which are added in a fixed order at the end.  A token's choices are neighbours, so that its
 // gradient row comes from the caches for all but one of them.  Workgroups ahead of theirs clear the rows of no expert.
 // No atomics: the order of every sum is fixed.  HBM-bound: 4096 tokens of 7168, eight choices (1.14 GB with 16200 padding rows)
-// 173 to 185 us and 20 for the padding, 5.8 TB/s; 1537 of 2816, six choices (115 MB) 21 to 23 us, 5.2 TB/s.
+// 169 to 171 us and 22 for the padding, 5.9 TB/s; 1537 of 2816, six choices (115 MB) 20 to 23 us, 5.2 TB/s.
 __global__ void __launch_bounds__(kBlockThreads) combine_weighted_backward_kernel(const u32x4* __restrict__ grad,  // [T][vectors]
                                                                                   const u32x4* __restrict__ y,     // [C][vectors]
                                                                                   const int32_t* __restrict__ token_slots,

@@ -192,8 +192,9 @@ def combine_weighted(
     rounded once.  `token_slots` is an expanded handle's int32 [tokens, topk]; a choice outside y's rows counts as
     masked, and neither its weight nor any row is looked at for it.
 
-    It has a gradient in y, weights and bias.  The rows of y that no choice names have the gradient zero: with the layout's
-    `expert_offsets` and `expert_counts` only those are cleared, without them all rows are first."""
+    It has a gradient in y, weights and bias.  The rows of y that no choice names have the gradient zero: all rows are cleared
+    first.  With the layout's `expert_offsets` and `expert_counts` only the rows of no expert are: give the two with their
+    handle's own `token_slots`, in which a choice names every expert's row, and not with a table that leaves some out."""
     tracked = y.requires_grad or weights.requires_grad or (bias is not None and bias.requires_grad)
     if tracked and torch.is_grad_enabled():
         return _CombineWeighted.apply(y, token_slots, weights, bias, expert_offsets, expert_counts)
