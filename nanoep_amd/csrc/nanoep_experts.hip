@@ -618,10 +618,13 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                 for (int i = 0; i < Shape::kWeightLoads; ++i)
                     load_to_lds<16>(weight + at, weight_offset[i] + piece * 16, to + i * kStep);
             } else {
+                // (whole addresses, made from the offsets here: kept over the loops they would cost the registers of twice as many)
 #pragma unroll
-                for (int i = 0; i < Shape::kWeightLoads; ++i)
-                    load_to_lds<16>(at + piece * 16 < p.inner ? weight + at + static_cast<uint32_t>(afresh(static_cast<int>(weight_offset[i]))) + piece * 16 : reinterpret_cast<const char*>(&kZeroPiece),
-                                to + i * kStep);
+                for (int i = 0; i < Shape::kWeightLoads; ++i) {
+                    const uint32_t offset = static_cast<uint32_t>(afresh(static_cast<int>(weight_offset[i])));
+                    load_to_lds<16>(at + piece * 16 < p.inner ? weight + at + offset + piece * 16 : reinterpret_cast<const char*>(&kZeroPiece),
+                                    to + i * kStep);
+                }
             }
             weight_slot = after(weight_slot);
             if (++weight_block == p.blocks)
@@ -665,9 +668,11 @@ __global__ void __launch_bounds__(kRowWaves * kColWaves * kWave, 2)
                     load_to_lds<16>(values + at, row_offset[i] + piece * 16, to + i * kStep);
             } else {
 #pragma unroll
-                for (int i = 0; i < Shape::kRowLoads; ++i)
-                    load_to_lds<16>(at + piece * 16 < p.inner ? values + at + static_cast<uint32_t>(afresh(static_cast<int>(row_offset[i]))) + piece * 16 : reinterpret_cast<const char*>(&kZeroPiece),
-                                to + i * kStep);
+                for (int i = 0; i < Shape::kRowLoads; ++i) {
+                    const uint32_t offset = static_cast<uint32_t>(afresh(static_cast<int>(row_offset[i])));
+                    load_to_lds<16>(at + piece * 16 < p.inner ? values + at + offset + piece * 16 : reinterpret_cast<const char*>(&kZeroPiece),
+                                    to + i * kStep);
+                }
             }
             // (where there are more wavefronts than 64 rows, some bring in the same scales)
             load_to_lds<4>(scales + static_cast<int64_t>(row_block) * 4, scale_offset, scales_at + row_slot * Shape::kRows * 4);
@@ -1134,8 +1139,9 @@ int nanoep_experts_gated(const void* values, int64_t value_stride, const float* 
     const int launched = launch_streams<true>(p, workspace, columns / 2, on);
     if (launched != NANOEP_OK)
         return launched;
-    quantize_rows_kernel<<<grid_of((rows + kWavesPerBlock - 1) / kWavesPerBlock), kBlockThreads, 0, on>>>(static_cast<const float*>(workspace), static_cast<char*>(records), rows,
-                                                           record_bytes_of(columns / 2), columns / 2, static_cast<int>(scale_groups(columns / 2)));
+    quantize_rows_kernel<<<grid_of((rows + kWavesPerBlock - 1) / kWavesPerBlock), kBlockThreads, 0, on>>>(
+        static_cast<const float*>(workspace), static_cast<char*>(records), rows, record_bytes_of(columns / 2), columns / 2,
+        static_cast<int>(scale_groups(columns / 2)));
     NANOEP_HIP_TRY(hipGetLastError());
     return NANOEP_OK;
 }
