@@ -351,6 +351,70 @@ int nanoep_combine_weighted_backward(const void* grad, const void* y, int64_t y_
                                      const int64_t* expert_offsets, const int64_t* expert_counts, int64_t num_local_experts,
                                      int64_t num_tokens, int hidden, int num_topk, void* grad_y, float* grad_weights, void* stream);
 
+/*
+ * The entry of an expert layer as it is trained and served: norms with gradients, the router's choice, the loss that balances the
+ * experts.  No counterpart in the reference.  Types of rows, parameters and logits:
+ */
+#define NANOEP_BF16 0
+#define NANOEP_FP32 1
+
+/*
+ * Layer norm, or with mean NULL the root-mean-square norm (beta NULL then): s = x + residual, rounded to the rows' type and written
+ * to total (residual NULL: s = x, total NULL); m = sum(s) / hidden (root mean square: 0), r = 1 / sqrt(sum((s - m)^2) / hidden + eps);
+ * normalized = (s - m) * r * gamma + beta (NULL: none), in fp32, rounded once; m and r go to mean and rstd (fp32 [T]).
+ * x, residual, total, normalized: [T, hidden] of rows_type; gamma, beta: [hidden] of parameters_type: the rows' own, or fp32;
+ * hidden % 8 == 0, hidden <= 16384; all but mean and rstd 16-byte aligned.  Outputs overlap no input.
+ * The gradient, for grad of normalized and grad_residual of total itself (NULL: none): grad_x (that of x and of residual; NULL: not
+ * wanted), grad_gamma and, with mean, grad_beta (in parameters_type; both NULL: not wanted).  total: the rows that were normed.  Needs
+ * nanoep_layer_norm_backward_workspace_bytes of 16-byte aligned device scratch if grad_gamma is wanted; the sums over the rows are in
+ * a fixed order.  With no rows their arrays may be NULL, and the parameters' gradients are zero.
+ */
+int nanoep_layer_norm(const void* x, const void* residual, const void* gamma, const void* beta, int64_t num_tokens, int hidden, float eps,
+                      int rows_type, int parameters_type, void* total, void* normalized, float* mean, float* rstd, void* stream);
+size_t nanoep_layer_norm_backward_workspace_bytes(int64_t num_tokens, int hidden, int rows_type);
+int nanoep_layer_norm_backward(const void* grad, const void* total, const void* gamma, const float* mean, const float* rstd,
+                               const void* grad_residual, int64_t num_tokens, int hidden, int rows_type, int parameters_type, void* grad_x,
+                               void* grad_gamma, void* grad_beta, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Scores of a token's logits l over the experts: softmax, or 1 / (1 + e^-l) each. */
+#define NANOEP_SOFTMAX 0
+#define NANOEP_SIGMOID 1
+
+/*
+ * The router's choice.  ids (int64 [T, K]): the K experts of the largest value, in descending order, the lowest index first among
+ * equals; -1 where no expert is left, and for tokens whose mask (one byte a token; NULL: none) is 0.  An expert's value is its logit;
+ * with bias (fp32 [E]) or several groups it is its score (plus bias), in 64 bits.  Experts at -infinity cannot be chosen; NaN is
+ * above everything.  groups > topk_groups: only experts of the topk_groups best groups are chosen from, groups being equal parts of
+ * neighbouring experts, each as good as the sum of its two largest values.
+ * weights (fp32 [T, K]): scale * the chosen experts' scores, without the bias, with normalize over their sum; 0 where ids is -1.
+ * logits: [T, E] of logits_type, tokens logits_stride elements apart (at least E); E <= 4096, K <= min(E, 32), groups <= 64.
+ * The gradient of the weights: grad (fp32 [T, K]) to grad_logits ([T, E], contiguous, of logits_type); ids outside [0, E) are masked
+ * choices, an id that a token has twice counts twice.
+ */
+int nanoep_route_topk(const void* logits, int64_t logits_stride, int logits_type, const float* bias, const uint8_t* mask, int64_t num_tokens,
+                      int num_experts, int num_topk, int groups, int topk_groups, int scoring, int normalize, float scale, int64_t* ids,
+                      float* weights, void* stream);
+int nanoep_route_topk_backward(const float* grad, const void* logits, int64_t logits_stride, int logits_type, const int64_t* ids,
+                               int64_t num_tokens, int num_experts, int num_topk, int scoring, int normalize, float scale, void* grad_logits,
+                               void* stream);
+
+/*
+ * The balance loss of each of S sequences of tokens (sequence_offsets int64 [S + 1], from 0 on; NULL: all tokens are one):
+ *   loss[s] = E * sum over e of counts[s][e] / C * mean of share[t][e] over the tokens of s with a choice
+ * counts (int64 [S, E]): the choices of e in s, C their sum; share: softmax of the token's logits, or sigmoids over their sum; tokens
+ * (int64 [S]): the tokens with a choice.  A token without one, all of its ids outside [0, E), is not looked at; a sequence without
+ * one has loss 0.  Needs nanoep_balance_loss_workspace_bytes of 16-byte aligned device scratch (may be 0).
+ * The gradient in the logits, for grad (fp32 [S]) and the counts and tokens that the loss left (counts have none): [T, E],
+ * contiguous, zero for tokens without a choice and those of no sequence.
+ */
+size_t nanoep_balance_loss_workspace_bytes(int64_t num_tokens, int num_experts, int64_t sequences);
+int nanoep_balance_loss(const void* logits, int64_t logits_stride, int logits_type, const int64_t* ids, const int64_t* sequence_offsets,
+                        int64_t num_tokens, int num_experts, int num_topk, int64_t sequences, int scoring, float* loss, int64_t* counts,
+                        int64_t* tokens, void* workspace, size_t workspace_bytes, void* stream);
+int nanoep_balance_loss_backward(const float* grad, const void* logits, int64_t logits_stride, int logits_type, const int64_t* ids,
+                                 const int64_t* counts, const int64_t* tokens, const int64_t* sequence_offsets, int64_t num_tokens,
+                                 int num_experts, int num_topk, int64_t sequences, int scoring, void* grad_logits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -27,9 +27,9 @@ EXTENSION_LIBRARY = PACKAGE / f"{EXTENSION_NAME}.so"
 
 KERNEL_SOURCES = [
     "nanoep_layout.hip", "nanoep_dispatch.hip", "nanoep_combine.hip", "nanoep_abi.hip", "nanoep_norm.hip", "nanoep_experts.hip",
-    "nanoep_weighted.hip",
+    "nanoep_weighted.hip", "nanoep_layer_norm.hip", "nanoep_router.hip",
 ]
-EXTENSION_SOURCES = ["nanoep_torch.cpp", "nanoep_operators.cpp"]
+EXTENSION_SOURCES = ["nanoep_torch.cpp", "nanoep_operators.cpp", "nanoep_entry.cpp"]
 
 OFFLOAD_ARCH = "gfx950"
 # Packed fp32 instructions are disabled for every HIP translation unit of this project.

@@ -4,46 +4,17 @@
 
 #include "nanoep_operators_host.h"
 
-#include <ATen/hip/EmptyTensor.h>
-#include <ATen/hip/HIPContext.h>
-#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <c10/core/AutogradState.h>
-
-#include <initializer_list>
-#include <optional>
-#include <sstream>
 #include <tuple>
 
 #include "nanoep_hip.h"
 
 namespace nanoep {
+
+using namespace host;
+
 namespace {
 
-using Device = c10::Device;
-using DeviceGuard = c10::hip::HIPGuardMasqueradingAsCUDA;
-
 constexpr int64_t kScaleBlock = 128;
-
-template <class... Parts>
-[[noreturn]] void refuse(const Parts&... parts) {
-    std::ostringstream text;
-    (text << ... << parts);
-    throw py::value_error(text.str());
-}
-
-void check(int status, const char* what) {
-    TORCH_CHECK(status == NANOEP_OK, "nanoep ", what, " failed: ", nanoep_status_string(status), " ", nanoep_last_hip_error());
-}
-
-void* current_stream(const Device& device) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device.index()).stream(); }
-
-torch::Tensor make(at::IntArrayRef sizes, at::ScalarType dtype, const Device& device) {
-    const auto& context = at::globalContext();
-    if (C10_UNLIKELY(context.deterministicAlgorithms() && context.deterministicFillUninitializedMemory()))
-        return torch::empty(sizes, torch::TensorOptions().dtype(dtype).device(device));
-    return torch::Tensor(at::detail::empty_cuda(sizes, dtype, device, std::nullopt));
-}
 
 // Rows of another type within a tensor of records, made without the dispatcher; a view for autograd's version counter.
 torch::Tensor rows_within(const torch::Tensor& base, at::ScalarType dtype, int64_t offset, int64_t rows, int64_t columns, int64_t row_stride) {
@@ -56,51 +27,6 @@ torch::Tensor rows_within(const torch::Tensor& base, at::ScalarType dtype, int64
         impl->set_version_counter(base.unsafeGetTensorImpl()->version_counter());
     return part;
 }
-
-void require_gpu(const torch::Tensor& tensor, const char* what, const char* name) {
-    if (!tensor.is_cuda())
-        refuse(what, " ", name, " must be a CUDA tensor");
-}
-
-void require(const torch::Tensor& tensor, const Device& device, at::ScalarType dtype, std::initializer_list<int64_t> sizes, const char* what,
-             const char* name) {
-    bool fits = tensor.device() == device && tensor.scalar_type() == dtype && tensor.dim() == static_cast<int64_t>(sizes.size()) &&
-                tensor.is_contiguous();
-    int64_t d = 0;
-    for (const int64_t size : sizes)
-        fits = fits && tensor.size(d++) == size;
-    if (!fits) {
-        std::ostringstream shape;
-        d = 0;
-        for (const int64_t size : sizes)
-            shape << (d++ ? ", " : "") << size;
-        refuse(what, " ", name, " must be contiguous ", c10::toString(dtype), " of shape [", shape.str(), "] on ", device.str());
-    }
-}
-
-// Kernels move 16 bytes at a time; a view may start anywhere.
-void require_aligned(const torch::Tensor& tensor, const char* what, const char* name) {
-    if (reinterpret_cast<uintptr_t>(tensor.data_ptr()) % 16 != 0)
-        refuse(what, " ", name, " must start at a multiple of 16 bytes");
-}
-
-// Forward mode goes by the tensors alone: torch.no_grad() leaves it on.
-void require_no_tangent(const char* what, std::initializer_list<const torch::Tensor*> tensors) {
-    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode())
-        return;
-    for (const torch::Tensor* tensor : tensors)
-        TORCH_CHECK(tensor == nullptr || !tensor->_fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative");
-}
-
-void require_no_gradient(const char* what, std::initializer_list<const torch::Tensor*> tensors) {
-    require_no_tangent(what, tensors);
-    if (!at::GradMode::is_enabled())
-        return;
-    for (const torch::Tensor* tensor : tensors)
-        TORCH_CHECK(tensor == nullptr || !tensor->requires_grad(), what, " has no gradient: call it under torch.no_grad() or detach its inputs");
-}
-
-const void* pointer_of(const std::optional<torch::Tensor>& tensor) { return tensor.has_value() ? tensor->data_ptr() : nullptr; }
 
 struct Records {
     torch::Tensor payload, values, scales;

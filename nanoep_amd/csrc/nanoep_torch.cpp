@@ -1669,6 +1669,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, module) {
     py::class_<nanoep::CompletionEvent, std::shared_ptr<nanoep::CompletionEvent>>(module, "CompletionEvent")
         .def("current_stream_wait", &nanoep::CompletionEvent::current_stream_wait);
     nanoep::bind_operators(module);
+    nanoep::bind_entry(module);
     static nanoep::CallAhead dispatch_ahead, combine_ahead;
     nanoep::call_ahead_of(module, dispatch_ahead, "dispatch", &nanoep::call_dispatch, nanoep::g_bound_dispatch);
     nanoep::call_ahead_of(module, combine_ahead, "combine", &nanoep::call_combine, nanoep::g_bound_combine);
