@@ -17,6 +17,8 @@ namespace nanoep {
 namespace {
 
 constexpr int kMostThreads = 1024;
+constexpr int kBackwardThreads = 512;  // two wavefronts a SIMD: 256 registers a lane
+constexpr int kMostRowWaves = kMostThreads / kWave;
 constexpr int kMostHidden = 16384;
 
 struct Bf16 {};  // two bytes a value
@@ -44,48 +46,39 @@ struct RowType<Fp32> {
     }
 };
 
-// The parameters beside a row's vector `at`: as wide as its values, or fp32 beside bf16.
+// The parameters of a lane's vectors, kept as narrow as they lie in memory.
 template <class P, int kColumns>
-__device__ __forceinline__ void load_parameters(const u32x4* parameters, int at, float (&out)[kColumns]) {
-    if constexpr (RowType<P>::kColumns == kColumns) {
-        RowType<P>::unpack(parameters[at], out);
-    } else {
-        static_assert(kColumns == 8 && RowType<P>::kColumns == 4, "fp32 beside bf16");
+struct HeldParameters {
+    u32x4 data[kColumns / RowType<P>::kColumns];
+    __device__ __forceinline__ void load(const u32x4* parameters, int at) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const u32x4 data = parameters[2 * at + half];
+        for (int part = 0; part < kColumns / RowType<P>::kColumns; ++part)
+            data[part] = parameters[at * (kColumns / RowType<P>::kColumns) + part];
+    }
+    __device__ __forceinline__ void unpack(float (&out)[kColumns]) const {
+        if constexpr (RowType<P>::kColumns == 8) {
+            unpack_bf16(data[0], out);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                out[4 * half + i] = __uint_as_float(data[i]);
+            for (int i = 0; i < kColumns; ++i)
+                out[i] = __uint_as_float(data[i / 4][i % 4]);
         }
     }
+};
+
+// What the wavefronts of a row left in LDS, one in each of 16 neighbouring lanes; nothing behind the last.
+__device__ __forceinline__ float2 of_wavefront(const float2* places, int waves) {
+    const int lane = threadIdx.x % kMostRowWaves;
+    return lane < waves ? places[lane] : make_float2(0.0f, 0.0f);
 }
 
-// The sums over the wavefronts that share a row, in all of them.  One barrier; `place` is not used again before the next one.
-template <int kValues>
-__device__ __forceinline__ void row_sums(float (&v)[kValues], float (*place)[kValues], int first_wave, int wave, int waves) {
-#pragma unroll
-    for (int i = 0; i < kValues; ++i)
-        v[i] = lanes_sum<kWave>(v[i]);
-    if (waves == 1)
-        return;
-    if (threadIdx.x % kWave == 0)
-#pragma unroll
-        for (int i = 0; i < kValues; ++i)
-            place[first_wave + wave][i] = v[i];
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kValues; ++i)
-        v[i] = 0.0f;
-    for (int w = 0; w < waves; ++w)
-#pragma unroll
-        for (int i = 0; i < kValues; ++i)
-            v[i] += place[first_wave + w][i];
-}
-
-// blockDim.x lanes a row, blockDim.y rows; the row stays in registers (kVectors 16-byte vectors a lane) between its two
-// sums and its output, so that every input byte is read once.
-template <class T, class P, int kVectors>
+// A workgroup works through rows (`teams` at a time, those of a turn neighbours over all workgroups), blockDim.x lanes a row, with the
+// parameters in registers; a row stays there (kVectors 16-byte vectors a lane) between its sums and its output, so that every input
+// byte is read once, and the next row's inputs are on their way meanwhile.
+// One barrier a row: every wavefront has the mean and the squares about it of its own part, and the parts are put together as
+// mean = sum n_w m_w / H, squares = sum (squares_w + n_w (m_w - mean)^2), as good as squares about the row's mean.
+// kPastCache: the call's rows do not fit the last-level cache; then loads are the nontemporal ones, else the stores.
+template <class T, class P, int kVectors, bool kPastCache>
 __global__ void __launch_bounds__(kMostThreads) layer_norm_kernel(const u32x4* __restrict__ x,         // [T][vectors]
                                                                   const u32x4* __restrict__ residual,  // [T][vectors] or null
                                                                   const u32x4* __restrict__ gamma,
@@ -95,184 +88,266 @@ __global__ void __launch_bounds__(kMostThreads) layer_norm_kernel(const u32x4* _
                                                                   float* __restrict__ means,  // [T], null: the root-mean-square norm
                                                                   float* __restrict__ rstds,  // [T]
                                                                   int64_t rows,
+                                                                  int64_t groups,
                                                                   int vectors,
                                                                   float columns,
                                                                   float eps) {
     using Row = RowType<T>;
     constexpr int kColumns = Row::kColumns;
-    __shared__ float places[2][kMostThreads / kWave][1];
-    const int waves = blockDim.x / kWave, wave = threadIdx.x / kWave, first_wave = threadIdx.y * waves;
-    const int64_t row = workgroup_number() * blockDim.y + threadIdx.y;
-    const bool here = row < rows;
-    const int64_t base = here ? row * vectors : 0;
-    const int mine = here ? vectors : 0;  // (a row past the end has no vectors, but stays for the barriers)
+    __shared__ float2 places[2][kMostRowWaves];  // of a wavefront: squares, mean
+    // (a wavefront is one team's: what goes by the row is scalar)
+    const int waves = blockDim.x / kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int teams = blockDim.y, team = __builtin_amdgcn_readfirstlane(threadIdx.y), first_wave = team * waves;
+    const int64_t group = workgroup_number();
+    const bool centred = means != nullptr;
 
-    float s[kVectors][kColumns];
-    u32x4 data[kVectors], other[kVectors];
-    if (residual != nullptr) {
+    HeldParameters<P, kColumns> factors[kVectors], shifts[kVectors];
+    bool in_row[kVectors];
+    uint32_t place[kVectors];  // of a lane's vector in its row; lanes beside the row read the first one and count nothing
 #pragma unroll
-        for (int v = 0; v < kVectors; ++v) {
-            const int at = threadIdx.x + v * blockDim.x;
-            other[v] = at < mine ? residual[base + at] : u32x4{0u, 0u, 0u, 0u};
+    for (int v = 0; v < kVectors; ++v) {
+        const int at = threadIdx.x + v * blockDim.x;
+        in_row[v] = at < vectors;
+        place[v] = in_row[v] ? at : 0;
+    }
+    // columns of the row that wavefront w has
+    const auto part_of = [&](int w) {
+        int held = 0;
+#pragma unroll
+        for (int v = 0; v < kVectors && w < waves; ++v) {
+            const int left = vectors - w * kWave - v * static_cast<int>(blockDim.x);
+            held += left < 0 ? 0 : left > kWave ? kWave : left;
         }
-    }
-#pragma unroll
-    for (int v = 0; v < kVectors; ++v) {
-        const int at = threadIdx.x + v * blockDim.x;
-        data[v] = at < mine ? x[base + at] : u32x4{0u, 0u, 0u, 0u};
-    }
-    float factor[kVectors][kColumns], shift[kVectors][kColumns];
-#pragma unroll
-    for (int v = 0; v < kVectors; ++v) {
-        const int at = threadIdx.x + v * blockDim.x;
-        const int from = at < vectors ? at : 0;
-        load_parameters<P>(gamma, from, factor[v]);
-        if (beta != nullptr)
-            load_parameters<P>(beta, from, shift[v]);
-    }
-#pragma unroll
-    for (int v = 0; v < kVectors; ++v) {
-        Row::unpack(data[v], s[v]);
+        return static_cast<float>(held * kColumns);
+    };
+    const float own_part = part_of(wave), part = part_of(threadIdx.x % kMostRowWaves);
+    const float per_part = own_part > 0.0f ? 1.0f / own_part : 0.0f, per_column = 1.0f / columns;
+    u32x4 next[kVectors], next_added[kVectors];
+    const auto load = [&](int64_t row) {
+        row = row < rows ? row : rows - 1;  // (rows past the end are the last one again, and leave nothing)
+        const u32x4* row_x = x + row * vectors;
         if (residual != nullptr) {
-            const int at = threadIdx.x + v * blockDim.x;
-            float added[kColumns];
-            Row::unpack(other[v], added);
+            const u32x4* row_residual = residual + row * vectors;
 #pragma unroll
-            for (int i = 0; i < kColumns; ++i)
-                s[v][i] += added[i];
-            const u32x4 packed = Row::pack(s[v]);
-            if (at < mine)
-                store_vec<true>(total + base + at, packed);
-            Row::unpack(packed, s[v]);
+            for (int v = 0; v < kVectors; ++v)
+                next_added[v] = load_vec<kPastCache>(row_residual + place[v]);
         }
-    }
-    float mean = 0.0f;
-    if (means != nullptr) {
-        float sum[1] = {0.0f};
 #pragma unroll
         for (int v = 0; v < kVectors; ++v)
+            next[v] = load_vec<kPastCache>(row_x + place[v]);
+    };
+    const int64_t apart = groups * teams;
+    load(group * teams + team);
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v) {
+        factors[v].load(gamma, place[v]);
+        if (beta != nullptr)
+            shifts[v].load(beta, place[v]);
+    }
+    int turn = 0;
+    for (int64_t first = group * teams; first < rows; first += apart, turn ^= 1) {
+        const int64_t row = first + team;
+        const bool here = row < rows;
+        float s[kVectors][kColumns];
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            Row::unpack(next[v], s[v]);
+            if (residual != nullptr) {
+                float added[kColumns];
+                Row::unpack(next_added[v], added);
+#pragma unroll
+                for (int i = 0; i < kColumns; ++i)
+                    s[v][i] += added[i];
+                const u32x4 packed = Row::pack(s[v]);
+                if (here && in_row[v])
+                    store_vec<!kPastCache>(total + row * vectors + place[v], packed);
+                Row::unpack(packed, s[v]);
+            }
+        }
+        if (first + apart < rows)
+            load(row + apart);
+        float mean = 0.0f, squares = 0.0f;
+        if (centred) {
+#pragma unroll
+            for (int v = 0; v < kVectors; ++v) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kColumns; ++i)
+                    sum += s[v][i];
+                mean += in_row[v] ? sum : 0.0f;
+            }
+            mean = lanes_sum<kWave>(mean) * per_part;
+        }
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < kColumns; ++i)
-                sum[0] += s[v][i];
-        row_sums<1>(sum, places[0], first_wave, wave, waves);
-        mean = sum[0] / columns;
-    }
-    float squares[1] = {0.0f};
-#pragma unroll
-    for (int v = 0; v < kVectors; ++v) {
-        const bool in_row = static_cast<int>(threadIdx.x + v * blockDim.x) < mine;
-#pragma unroll
-        for (int i = 0; i < kColumns; ++i) {
-            s[v][i] = in_row ? s[v][i] - mean : 0.0f;
-            squares[0] = fmaf(s[v][i], s[v][i], squares[0]);
+                sum = fmaf(s[v][i] - mean, s[v][i] - mean, sum);
+            squares += in_row[v] ? sum : 0.0f;
         }
-    }
-    row_sums<1>(squares, places[1], first_wave, wave, waves);
-    const float rstd = 1.0f / sqrtf(squares[0] / columns + eps);
-    if (threadIdx.x == 0 && here) {
-        rstds[row] = rstd;
-        if (means != nullptr)
-            means[row] = mean;
-    }
-#pragma unroll
-    for (int v = 0; v < kVectors; ++v) {
-        const int at = threadIdx.x + v * blockDim.x;
-        if (at < mine) {
-            float y[kColumns];
-#pragma unroll
-            for (int i = 0; i < kColumns; ++i) {
-                y[i] = s[v][i] * rstd * factor[v][i];
-                if (beta != nullptr)
-                    y[i] += shift[v][i];
+        squares = lanes_sum<kWave>(squares);
+        if (waves > 1) {
+            if (threadIdx.x % kWave == 0)
+                places[turn][first_wave + wave] = make_float2(squares, mean);
+            __syncthreads();
+            const float2 other = of_wavefront(places[turn] + first_wave, waves);
+            squares = other.x;
+            if (centred) {
+                mean = lanes_sum<kMostRowWaves>(part * other.y) * per_column;
+                squares = fmaf(part * (other.y - mean), other.y - mean, squares);
             }
-            store_vec<true>(normalized + base + at, Row::pack(y));
+            squares = lanes_sum<kMostRowWaves>(squares);
+        }
+        const float rstd = rsqrtf(fmaf(squares, per_column, eps));
+        if (!here)
+            continue;
+        if (threadIdx.x == 0) {
+            rstds[row] = rstd;
+            if (centred)
+                means[row] = mean;
+        }
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            float factor[kColumns];
+            factors[v].unpack(factor);
+#pragma unroll
+            for (int i = 0; i < kColumns; ++i)
+                s[v][i] = (s[v][i] - mean) * rstd * factor[i];
+            if (beta != nullptr) {
+                float shift[kColumns];
+                shifts[v].unpack(shift);
+#pragma unroll
+                for (int i = 0; i < kColumns; ++i)
+                    s[v][i] += shift[i];
+            }
+            if (in_row[v])
+                store_vec<!kPastCache>(normalized + row * vectors + place[v], Row::pack(s[v]));
         }
     }
 }
 
-// The gradient.  A workgroup works through rows of its own (`per_team` rows a team of blockDim.x lanes) and keeps the two sums
-// over rows in registers; at its end it writes them, added over its teams, to its row of `sums` ([workgroups][2][columns] fp32),
-// which parameter_gradient_kernel adds up in a fixed order.  No atomics.
+// The gradient.  A workgroup works through rows (those of a turn are neighbours over all workgroups; `teams` of them at a time in a
+// workgroup) and keeps the two sums over rows in registers; at its end it writes them, added over its teams, to its row of `sums`
+// ([workgroups][2][columns] fp32), which parameter_gradient_kernel adds up in a fixed order.  No atomics.
+// With d = s - mean, along = sum(u * d): dx = r * u - r * mean(u) - d * r^3 * along / H.  d and u stay in registers between a row's sums
+// and its output; the next row's inputs are on their way meanwhile.
 template <class T, class P, int kVectors>
-__global__ void __launch_bounds__(kMostThreads) layer_norm_backward_kernel(const u32x4* __restrict__ grad,   // [T][vectors]
-                                                                           const u32x4* __restrict__ total,  // [T][vectors]
-                                                                           const u32x4* __restrict__ gamma,
-                                                                           const float* __restrict__ means,  // null: the root-mean-square norm
-                                                                           const float* __restrict__ rstds,
-                                                                           const u32x4* __restrict__ grad_residual,  // [T][vectors] or null
-                                                                           u32x4* __restrict__ grad_x,               // [T][vectors] or null
-                                                                           float* __restrict__ sums,                 // null: not wanted
-                                                                           int64_t rows,
-                                                                           int64_t per_team,
-                                                                           int vectors,
-                                                                           float columns) {
+__global__ void __launch_bounds__(kBackwardThreads) layer_norm_backward_kernel(const u32x4* __restrict__ grad,   // [T][vectors]
+                                                                               const u32x4* __restrict__ total,  // [T][vectors]
+                                                                               const u32x4* __restrict__ gamma,
+                                                                               const float* __restrict__ means,  // null: the root-mean-square norm
+                                                                               const float* __restrict__ rstds,
+                                                                               const u32x4* __restrict__ grad_residual,  // [T][vectors] or null
+                                                                               u32x4* __restrict__ grad_x,               // [T][vectors] or null
+                                                                               float* __restrict__ sums,                 // null: not wanted
+                                                                               int64_t rows,
+                                                                               int64_t groups,
+                                                                               int vectors,
+                                                                               float columns) {
     using Row = RowType<T>;
     constexpr int kColumns = Row::kColumns;
-    __shared__ float places[2][kMostThreads / kWave][2];
+    __shared__ float2 places[2][kBackwardThreads / kWave];
     extern __shared__ float team_sums[];  // [blockDim.y - 1][columns], if there are several teams
-    const int waves = blockDim.x / kWave, wave = threadIdx.x / kWave, first_wave = threadIdx.y * waves;
-    const int teams = blockDim.y;
-    const int64_t group = workgroup_number();
+    // (a wavefront is one team's: what goes by the row is scalar)
+    const int waves = blockDim.x / kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int teams = blockDim.y, team = __builtin_amdgcn_readfirstlane(threadIdx.y), first_wave = team * waves;
+    const int64_t group = blockIdx.x;
 
-    float factor[kVectors][kColumns], sum_z[kVectors][kColumns], sum_g[kVectors][kColumns];
+    HeldParameters<P, kColumns> held[kVectors];
+    float sum_z[kVectors][kColumns], sum_g[kVectors][kColumns];
+    bool in_row[kVectors];
+    uint32_t place[kVectors];  // of a lane's vector in its row; lanes beside the row read the first one and count nothing
 #pragma unroll
     for (int v = 0; v < kVectors; ++v) {
         const int at = threadIdx.x + v * blockDim.x;
-        load_parameters<P>(gamma, at < vectors ? at : 0, factor[v]);
+        in_row[v] = at < vectors;
+        place[v] = in_row[v] ? at : 0;
+        held[v].load(gamma, place[v]);
 #pragma unroll
         for (int i = 0; i < kColumns; ++i)
             sum_z[v][i] = sum_g[v][i] = 0.0f;
     }
-    for (int64_t turn = 0; turn < per_team; ++turn) {
-        const int64_t row = (group * per_team + turn) * teams + threadIdx.y;
-        const bool here = row < rows;
-        const int64_t base = here ? row * vectors : 0;
-        const int mine = here ? vectors : 0;
-        u32x4 data[kVectors], grads[kVectors], added[kVectors];
+    struct Inputs {
+        u32x4 total[kVectors], grad[kVectors], added[kVectors];
+        float mean, rstd;
+    };
+    // rows past the end are the last one again, and count nothing
+    const auto load = [&](int64_t row, Inputs& in) {
+        row = row < rows ? row : rows - 1;
+        const u32x4 *row_total = total + row * vectors, *row_grad = grad + row * vectors;
+        in.rstd = rstds[row];
+        in.mean = means != nullptr ? means[row] : 0.0f;
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
-            const int at = threadIdx.x + v * blockDim.x;
-            data[v] = at < mine ? load_vec<true>(total + base + at) : u32x4{0u, 0u, 0u, 0u};
-            grads[v] = at < mine ? load_vec<true>(grad + base + at) : u32x4{0u, 0u, 0u, 0u};
-            if (grad_residual != nullptr)
-                added[v] = at < mine ? load_vec<true>(grad_residual + base + at) : u32x4{0u, 0u, 0u, 0u};
+            in.total[v] = row_total[place[v]];
+            in.grad[v] = row_grad[place[v]];
         }
-        const float rstd = here ? rstds[row] : 0.0f, mean = here && means != nullptr ? means[row] : 0.0f;
-        float z[kVectors][kColumns], u[kVectors][kColumns], both[2] = {0.0f, 0.0f};
+        if (grad_residual != nullptr) {
+            const u32x4* row_added = grad_residual + row * vectors;
+#pragma unroll
+            for (int v = 0; v < kVectors; ++v)
+                in.added[v] = row_added[place[v]];
+        }
+    };
+    const float per_column = 1.0f / columns;
+    Inputs next;
+    const int64_t apart = groups * teams;
+    load(group * teams + team, next);
+    int turn = 0;
+    for (int64_t first = group * teams; first < rows; first += apart, turn ^= 1) {
+        const int64_t row = first + team;
+        const bool here = row < rows;
+        const float mean = next.mean, rstd = next.rstd;
+        float d[kVectors][kColumns], u[kVectors][kColumns], both[2] = {0.0f, 0.0f};
+        u32x4 added[kVectors];
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
-            const bool in_row = static_cast<int>(threadIdx.x + v * blockDim.x) < mine;
-            Row::unpack(data[v], z[v]);
-            Row::unpack(grads[v], u[v]);
+            float factor[kColumns];
+            Row::unpack(next.total[v], d[v]);
+            Row::unpack(next.grad[v], u[v]);
+            held[v].unpack(factor);
+            added[v] = next.added[v];
+            if (here && in_row[v]) {
 #pragma unroll
-            for (int i = 0; i < kColumns; ++i) {
-                const float g = u[v][i];
-                z[v][i] = in_row ? (z[v][i] - mean) * rstd : 0.0f;
-                u[v][i] = in_row ? g * factor[v][i] : 0.0f;
-                sum_g[v][i] += g;
-                sum_z[v][i] = fmaf(g, z[v][i], sum_z[v][i]);
-                both[0] += u[v][i];
-                both[1] = fmaf(u[v][i], z[v][i], both[1]);
+                for (int i = 0; i < kColumns; ++i) {
+                    const float g = u[v][i];
+                    d[v][i] -= mean;
+                    u[v][i] *= factor[i];
+                    sum_g[v][i] += g;
+                    sum_z[v][i] = fmaf(g * rstd, d[v][i], sum_z[v][i]);
+                    both[0] += u[v][i];
+                    both[1] = fmaf(u[v][i], d[v][i], both[1]);
+                }
             }
         }
+        load(row + apart, next);
         if (grad_x != nullptr) {
-            row_sums<2>(both, places[turn % 2], first_wave, wave, waves);
-            const float across = means != nullptr ? both[0] / columns : 0.0f, along = both[1] / columns;
+            both[0] = lanes_sum<kWave>(both[0]);
+            both[1] = lanes_sum<kWave>(both[1]);
+            if (waves > 1) {
+                if (threadIdx.x % kWave == 0)
+                    places[turn][first_wave + wave] = make_float2(both[0], both[1]);
+                __syncthreads();
+                const float2 other = of_wavefront(places[turn] + first_wave, waves);
+                both[0] = lanes_sum<kMostRowWaves>(other.x);
+                both[1] = lanes_sum<kMostRowWaves>(other.y);
+            }
+            const float across = means != nullptr ? both[0] * per_column * -rstd : 0.0f, along = both[1] * per_column * rstd * rstd * -rstd;
 #pragma unroll
             for (int v = 0; v < kVectors; ++v) {
-                const int at = threadIdx.x + v * blockDim.x;
-                if (at < mine) {
-                    float out[kColumns], more[kColumns];
-                    if (grad_residual != nullptr)
-                        Row::unpack(added[v], more);
 #pragma unroll
-                    for (int i = 0; i < kColumns; ++i) {
-                        out[i] = (u[v][i] - across - z[v][i] * along) * rstd;
-                        if (grad_residual != nullptr)
-                            out[i] += more[i];
-                    }
-                    store_vec<true>(grad_x + base + at, Row::pack(out));
+                for (int i = 0; i < kColumns; ++i)
+                    u[v][i] = fmaf(u[v][i], rstd, fmaf(d[v][i], along, across));
+                if (grad_residual != nullptr) {
+                    float more[kColumns];
+                    Row::unpack(added[v], more);
+#pragma unroll
+                    for (int i = 0; i < kColumns; ++i)
+                        u[v][i] += more[i];
                 }
+                if (here && in_row[v])
+                    store_vec<true>(grad_x + row * vectors + place[v], Row::pack(u[v]));
             }
         }
     }
@@ -287,27 +362,27 @@ __global__ void __launch_bounds__(kMostThreads) layer_norm_backward_kernel(const
         auto& own = which == 0 ? sum_z : sum_g;
         if (teams > 1) {
             __syncthreads();
-            if (threadIdx.y > 0)
+            if (team > 0)
 #pragma unroll
                 for (int v = 0; v < kVectors; ++v) {
                     const int at = threadIdx.x + v * blockDim.x;
                     if (at < vectors)
 #pragma unroll
                         for (int i = 0; i < kColumns; ++i)
-                            team_sums[(threadIdx.y - 1) * width + at * kColumns + i] = own[v][i];
+                            team_sums[(team - 1) * width + at * kColumns + i] = own[v][i];
                 }
             __syncthreads();
         }
-        if (threadIdx.y == 0)
+        if (team == 0)
 #pragma unroll
             for (int v = 0; v < kVectors; ++v) {
                 const int at = threadIdx.x + v * blockDim.x;
                 if (at >= vectors)
                     continue;
-                for (int team = 1; team < teams; ++team)
+                for (int other = 1; other < teams; ++other)
 #pragma unroll
                     for (int i = 0; i < kColumns; ++i)
-                        own[v][i] += team_sums[(team - 1) * width + at * kColumns + i];
+                        own[v][i] += team_sums[(other - 1) * width + at * kColumns + i];
                 float* to = sums + (2 * group + which) * width + static_cast<int64_t>(at) * kColumns;
 #pragma unroll
                 for (int i = 0; i < kColumns; i += 4)
@@ -316,8 +391,8 @@ __global__ void __launch_bounds__(kMostThreads) layer_norm_backward_kernel(const
     }
 }
 
-// dgamma and dbeta from the workgroups' sums: 64 columns a workgroup, its 16 groups of 16 lanes share out the rows of sums.
-constexpr int kSumLanes = 16, kSumGroups = 16;
+// dgamma and dbeta from the workgroups' sums: 64 columns a workgroup, its 64 groups of 16 lanes share out the rows of sums.
+constexpr int kSumLanes = 16, kSumGroups = 64;
 template <class P>
 __global__ void __launch_bounds__(kSumLanes * kSumGroups) parameter_gradient_kernel(const u32x4* __restrict__ sums,  // [groups][2][columns / 4]
                                                                                     void* __restrict__ grad_gamma,
@@ -330,7 +405,7 @@ __global__ void __launch_bounds__(kSumLanes * kSumGroups) parameter_gradient_ker
     const int which = blockIdx.y;
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (at < quads) {
-#pragma unroll 8
+#pragma unroll 4
         for (int64_t group = part; group < groups; group += kSumGroups) {
             const u32x4 data = sums[(2 * group + which) * quads + at];
 #pragma unroll
@@ -341,13 +416,15 @@ __global__ void __launch_bounds__(kSumLanes * kSumGroups) parameter_gradient_ker
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         parts[part][lane][i] = sum[i];
-    __syncthreads();
+    for (int half = kSumGroups / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if (part < half)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                parts[part][lane][i] = sum[i] += parts[part + half][lane][i];
+    }
     if (part > 0 || at >= quads)
         return;
-    for (int other = 1; other < kSumGroups; ++other)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            sum[i] += parts[other][lane][i];
     void* out = which == 0 ? grad_gamma : grad_beta;
     if constexpr (RowType<P>::kColumns == 8)
         static_cast<uint2*>(out)[at] = make_uint2(to_bf16_pair(sum[0], sum[1]), to_bf16_pair(sum[2], sum[3]));
@@ -355,20 +432,20 @@ __global__ void __launch_bounds__(kSumLanes * kSumGroups) parameter_gradient_ker
         static_cast<u32x4*>(out)[at] = RowType<Fp32>::pack(sum);
 }
 
-// Lanes and vectors a lane for rows of `vectors` vectors: two vectors a lane, more only where 1024 lanes would not do.  By the
+// Lanes and vectors a lane for rows of `vectors` vectors: two vectors a lane, more only where `most` lanes would not do.  By the
 // row's length alone, so that a row's result is the same in any batch.
 struct RowShape {
-    int held;     // 1, 2 or 4
+    int held;     // 1, 2, 4 or 8
     int threads;  // a multiple of 64
 };
-RowShape shape_of(int vectors) {
+RowShape shape_of(int vectors, int most) {
     int held = vectors > kWave ? 2 : 1;
-    while ((vectors + held - 1) / held > kMostThreads)
+    while ((vectors + held - 1) / held > most)
         held *= 2;
     return {held, static_cast<int>(align_up(static_cast<size_t>((vectors + held - 1) / held), kWave))};
 }
 
-// Rows of a workgroup: several where a row takes few lanes.
+// Rows of a workgroup of the norm: several where a row takes few lanes.
 int teams_of(int threads) { return std::max(1, kBlockThreads / threads); }
 
 bool types_fit(int rows_type, int parameters_type) {
@@ -381,19 +458,19 @@ bool norm_sizes_fit(int64_t num_tokens, int hidden, int rows_type, int parameter
            types_fit(rows_type, parameters_type);
 }
 
+// One workgroup a compute unit (or less), so that there are few rows of sums to write and to add up again.
 struct BackwardPlan {
     RowShape shape;
     int vectors, teams;
-    int64_t per_team, groups;
+    int64_t groups;
 };
 BackwardPlan plan_backward(int64_t num_tokens, int hidden, int rows_type, const Topology& topology) {
     BackwardPlan plan;
     plan.vectors = hidden / (rows_type == NANOEP_BF16 ? 8 : 4);
-    plan.shape = shape_of(plan.vectors);
-    plan.teams = teams_of(plan.shape.threads);
-    const int64_t most = 2 * int64_t{topology.cus};
-    plan.per_team = std::max<int64_t>(1, (num_tokens + most * plan.teams - 1) / (most * plan.teams));
-    plan.groups = (num_tokens + plan.per_team * plan.teams - 1) / (plan.per_team * plan.teams);
+    plan.shape = shape_of(plan.vectors, kBackwardThreads);
+    const int64_t most = topology.cus, rows_each = std::max<int64_t>(1, (num_tokens + most - 1) / most);
+    plan.teams = static_cast<int>(std::min<int64_t>(kBackwardThreads / plan.shape.threads, rows_each));
+    plan.groups = std::min(most, (num_tokens + plan.teams - 1) / plan.teams);
     return plan;
 }
 
@@ -401,20 +478,30 @@ template <class T, class P>
 int launch_norm(const void* x, const void* residual, const void* gamma, const void* beta, int64_t num_tokens, int hidden, float eps, void* total,
                 void* normalized, float* mean, float* rstd, hipStream_t stream) {
     const int vectors = hidden / RowType<T>::kColumns;
-    const RowShape shape = shape_of(vectors);
+    const RowShape shape = shape_of(vectors, kMostThreads);
     const int teams = teams_of(shape.threads);
-    const dim3 grid = grid_of((num_tokens + teams - 1) / teams), block(shape.threads, teams);
+    // 16 wavefronts a compute unit, the rows dealt out evenly (4096 x 7168 with a residual, two workgroups of seven: 37.6 us, one 39.4,
+    // three 41.9, a row a workgroup 41.5)
+    const int64_t most = int64_t{current_topology(current_tuning()).cus} * std::max(1, kMostRowWaves / (shape.threads / kWave * teams));
+    const int64_t turns = (num_tokens + most * teams - 1) / (most * teams);
+    const int64_t groups = (num_tokens + turns * teams - 1) / (turns * teams);
+    const dim3 grid = grid_of(groups), block(shape.threads, teams);
     const auto launch = [&](auto kernel) {
         kernel<<<grid, block, 0, stream>>>(static_cast<const u32x4*>(x), static_cast<const u32x4*>(residual), static_cast<const u32x4*>(gamma),
                                            static_cast<const u32x4*>(beta), static_cast<u32x4*>(total), static_cast<u32x4*>(normalized), mean,
-                                           rstd, num_tokens, vectors, static_cast<float>(hidden), eps);
+                                           rstd, num_tokens, groups, vectors, static_cast<float>(hidden), eps);
     };
+    // Nontemporal loads or stores, by the bytes of all rows (us; nontemporal loads, nontemporal stores): 235 MB 38.2, 42.0; 196 MB
+    // 32.1, 32.3; 134 MB 23.3, 21.2; 82 MB 15.9, 13.9.
+    const int64_t bytes = num_tokens * vectors * 16 * (residual != nullptr ? 4 : 2);
+    const bool past_cache = bytes > kLastLevelCacheBytes / 4 * 3;
+    const auto pick = [&](auto near, auto far) { past_cache ? launch(far) : launch(near); };
     if (shape.held == 1)
-        launch(layer_norm_kernel<T, P, 1>);
+        pick(layer_norm_kernel<T, P, 1, false>, layer_norm_kernel<T, P, 1, true>);
     else if (shape.held == 2)
-        launch(layer_norm_kernel<T, P, 2>);
+        pick(layer_norm_kernel<T, P, 2, false>, layer_norm_kernel<T, P, 2, true>);
     else if constexpr (RowType<T>::kColumns == 4)  // (the longest rows in bf16 are two vectors a lane)
-        launch(layer_norm_kernel<T, P, 4>);
+        pick(layer_norm_kernel<T, P, 4, false>, layer_norm_kernel<T, P, 4, true>);
     NANOEP_HIP_TRY(hipGetLastError());
     return NANOEP_OK;
 }
@@ -425,19 +512,21 @@ int launch_backward(const BackwardPlan& plan, const void* grad, const void* tota
                     hipStream_t stream) {
     if (plan.groups > 0) {
         const size_t lds = grad_gamma != nullptr ? static_cast<size_t>(plan.teams - 1) * hidden * sizeof(float) : 0;
-        const dim3 grid = grid_of(plan.groups), block(plan.shape.threads, plan.teams);
+        const dim3 grid(static_cast<unsigned>(plan.groups)), block(plan.shape.threads, plan.teams);
         const auto launch = [&](auto kernel) {
             kernel<<<grid, block, lds, stream>>>(static_cast<const u32x4*>(grad), static_cast<const u32x4*>(total),
                                                  static_cast<const u32x4*>(gamma), mean, rstd, static_cast<const u32x4*>(grad_residual),
                                                  static_cast<u32x4*>(grad_x), grad_gamma != nullptr ? static_cast<float*>(workspace) : nullptr,
-                                                 num_tokens, plan.per_team, plan.vectors, static_cast<float>(hidden));
+                                                 num_tokens, plan.groups, plan.vectors, static_cast<float>(hidden));
         };
         if (plan.shape.held == 1)
             launch(layer_norm_backward_kernel<T, P, 1>);
         else if (plan.shape.held == 2)
             launch(layer_norm_backward_kernel<T, P, 2>);
-        else if constexpr (RowType<T>::kColumns == 4)
+        else if (plan.shape.held == 4)
             launch(layer_norm_backward_kernel<T, P, 4>);
+        else if constexpr (RowType<T>::kColumns == 4)
+            launch(layer_norm_backward_kernel<T, P, 8>);
         NANOEP_HIP_TRY(hipGetLastError());
     }
     if (grad_gamma != nullptr) {
