@@ -7,6 +7,9 @@
 
 namespace nanoep {
 
+struct LanesMin {
+    __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return a < b ? a : b; }
+};
 struct LanesMax {
     __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return a > b ? a : b; }
     // (of two values the one that is no NaN)
@@ -82,9 +85,61 @@ template <int kLanes, class T>
 __device__ __forceinline__ T lanes_max(T v) {
     return lanes_reduce<kLanes>(v, LanesMax{});
 }
+template <int kLanes>
+__device__ __forceinline__ uint32_t lanes_min(uint32_t v) {
+    return lanes_reduce<kLanes>(v, LanesMin{});
+}
 template <int kLanes, class T>
 __device__ __forceinline__ T lanes_sum(T v) {
     return lanes_reduce<kLanes>(v, LanesSum{});
+}
+
+// The lanes of a group of kLanes for which `condition` holds, the group's first lane as bit 0.
+template <int kLanes>
+__device__ __forceinline__ uint64_t lanes_where(bool condition) {
+    const uint64_t all = __ballot(condition);
+    if constexpr (kLanes == 64)
+        return all;
+    return all >> (threadIdx.x % kWave / kLanes * kLanes) & ((uint64_t{1} << kLanes) - 1);
+}
+
+// The sum over the lanes of a group of kLanes ahead of this one.
+template <int kLanes>
+__device__ __forceinline__ uint32_t lanes_before(uint32_t v) {
+    static_assert(kLanes >= 16, "whole rows of 16");
+    uint32_t up_to = v;
+    up_to += lanes_moved<0x111>(up_to);  // row_shr 1, zero at the row's start
+    up_to += lanes_moved<0x112>(up_to);
+    up_to += lanes_moved<0x114>(up_to);
+    up_to += lanes_moved<0x118>(up_to);
+    for (int row = 16; row < kLanes; row += 16) {  // a row's end goes into the next one
+        const uint32_t ahead = __shfl(up_to, (threadIdx.x % kWave / kLanes) * kLanes + row - 1, kWave);
+        up_to += threadIdx.x % kLanes / 16 * 16 == row ? ahead : 0;
+    }
+    return up_to - v;
+}
+
+// The sum over the lanes of a wavefront that are in the same place of their groups of kLanes.
+template <int kLanes>
+__device__ __forceinline__ float groups_sum(float v) {
+    float a, b;
+    if constexpr (kLanes <= 8)
+        v += lanes_moved<0x128>(v);  // row_ror 8
+    if constexpr (kLanes <= 16) {
+        lanes_pair<16>(v, a, b);
+        v = a + b;
+    }
+    if constexpr (kLanes <= 32) {
+        lanes_pair<32>(v, a, b);
+        v = a + b;
+    }
+    return v;
+}
+
+// What a wavefront's lanes wrote to LDS is there for its other lanes (LDS works a wavefront's accesses off in order).
+__device__ __forceinline__ void wavefront_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 }  // namespace nanoep
