@@ -407,7 +407,7 @@ int nanoep_route_topk_backward(const float* grad, const void* logits, int64_t lo
  * The gradient in the logits, for grad (fp32 [S]) and the counts and tokens that the loss left (counts have none): [T, E],
  * contiguous, zero for tokens without a choice and those of no sequence.
  */
-size_t nanoep_balance_loss_workspace_bytes(int64_t num_tokens, int num_experts, int64_t sequences);
+size_t nanoep_balance_loss_workspace_bytes(int64_t num_tokens, int num_experts, int num_topk, int64_t sequences);
 int nanoep_balance_loss(const void* logits, int64_t logits_stride, int logits_type, const int64_t* ids, const int64_t* sequence_offsets,
                         int64_t num_tokens, int num_experts, int num_topk, int64_t sequences, int scoring, float* loss, int64_t* counts,
                         int64_t* tokens, void* workspace, size_t workspace_bytes, void* stream);

@@ -247,7 +247,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> balance_loss(const torch
         counts = make({a.experts}, at::kLong, device);
         tokens = make({}, at::kLong, device);
     }
-    const size_t bytes = nanoep_balance_loss_workspace_bytes(a.tokens, a.experts, sequences);
+    const size_t bytes = nanoep_balance_loss_workspace_bytes(a.tokens, a.experts, topk, sequences);
     if (bytes > 0)
         workspace = make({static_cast<int64_t>(bytes)}, at::kByte, device);
     check(nanoep_balance_loss(logits.data_ptr(), a.stride, a.type, static_cast<const int64_t*>(ids.data_ptr()),

@@ -556,6 +556,14 @@ __global__ void __launch_bounds__(kBlockThreads) route_values_kernel(const Route
 
 // ------------------------------------------------------------------ gradients of a token's scores
 
+// e^x for x <= 0, good to 2^-22: the product with log2 e is kept with its rounding.
+__device__ __forceinline__ float exp_below(float x) {
+    x = x < -200.0f ? -200.0f : x;  // (a NaN stays one)
+    const float whole = x * 0x1.715476p+0f;
+    const float rounding = fmaf(x, 0x1.4ae0cp-26f, fmaf(x, 0x1.715476p+0f, -whole));
+    return fmaf(__builtin_amdgcn_exp2f(whole), rounding * 0x1.62e43p-1f, __builtin_amdgcn_exp2f(whole));
+}
+
 // Every expert's share of its token: softmax, or sigmoid over its sum.  rest: what is left of its sigmoid to one (softmax: 1).
 // Experts at -infinity have none; a token of nothing else has no shares.
 template <int kLanes, int kEach>
@@ -565,20 +573,27 @@ __device__ __forceinline__ void shares_of(const float (&logit)[kEach], bool sigm
     for (int i = 0; i < kEach; ++i)
         largest = fmaxf(largest, logit[i]);
     largest = lanes_max<kLanes>(largest);
-    const float shift = largest == -INFINITY ? 0.0f : sigmoid ? fminf(largest, 0.0f) : largest;
+    if (sigmoid) {
+        // times e^-shift, so that the sum is not lost where all of them are tiny; mostly there is a logit above 0
+        const float shift = largest == -INFINITY ? 0.0f : fminf(largest, 0.0f);
+        const bool shifted = __any(shift < 0.0f);
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        if (sigmoid) {
-            // e^-shift * sigmoid: the sum is not lost where all of them are tiny
-            const float tail = expf(-fabsf(logit[i]));
-            const float inverse = 1.0f / (1.0f + tail);
-            share[i] = logit[i] != logit[i] ? logit[i] : expf(fminf(logit[i], 0.0f) - shift) * inverse;
+        for (int i = 0; i < kEach; ++i) {
+            const float tail = exp_below(-fabsf(logit[i])), inverse = __builtin_amdgcn_rcpf(1.0f + tail);
+            share[i] = logit[i] >= 0.0f ? inverse : tail * inverse;
             rest[i] = logit[i] >= 0.0f ? tail * inverse : inverse;
-        } else {
-            share[i] = expf(logit[i] - shift);
-            rest[i] = 1.0f;
+            if (shifted && logit[i] < 0.0f)
+                share[i] = exp_below(logit[i] - shift) * inverse;
+            total += share[i];
         }
-        total += share[i];
+    } else {
+        const float shift = largest == -INFINITY ? 0.0f : largest;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            share[i] = exp_below(logit[i] - shift);
+            rest[i] = 1.0f;
+            total += share[i];
+        }
     }
     total = lanes_sum<kLanes>(total);
     const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
@@ -688,36 +703,46 @@ struct Balance {
     const int64_t* ids;      // [T][K]
     const int64_t* offsets;  // [S + 1], null: all tokens are one sequence
     int64_t tokens, sequences;
-    int experts, topk, parts;  // workgroups a sequence
+    int chunk_bits;  // a workgroup (the gradient: a wavefront) has 2^chunk_bits tokens, wherever sequences begin
+    int experts, topk;
     bool sigmoid;
 };
 
-// The tokens of a part of a sequence, within the batch whatever the offsets say.
-__device__ __forceinline__ void part_of(const Balance& a, int64_t sequence, int part, int64_t& from, int64_t& to) {
-    int64_t begin = 0, end = a.tokens;
-    if (a.offsets != nullptr) {
-        begin = a.offsets[sequence];
-        end = a.offsets[sequence + 1];
-        begin = begin < 0 ? 0 : begin;
-        end = end > a.tokens ? a.tokens : end;
-    }
-    const int64_t length = end > begin ? end - begin : 0, each = (length + a.parts - 1) / a.parts;
-    from = begin + (part * each < length ? part * each : length);
-    to = from + each < begin + length ? from + each : begin + length;
+// The tokens of a sequence that are in [from, to).
+__device__ __forceinline__ void clip(const Balance& a, int64_t sequence, int64_t& from, int64_t& to) {
+    if (a.offsets == nullptr)
+        return;
+    const int64_t begin = uniform_load(a.offsets + sequence), end = uniform_load(a.offsets + sequence + 1);
+    from = begin > from ? begin : from;
+    to = end < to ? end : to;
 }
 
-// Whether the token that kLanes lanes share has a choice; each one is given to `count`, once.
-template <int kLanes, class Count>
-__device__ __forceinline__ bool has_choice(const Balance& a, int64_t token, bool here, Count count) {
-    bool any = false;
-    for (int k = threadIdx.x % kLanes; k < a.topk; k += kLanes) {
-        const int64_t named = here ? a.ids[token * a.topk + k] : -1;
-        if (named >= 0 && named < a.experts) {
-            any = true;
-            count(static_cast<int>(named));
+// The sequences that end at or ahead of a token, counted by the threads of a wavefront: the first that can have it.
+__device__ __forceinline__ int64_t sequences_ahead(const Balance& a, int64_t token) {
+    int64_t ahead = 0;
+    if (a.offsets != nullptr)
+        for (int64_t base = 0; base < a.sequences; base += kWave) {
+            const int64_t sequence = base + threadIdx.x % kWave;
+            ahead += __popcll(__ballot(sequence < a.sequences && a.offsets[sequence + 1] <= token));
         }
-    }
-    return lanes_where<kLanes>(any) != 0;
+    return ahead;
+}
+
+// A token of each group of kLanes lanes: its logits, and choice k in lane k.
+template <int kEach>
+struct BalanceToken {
+    float logit[kEach];
+    int64_t named;
+    bool here;
+};
+template <int kLanes, int kEach>
+__device__ __forceinline__ void load_token(const Balance& a, int64_t token, bool here, BalanceToken<kEach>& out) {
+    const int lane = threadIdx.x % kLanes;
+    out.here = here;
+    out.named = -1;
+    if (here && lane < a.topk)
+        out.named = a.ids[token * a.topk + lane];
+    load_spread<kLanes, kEach>(a.logits, token, here, a.experts, out.logit);
 }
 
 __device__ __forceinline__ float workgroup_sum(float v, float* place) {
@@ -732,215 +757,290 @@ __device__ __forceinline__ float workgroup_sum(float v, float* place) {
     return v;
 }
 
-// counts, tokens and loss of a sequence from the sums over its tokens: loss = E / (C T') * sum over e of c_e * sum of shares.
-// Each thread has the experts from threadIdx.x on, blockDim.x apart.
-__device__ __forceinline__ void finish_sequence(int64_t sequence, int experts, const float* shares, const int* chosen, int live, float* loss,
-                                                int64_t* counts, int64_t* tokens, float* place) {
-    float sum = 0.0f, number = 0.0f;
-    for (int e = threadIdx.x; e < experts; e += blockDim.x) {
-        counts[sequence * experts + e] = chosen[e];
-        sum = fmaf(static_cast<float>(chosen[e]), shares[e], sum);
-        number += static_cast<float>(chosen[e]);
-    }
-    sum = workgroup_sum(sum, place);
-    number = workgroup_sum(number, place);
-    if (threadIdx.x == 0) {
-        tokens[sequence] = live;
-        loss[sequence] = live > 0 ? sum * static_cast<float>(experts) / number / static_cast<float>(live) : 0.0f;
-    }
+// loss = E / (C T') * sum over e of c_e * its sum of shares.
+__device__ __forceinline__ float loss_of(int experts, float sum, float number, int live) {
+    return live > 0 ? sum * static_cast<float>(experts) / number / static_cast<float>(live) : 0.0f;
 }
 
-// Wavefronts of a workgroup, by the experts a lane has (registers, and LDS: half of the wavefronts' sums and the counts).
-constexpr int kMostBalanceWaves = 16;
-constexpr int balance_waves(int each) { return each <= 16 ? kMostBalanceWaves : 4; }
-
-// A workgroup a part of a sequence: kLanes lanes a token at a time, which keep their experts' sums of shares in registers;
-// choices are counted in LDS (whole numbers: any order gives the same).  The sums of a wavefront's tokens, then those of the wavefronts
-// are added in a fixed order.  A sequence of one part is finished here, others leave a row of sums to balance_finish_kernel.
+// A workgroup has a chunk of tokens, whatever sequences they are of: kLanes lanes a token at a time, which keep their experts' sums of shares in
+// registers, the next token's inputs on their way; choices are counted in LDS (whole numbers: any order gives the same).  The sums of a
+// wavefront's tokens, then those of the wavefronts are added in a fixed order.  Chunk c leaves its part of sequence s in row c + s of
+// `rows` (from one to the next either c or s goes up by one), shares, then counts, as wide as the lanes' experts, for
+// balance_finish_kernel, whose count of workgroups that have arrived the first one clears.  One sequence of one chunk is finished here.
 template <int kLanes, int kEach>
-__global__ void __launch_bounds__(balance_waves(kEach) * kWave) balance_loss_kernel(const Balance a, float* __restrict__ part_shares,  // [S * parts][E]
-                                                                                    int* __restrict__ part_counts,  // [S * parts][E + 1]
-                                                                                    float* __restrict__ loss, int64_t* __restrict__ counts,
-                                                                                    int64_t* __restrict__ tokens) {
-    constexpr int kWidth = kLanes * kEach, kWaves = balance_waves(kEach);
+__global__ void __launch_bounds__(kBlockThreads) balance_loss_kernel(const Balance a, uint32_t* __restrict__ rows,  // null: finished here
+                                                                     int* __restrict__ live_of_rows, int* __restrict__ arrived,
+                                                                     float* __restrict__ loss, int64_t* __restrict__ counts,
+                                                                     int64_t* __restrict__ tokens) {
+    constexpr int kWidth = kLanes * kEach, kWaves = kWavesPerBlock, kTokens = kBlockThreads / kLanes;
     __shared__ float sums[kWaves / 2 * kWidth];
     __shared__ int chosen[kWidth];
     __shared__ float place[kWaves];
     __shared__ int live_tokens;
-    const int64_t block = workgroup_number();
-    if (block >= a.sequences * a.parts)
+    const int64_t chunk = workgroup_number(), begin = chunk << a.chunk_bits, length = int64_t{1} << a.chunk_bits;
+    if (begin >= a.tokens)
         return;
-    const int64_t sequence = block / a.parts;
-    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kLanes;
-    for (int e = threadIdx.x; e < kWidth; e += kWaves * kWave)
-        chosen[e] = 0;
-    if (threadIdx.x == 0)
-        live_tokens = 0;
-    __syncthreads();
-
-    int64_t from, to;
-    part_of(a, sequence, static_cast<int>(block - sequence * a.parts), from, to);
-    float own[kEach];
-#pragma unroll
-    for (int i = 0; i < kEach; ++i)
-        own[i] = 0.0f;
-    int number = 0;
-    constexpr int kTokens = kWaves * kWave / kLanes;
-    for (int64_t first = from; first < to; first += kTokens) {
-        const int64_t token = first + threadIdx.x / kLanes;
-        const bool here = token < to;
-        float logit[kEach], share[kEach], rest[kEach];
-        load_spread<kLanes, kEach>(a.logits, token, here, a.experts, logit);
-        const bool live = has_choice<kLanes>(a, token, here, [&](int expert) { atomicAdd(&chosen[expert], 1); });
-        number += live ? 1 : 0;
-        shares_of<kLanes, kEach>(logit, a.sigmoid, share, rest);
-#pragma unroll
-        for (int i = 0; i < kEach; ++i)
-            own[i] += live ? share[i] : 0.0f;
-    }
-    if (lane == 0 && number > 0)
-        atomicAdd(&live_tokens, number);
-#pragma unroll
-    for (int i = 0; i < kEach; ++i)
-        own[i] = groups_sum<kLanes>(own[i]);
-    const bool writes = threadIdx.x % kWave < kLanes;
-    for (int half = kWaves / 2; half > 0; half /= 2) {
-        if (wave >= half && wave < 2 * half && writes)
-#pragma unroll
-            for (int i = 0; i < kEach; ++i)
-                sums[(wave - half) * kWidth + i * kLanes + lane] = own[i];
-        __syncthreads();
-        if (wave < half)
-#pragma unroll
-            for (int i = 0; i < kEach; ++i)
-                own[i] += sums[wave * kWidth + i * kLanes + lane];
-        __syncthreads();
-    }
-    if (wave == 0 && writes)
-#pragma unroll
-        for (int i = 0; i < kEach; ++i)
-            sums[i * kLanes + lane] = own[i];
-    __syncthreads();
-    if (a.parts > 1) {
-        for (int e = threadIdx.x; e < a.experts; e += kWaves * kWave) {
-            part_shares[block * a.experts + e] = sums[e];
-            part_counts[block * (a.experts + 1) + e] = chosen[e];
-        }
+    if (arrived != nullptr && chunk == 0 && threadIdx.x == 0)
+        *arrived = 0;
+    const int64_t end = begin + length < a.tokens ? begin + length : a.tokens;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    for (int64_t sequence = sequences_ahead(a, begin); sequence < a.sequences; ++sequence) {
+        int64_t from = begin, to = end;
+        clip(a, sequence, from, to);
+        if (from >= end)
+            break;
+        BalanceToken<kEach> next;
+        load_token<kLanes, kEach>(a, from + group, from + group < to, next);
+        __syncthreads();  // (the last sequence's are read)
+        for (int e = threadIdx.x; e < kWidth; e += kWaves * kWave)
+            chosen[e] = 0;
         if (threadIdx.x == 0)
-            part_counts[block * (a.experts + 1) + a.experts] = live_tokens;
-        return;
+            live_tokens = 0;
+        __syncthreads();
+        float own[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            own[i] = 0.0f;
+        int number = 0;
+        for (int64_t first = from; first < to; first += kTokens) {
+            const BalanceToken<kEach> token = next;
+            load_token<kLanes, kEach>(a, first + kTokens + group, first + kTokens + group < to, next);
+            const bool valid = token.named >= 0 && token.named < a.experts;
+            if (valid)
+                atomicAdd(&chosen[token.named], 1);
+            const bool live = lanes_where<kLanes>(valid) != 0;
+            number += live ? 1 : 0;
+            float share[kEach], rest[kEach];
+            shares_of<kLanes, kEach>(token.logit, a.sigmoid, share, rest);
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+                own[i] += live ? share[i] : 0.0f;
+        }
+        if (lane == 0 && number > 0)
+            atomicAdd(&live_tokens, number);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            own[i] = groups_sum<kLanes>(own[i]);
+        const bool writes = threadIdx.x % kWave < kLanes;
+        for (int half = kWaves / 2; half > 0; half /= 2) {
+            if (wave >= half && wave < 2 * half && writes)
+#pragma unroll
+                for (int i = 0; i < kEach; ++i)
+                    sums[(wave - half) * kWidth + i * kLanes + lane] = own[i];
+            __syncthreads();
+            if (wave < half)
+#pragma unroll
+                for (int i = 0; i < kEach; ++i)
+                    own[i] += sums[wave * kWidth + i * kLanes + lane];
+            __syncthreads();
+        }
+        if (rows != nullptr) {
+            uint32_t* row = rows + (chunk + sequence) * 2 * kWidth;
+            if (wave == 0 && writes)
+#pragma unroll
+                for (int i = 0; i < kEach; ++i)
+                    row[i * kLanes + lane] = __float_as_uint(own[i]);
+            for (int e = threadIdx.x; e < kWidth; e += kWaves * kWave)
+                row[kWidth + e] = static_cast<uint32_t>(chosen[e]);
+            if (threadIdx.x == 0)
+                live_of_rows[chunk + sequence] = live_tokens;
+            continue;
+        }
+        if (wave == 0 && writes)
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+                sums[i * kLanes + lane] = own[i];
+        __syncthreads();
+        float sum = 0.0f, all = 0.0f;
+        for (int e = threadIdx.x; e < a.experts; e += kBlockThreads) {
+            counts[e] = chosen[e];
+            sum = fmaf(static_cast<float>(chosen[e]), sums[e], sum);
+            all += static_cast<float>(chosen[e]);
+        }
+        sum = workgroup_sum(sum, place);
+        all = workgroup_sum(all, place);
+        if (threadIdx.x == 0) {
+            *tokens = live_tokens;
+            *loss = loss_of(a.experts, sum, all, live_tokens);
+        }
     }
-    finish_sequence(sequence, a.experts, sums, chosen, live_tokens, loss, counts, tokens, place);
 }
 
-constexpr int kFinishThreads = 1024;
+// The sum over `lanes` (a power of two) neighbouring lanes, in all of them.
+template <class T>
+__device__ __forceinline__ T sum_of_lanes(T v, int lanes) {
+    T a, b;
+    v += lanes >= 2 ? lanes_moved<0xB1>(v) : T{0};
+    v += lanes >= 4 ? lanes_moved<0x4E>(v) : T{0};
+    v += lanes >= 8 ? lanes_moved<0x141>(v) : T{0};
+    v += lanes >= 16 ? lanes_moved<0x140>(v) : T{0};
+    lanes_pair<16>(v, a, b);
+    v = lanes >= 32 ? a + b : v;
+    lanes_pair<32>(v, a, b);
+    return lanes >= 64 ? a + b : v;
+}
 
-// One workgroup a sequence adds up the rows of its parts, every expert's in the order of the parts (shared out among groups of threads).
-__global__ void __launch_bounds__(kFinishThreads) balance_finish_kernel(int64_t sequences, int experts, int parts, int width,  // a power of two, at most 1024
-                                                                        const float* __restrict__ part_shares, const int* __restrict__ part_counts,
-                                                                        float* __restrict__ loss, int64_t* __restrict__ counts,
-                                                                        int64_t* __restrict__ tokens) {
-    __shared__ float shares[kMostExperts];
-    __shared__ int chosen[kMostExperts];
-    __shared__ float group_shares[kFinishThreads];
-    __shared__ int group_counts[kFinishThreads];
-    __shared__ float place[kFinishThreads / kWave];
-    __shared__ int live_tokens;
-    const int64_t sequence = workgroup_number();
-    if (sequence >= sequences)
+// A sequence's rows are added up by 2^slice_bits workgroups, each for its part of the experts: four columns a thread, the rows shared out
+// among neighbouring threads, whose sums are then added in a fixed order.  Each leaves its part of sum c_e * share_e and of C; the one that
+// arrives last adds those up, in their order as well.  (Several slices only for one sequence: rows are many then.)  A chain of latencies
+// (offsets, rows, the slices' arrival), not of bytes.
+constexpr int kMostSlices = 16, kRowsAtOnce = 8;
+__global__ void __launch_bounds__(kBlockThreads) balance_finish_kernel(const Balance a, int width,  // columns of a row's half: 8 to 4096
+                                                                       int slice_bits, const u32x4* __restrict__ rows,
+                                                                       const int* __restrict__ live_of_rows, int* __restrict__ arrived,
+                                                                       uint64_t* __restrict__ parts_of_loss,  // [slices]: sum's bits, C's above them
+                                                                       float* __restrict__ loss, int64_t* __restrict__ counts,
+                                                                       int64_t* __restrict__ tokens) {
+    __shared__ float place[kWavesPerBlock][2];
+    __shared__ int live_place[kWavesPerBlock];
+    const int64_t sequence = workgroup_number() >> slice_bits;
+    const int slices = 1 << slice_bits, slice = static_cast<int>(workgroup_number()) & (slices - 1);
+    if (sequence >= a.sequences)
         return;
-    const int groups = kFinishThreads / width, group = threadIdx.x / width, column = threadIdx.x % width;
-    const int64_t first = sequence * parts;
-    if (threadIdx.x == 0)
-        live_tokens = 0;
-    __syncthreads();
-    for (int base = 0; base < experts; base += width) {
-        const int e = base + column;
-        float share = 0.0f;
-        int count = 0;
-        if (e < experts)
-#pragma unroll 8
-            for (int part = group; part < parts; part += groups) {
-                share += part_shares[(first + part) * experts + e];
-                count += part_counts[(first + part) * (experts + 1) + e];
-            }
-        group_shares[threadIdx.x] = share;
-        group_counts[threadIdx.x] = count;
-        __syncthreads();
-        if (group == 0 && e < experts) {
-            for (int other = 1; other < groups; ++other) {
-                share += group_shares[other * width + column];
-                count += group_counts[other * width + column];
-            }
-            shares[e] = share;
-            chosen[e] = count;
-        }
-        __syncthreads();
-    }
+    int64_t from = 0, to = a.tokens;
+    clip(a, sequence, from, to);
+    const int64_t first = (from >> a.chunk_bits) + sequence, end = to > from ? ((to - 1) >> a.chunk_bits) + sequence + 1 : first;
     int live = 0;
-    for (int part = threadIdx.x; part < parts; part += kFinishThreads)
-        live += part_counts[(first + part) * (experts + 1) + experts];
-    if (live > 0)
-        atomicAdd(&live_tokens, live);
+    for (int64_t row = first + threadIdx.x; row < end; row += kBlockThreads)
+        live += live_of_rows[row];
+    const int quads = width / 4 >> slice_bits;  // of this slice's columns
+    const int groups = quads >= kBlockThreads ? 1 : kBlockThreads / quads > kWave ? kWave : kBlockThreads / quads;
+    const int group = threadIdx.x & (groups - 1);
+    float sum = 0.0f, number = 0.0f;
+    for (int quad = threadIdx.x / groups; quad < quads; quad += kBlockThreads) {
+        const int at = slice * quads + quad;
+        float share[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        u32x4 count = {0u, 0u, 0u, 0u};
+        for (int64_t base = first + group; base < end; base += kRowsAtOnce * groups) {
+            u32x4 other[kRowsAtOnce], more[kRowsAtOnce];
+#pragma unroll
+            for (int r = 0; r < kRowsAtOnce; ++r) {
+                const int64_t row = base + r * groups < end ? base + r * groups : base;
+                other[r] = rows[row * (width / 2) + at];
+                more[r] = rows[row * (width / 2) + width / 4 + at];
+            }
+#pragma unroll
+            for (int r = 0; r < kRowsAtOnce; ++r)
+                if (base + r * groups < end) {
+                    count += more[r];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        share[i] += __uint_as_float(other[r][i]);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            share[i] = sum_of_lanes(share[i], groups);
+            count[i] = sum_of_lanes(count[i], groups);
+            if (group == 0 && at * 4 + i < a.experts) {
+                counts[sequence * a.experts + at * 4 + i] = count[i];
+                sum = fmaf(static_cast<float>(count[i]), share[i], sum);
+                number += static_cast<float>(count[i]);
+            }
+        }
+    }
+    sum = lanes_sum<kWave>(sum);
+    number = lanes_sum<kWave>(number);
+    live = static_cast<int>(sum_of_lanes(static_cast<uint32_t>(live), kWave));
+    if (threadIdx.x % kWave == 0) {
+        place[threadIdx.x / kWave][0] = sum;
+        place[threadIdx.x / kWave][1] = number;
+        live_place[threadIdx.x / kWave] = live;
+    }
     __syncthreads();
-    finish_sequence(sequence, experts, shares, chosen, live_tokens, loss, counts, tokens, place);
+    if (threadIdx.x > 0)
+        return;
+    sum = number = 0.0f;
+    live = 0;
+    for (int w = 0; w < kWavesPerBlock; ++w) {
+        sum += place[w][0];
+        number += place[w][1];
+        live += live_place[w];
+    }
+    if (slices > 1) {
+        // The exchange has been done where every workgroup sees it when it comes back; only then is this slice counted.
+        const uint64_t both = static_cast<uint64_t>(__float_as_uint(number)) << 32 | __float_as_uint(sum);
+        const uint64_t old = __hip_atomic_exchange(parts_of_loss + slice, both, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        int one = 1;
+        asm volatile("" : "+v"(one) : "v"(old) : "memory");
+        if (__hip_atomic_fetch_add(arrived, one, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != slices - 1)
+            return;
+        uint64_t all[kMostSlices];
+#pragma unroll
+        for (int other = 0; other < kMostSlices; ++other)
+            all[other] = other < slices ? __hip_atomic_load(parts_of_loss + other, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+        sum = number = 0.0f;
+#pragma unroll
+        for (int other = 0; other < kMostSlices; ++other) {
+            sum += __uint_as_float(static_cast<uint32_t>(all[other]));
+            number += __uint_as_float(static_cast<uint32_t>(all[other] >> 32));
+        }
+    }
+    tokens[sequence] = live;
+    loss[sequence] = loss_of(a.experts, sum, number, live);
 }
 
 // The gradient: with F_e = g E c_e / (C T') of the token's sequence, p_e (F_e - sum of F p) (times 1 - s_e for sigmoids); zero for
-// tokens without a choice and for those of no sequence, which the workgroups behind the last sequence's clear.
+// tokens without a choice and for those of no sequence.  A wavefront has a chunk of tokens, whatever sequences they are of; the next
+// tokens' inputs are on their way.
 template <int kLanes, int kEach>
 __global__ void __launch_bounds__(kBlockThreads) balance_loss_backward_kernel(const Balance a, const float* __restrict__ grad,  // [S]
                                                                               const int64_t* __restrict__ counts, const int64_t* __restrict__ tokens,
                                                                               void* __restrict__ grad_logits) {
-    constexpr int kTokens = kBlockThreads / kLanes;
-    const int64_t block = workgroup_number();
-    const int64_t sequence = block / a.parts;
-    const int part = static_cast<int>(block - sequence * a.parts);
-    const int lane = threadIdx.x % kLanes, place = threadIdx.x / kLanes;
-    float factor[kEach], out[kEach];
-    if (sequence >= a.sequences) {
-        if (sequence > a.sequences || a.offsets == nullptr)
-            return;
-        const int64_t begin = a.offsets[0], end = a.offsets[a.sequences];
-#pragma unroll
-        for (int i = 0; i < kEach; ++i)
-            out[i] = 0.0f;
-        for (int64_t token = static_cast<int64_t>(part) * kTokens + place; token < a.tokens; token += static_cast<int64_t>(a.parts) * kTokens)
-            store_spread<kLanes, kEach>(grad_logits, a.logits.wide, token, token < begin || token >= end, a.experts, out);
+    constexpr int kTokens = kWave / kLanes;
+    const int64_t begin = (workgroup_number() * kWavesPerBlock + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave)) << a.chunk_bits;
+    const int64_t length = int64_t{1} << a.chunk_bits;
+    if (begin >= a.tokens)
         return;
-    }
-    int64_t from, to;
-    part_of(a, sequence, part, from, to);
-    if (from >= to)
-        return;
-    float number = 0.0f;
+    const int64_t end = begin + length < a.tokens ? begin + length : a.tokens;
+    const int lane = threadIdx.x % kLanes, group = threadIdx.x % kWave / kLanes;
+    for (int64_t sequence = sequences_ahead(a, begin); sequence < a.sequences; ++sequence) {
+        int64_t from = begin, to = end;
+        clip(a, sequence, from, to);
+        if (from >= end)
+            break;
+        BalanceToken<kEach> next;
+        load_token<kLanes, kEach>(a, from + group, from + group < to, next);
+        float factor[kEach], number = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        const int expert = i * kLanes + lane;
-        factor[i] = expert < a.experts ? static_cast<float>(counts[sequence * a.experts + expert]) : 0.0f;
-        number += factor[i];
-    }
-    number = lanes_sum<kLanes>(number);
-    const int64_t live_tokens = tokens[sequence];
-    const float each = live_tokens > 0 && number > 0.0f ? grad[sequence] * static_cast<float>(a.experts) / number / static_cast<float>(live_tokens) : 0.0f;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i)
-        factor[i] *= each;
-    for (int64_t first = from; first < to; first += kTokens) {
-        const int64_t token = first + place;
-        const bool here = token < to;
-        float logit[kEach], share[kEach], rest[kEach], along = 0.0f;
-        load_spread<kLanes, kEach>(a.logits, token, here, a.experts, logit);
-        const bool live = has_choice<kLanes>(a, token, here, [](int) {});
-        shares_of<kLanes, kEach>(logit, a.sigmoid, share, rest);
+        for (int i = 0; i < kEach; ++i) {
+            const int expert = i * kLanes + lane;
+            const float count = static_cast<float>(counts[sequence * a.experts + (expert < a.experts ? expert : 0)]);
+            factor[i] = expert < a.experts ? count : 0.0f;
+            number += factor[i];
+        }
+        number = lanes_sum<kLanes>(number);
+        const int64_t live_tokens = tokens[sequence];
+        const float each =
+            live_tokens > 0 && number > 0.0f ? grad[sequence] * static_cast<float>(a.experts) / number / static_cast<float>(live_tokens) : 0.0f;
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
-            along = fmaf(factor[i], share[i], along);
-        along = lanes_sum<kLanes>(along);
+            factor[i] *= each;
+        for (int64_t first = from; first < to; first += kTokens) {
+            const BalanceToken<kEach> token = next;
+            load_token<kLanes, kEach>(a, first + kTokens + group, first + kTokens + group < to, next);
+            const bool live = lanes_where<kLanes>(token.named >= 0 && token.named < a.experts) != 0;
+            float share[kEach], rest[kEach], out[kEach], along = 0.0f;
+            shares_of<kLanes, kEach>(token.logit, a.sigmoid, share, rest);
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+                along = fmaf(factor[i], share[i], along);
+            along = lanes_sum<kLanes>(along);
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+                out[i] = live ? share[i] * rest[i] * (factor[i] - along) : 0.0f;
+            store_spread<kLanes, kEach>(grad_logits, a.logits.wide, first + group, token.here, a.experts, out);
+        }
+    }
+    if (a.offsets != nullptr) {
+        const int64_t behind = a.offsets[a.sequences], ahead = a.offsets[0];
+        float zero[kEach];
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
-            out[i] = live ? share[i] * rest[i] * (factor[i] - along) : 0.0f;
-        store_spread<kLanes, kEach>(grad_logits, a.logits.wide, token, here, a.experts, out);
+            zero[i] = 0.0f;
+        if (begin < ahead || end > behind)
+            for (int64_t token = begin + group; token < end; token += kTokens)
+                store_spread<kLanes, kEach>(grad_logits, a.logits.wide, token, token < ahead || token >= behind, a.experts, zero);
     }
 }
 
@@ -971,7 +1071,7 @@ Spread spread_for_choices(int64_t num_tokens, int experts, int needed) {
     return spread_of(experts, std::max(needed, num_tokens <= int64_t{32} * current_topology(current_tuning()).cus ? 32 : 1));
 }
 
-// CALL(lanes, experts a lane) for a Spread of 8 lanes or more, of 16 or more, and of whatever number suits the experts.
+// CALL(lanes, experts a lane) for a Spread of 8 lanes or more, and of 16 or more.
 #define NANOEP_BY_SPREAD(SPREAD, CALL)              \
     switch ((SPREAD).lanes * 100 + (SPREAD).each) { \
         case 801:                                   \
@@ -1089,40 +1189,6 @@ Spread spread_for_choices(int64_t num_tokens, int experts, int needed) {
             CALL(64, 64);                           \
             break;                                  \
     }
-#define NANOEP_BY_FREE_SPREAD(SPREAD, CALL)         \
-    switch ((SPREAD).lanes * 100 + (SPREAD).each) { \
-        case 801:                                   \
-            CALL(8, 1);                             \
-            break;                                  \
-        case 802:                                   \
-            CALL(8, 2);                             \
-            break;                                  \
-        case 804:                                   \
-            CALL(8, 4);                             \
-            break;                                  \
-        case 1604:                                  \
-            CALL(16, 4);                            \
-            break;                                  \
-        case 1608:                                  \
-            CALL(16, 8);                            \
-            break;                                  \
-        case 1616:                                  \
-            CALL(16, 16);                           \
-            break;                                  \
-        case 3216:                                  \
-            CALL(32, 16);                           \
-            break;                                  \
-        case 6416:                                  \
-            CALL(64, 16);                           \
-            break;                                  \
-        case 6432:                                  \
-            CALL(64, 32);                           \
-            break;                                  \
-        default:                                    \
-            CALL(64, 64);                           \
-            break;                                  \
-    }
-
 bool router_sizes_fit(int64_t stride, int logits_type, int64_t num_tokens, int experts, int topk, int scoring) {
     return num_tokens >= 0 && num_tokens <= 0x7fffffff / kMaxTopk && experts >= 1 && experts <= kMostExperts && topk >= 1 && topk <= kMaxTopk &&
            stride >= experts && stride <= int64_t{1} << 31 && (logits_type == NANOEP_BF16 || logits_type == NANOEP_FP32) &&
@@ -1131,12 +1197,37 @@ bool router_sizes_fit(int64_t stride, int logits_type, int64_t num_tokens, int e
 
 Logits logits_of(const void* data, int64_t stride, int type) { return {data, stride, type == NANOEP_FP32}; }
 
-// Parts of a sequence: one for every 64 tokens of an average one, at most 256 (balance_finish_kernel reads them all).
-constexpr int64_t kPartTokens = 64;
-constexpr int64_t kMostParts = 256;
-int parts_of(int64_t num_tokens, int64_t sequences) {
-    const int64_t average = (num_tokens + sequences - 1) / sequences;
-    return static_cast<int>(std::min(kMostParts, std::max<int64_t>(1, (average + kPartTokens - 1) / kPartTokens)));
+int bits_of(int64_t least) {
+    int bits = 0;
+    while ((int64_t{1} << bits) < least)
+        ++bits;
+    return bits;
+}
+
+// How the loss's tokens are dealt out: a workgroup has one round of tokens, more where that would be more than two workgroups a compute
+// unit, or a few rounds of one sequence, which then take one launch.  Each leaves rows of sums, which several workgroups add up for one
+// sequence, and one each for several.
+struct BalancePlan {
+    Spread spread;
+    int chunk_bits, slice_bits;
+    int64_t chunks, rows;  // rows of sums: 0 where none are needed
+};
+BalancePlan plan_balance(int64_t num_tokens, int experts, int topk, int64_t sequences) {
+    BalancePlan plan;
+    plan.spread = spread_of(experts, topk);
+    const int64_t round = kBlockThreads / plan.spread.lanes, most = int64_t{2} * current_topology(current_tuning()).cus;
+    plan.chunk_bits = bits_of(sequences == 1 && num_tokens <= 4 * round ? 4 * round : std::max(round, (num_tokens + most - 1) / most));
+    plan.chunks = (num_tokens + (int64_t{1} << plan.chunk_bits) - 1) >> plan.chunk_bits;
+    plan.rows = sequences == 1 && plan.chunks == 1 ? 0 : plan.chunks + sequences;
+    plan.slice_bits = 0;
+    while (sequences == 1 && (1 << plan.slice_bits) < kMostSlices && (1 << plan.slice_bits) < plan.spread.lanes * plan.spread.each / 4)
+        ++plan.slice_bits;
+    return plan;
+}
+// The slices' parts of the loss, rows, their numbers of tokens, the number of slices that are done.
+size_t balance_workspace(const BalancePlan& plan) {
+    const size_t row = 2 * static_cast<size_t>(plan.spread.lanes) * plan.spread.each * sizeof(uint32_t);
+    return plan.rows == 0 ? 0 : kMostSlices * sizeof(uint64_t) + static_cast<size_t>(plan.rows) * (row + sizeof(int)) + sizeof(int);
 }
 
 }  // namespace
@@ -1203,12 +1294,11 @@ int nanoep_route_topk_backward(const float* grad, const void* logits, int64_t lo
     return NANOEP_OK;
 }
 
-size_t nanoep_balance_loss_workspace_bytes(int64_t num_tokens, int num_experts, int64_t sequences) {
+size_t nanoep_balance_loss_workspace_bytes(int64_t num_tokens, int num_experts, int num_topk, int64_t sequences) {
     using namespace nanoep;
-    if (num_tokens < 0 || num_experts < 1 || num_experts > kMostExperts || sequences < 1 || sequences > 0x7fffffff)
+    if (!router_sizes_fit(num_experts, NANOEP_FP32, num_tokens, num_experts, num_topk, NANOEP_SOFTMAX) || sequences < 1 || sequences > 0x7fffffff)
         return 0;
-    const int parts = parts_of(num_tokens, sequences);
-    return parts == 1 ? 0 : static_cast<size_t>(sequences) * parts * (2 * static_cast<size_t>(num_experts) + 1) * sizeof(float);
+    return balance_workspace(plan_balance(num_tokens, num_experts, num_topk, sequences));
 }
 
 int nanoep_balance_loss(const void* logits, int64_t logits_stride, int logits_type, const int64_t* ids, const int64_t* sequence_offsets,
@@ -1220,29 +1310,35 @@ int nanoep_balance_loss(const void* logits, int64_t logits_stride, int logits_ty
         return NANOEP_ERR_INVALID_ARGUMENT;
     if (loss == nullptr || counts == nullptr || tokens == nullptr || (num_tokens > 0 && (logits == nullptr || ids == nullptr)))
         return NANOEP_ERR_INVALID_ARGUMENT;
-    if (workspace_bytes < nanoep_balance_loss_workspace_bytes(num_tokens, num_experts, sequences))
+    const BalancePlan plan = plan_balance(num_tokens, num_experts, num_topk, sequences);
+    if (workspace_bytes < balance_workspace(plan))
         return NANOEP_ERR_WORKSPACE;
-    const Balance arguments = {logits_of(logits, logits_stride, logits_type), ids, sequence_offsets, num_tokens, sequences, num_experts,
-                               num_topk, parts_of(num_tokens, sequences), scoring == NANOEP_SIGMOID};
-    if (arguments.parts > 1 && (workspace == nullptr || !aligned16(workspace)))
+    if (plan.rows > 0 && (workspace == nullptr || !aligned16(workspace)))
         return NANOEP_ERR_INVALID_ARGUMENT;
-    const Spread spread = spread_of(num_experts, 1);
-    const int64_t blocks = sequences * arguments.parts;
-    auto* part_shares = static_cast<float*>(workspace);
-    auto* part_counts = static_cast<int*>(workspace) + (arguments.parts > 1 ? blocks * num_experts : 0);
+    const Balance arguments = {logits_of(logits, logits_stride, logits_type), ids, sequence_offsets, num_tokens, sequences, plan.chunk_bits, num_experts,
+                               num_topk, scoring == NANOEP_SIGMOID};
+    const int width = plan.spread.lanes * plan.spread.each;
+    uint64_t* parts_of_loss = nullptr;
+    uint32_t* rows = nullptr;
+    int *live_of_rows = nullptr, *arrived = nullptr;
+    if (plan.rows > 0) {
+        parts_of_loss = static_cast<uint64_t*>(workspace);
+        rows = reinterpret_cast<uint32_t*>(parts_of_loss + kMostSlices);
+        live_of_rows = reinterpret_cast<int*>(rows + plan.rows * 2 * width);
+        arrived = live_of_rows + plan.rows;
+    }
     const auto on = static_cast<hipStream_t>(stream);
-#define NANOEP_LAUNCH_BALANCE(LANES, EACH)                                                                                        \
-    balance_loss_kernel<LANES, EACH><<<grid_of(blocks), balance_waves(EACH) * kWave, 0, on>>>(arguments, part_shares, part_counts, loss, \
-                                                                                             counts, tokens)
-    NANOEP_BY_FREE_SPREAD(spread, NANOEP_LAUNCH_BALANCE)
+    if (plan.chunks > 0) {
+#define NANOEP_LAUNCH_BALANCE(LANES, EACH)                                                                                                   \
+    balance_loss_kernel<LANES, EACH><<<grid_of(plan.chunks), kBlockThreads, 0, on>>>(arguments, rows, live_of_rows, arrived, loss, counts, tokens)
+        NANOEP_BY_SPREAD(plan.spread, NANOEP_LAUNCH_BALANCE)
 #undef NANOEP_LAUNCH_BALANCE
-    NANOEP_HIP_TRY(hipGetLastError());
-    if (arguments.parts > 1) {
-        int width = kWave;
-        while (width < num_experts && width < kFinishThreads)
-            width *= 2;
-        balance_finish_kernel<<<grid_of(sequences), kFinishThreads, 0, on>>>(sequences, num_experts, arguments.parts, width, part_shares, part_counts,
-                                                                           loss, counts, tokens);
+        NANOEP_HIP_TRY(hipGetLastError());
+    }
+    if (plan.rows > 0) {
+        const int slice_bits = plan.chunks > 0 ? plan.slice_bits : 0;  // (without tokens nobody cleared the number of those done)
+        balance_finish_kernel<<<grid_of(sequences << slice_bits), kBlockThreads, 0, on>>>(arguments, width, slice_bits, reinterpret_cast<const u32x4*>(rows),
+                                                                                   live_of_rows, arrived, parts_of_loss, loss, counts, tokens);
         NANOEP_HIP_TRY(hipGetLastError());
     }
     return NANOEP_OK;
@@ -1259,17 +1355,17 @@ int nanoep_balance_loss_backward(const float* grad, const void* logits, int64_t 
         return NANOEP_OK;
     if (grad == nullptr || logits == nullptr || ids == nullptr || counts == nullptr || tokens == nullptr || grad_logits == nullptr)
         return NANOEP_ERR_INVALID_ARGUMENT;
-    Balance arguments = {logits_of(logits, logits_stride, logits_type), ids, sequence_offsets, num_tokens, sequences, num_experts,
-                         num_topk, 1, scoring == NANOEP_SIGMOID};
-    // two rounds of tokens a workgroup
-    const Spread spread = spread_of(num_experts, 1);
-    const int64_t average = (num_tokens + sequences - 1) / sequences, each = 2 * kBlockThreads / spread.lanes;
-    arguments.parts = static_cast<int>(std::min<int64_t>(4096, (average + each - 1) / each));
-    const int64_t blocks = (sequences + (sequence_offsets != nullptr ? 1 : 0)) * arguments.parts;
+    // a wavefront one round of tokens, more where that would be more than 16 wavefronts a compute unit
+    const Spread spread = spread_of(num_experts, num_topk);
+    const int64_t held = int64_t{16} * current_topology(current_tuning()).cus;
+    const int chunk_bits = bits_of(std::max<int64_t>(kWave / spread.lanes, (num_tokens + held - 1) / held));
+    const Balance arguments = {logits_of(logits, logits_stride, logits_type), ids, sequence_offsets, num_tokens, sequences, chunk_bits, num_experts, num_topk,
+                               scoring == NANOEP_SIGMOID};
+    const int64_t chunks = (num_tokens + (int64_t{1} << chunk_bits) - 1) >> chunk_bits, blocks = (chunks + kWavesPerBlock - 1) / kWavesPerBlock;
     const auto on = static_cast<hipStream_t>(stream);
 #define NANOEP_LAUNCH_BALANCE_BACKWARD(LANES, EACH) \
     balance_loss_backward_kernel<LANES, EACH><<<grid_of(blocks), kBlockThreads, 0, on>>>(arguments, grad, counts, tokens, grad_logits)
-    NANOEP_BY_FREE_SPREAD(spread, NANOEP_LAUNCH_BALANCE_BACKWARD)
+    NANOEP_BY_SPREAD(spread, NANOEP_LAUNCH_BALANCE_BACKWARD)
 #undef NANOEP_LAUNCH_BALANCE_BACKWARD
     NANOEP_HIP_TRY(hipGetLastError());
     return NANOEP_OK;

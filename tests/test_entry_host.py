@@ -25,7 +25,7 @@ def library():
     lib.nanoep_route_topk.argtypes = [p, i64, i, p, p, i64, i, i, i, i, i, i, f, p, p, p]
     lib.nanoep_route_topk_backward.argtypes = [p, p, i64, i, p, i64, i, i, i, i, f, p, p]
     lib.nanoep_balance_loss_workspace_bytes.restype = sz
-    lib.nanoep_balance_loss_workspace_bytes.argtypes = [i64, i, i64]
+    lib.nanoep_balance_loss_workspace_bytes.argtypes = [i64, i, i, i64]
     lib.nanoep_balance_loss.argtypes = [p, i64, i, p, p, i64, i, i, i64, i, p, p, p, p, sz, p]
     lib.nanoep_balance_loss_backward.argtypes = [p, p, i64, i, p, p, p, p, i64, i, i, i64, i, p, p]
     return lib
@@ -96,8 +96,8 @@ def test_balance_losses_are_refused_before_any_device_work():
     for wrong in ({"stride": 63}, {"kind": 2}, {"tokens": -1}, {"tokens": 1 << 26}, {"experts": 0}, {"experts": 4097, "stride": 5000}, {"topk": 0}, {"topk": 33},
                   {"scoring": 2}, {"ids": null}, {"sequences": 0}, {"sequences": 2}, {"sequences": 1 << 31, "offsets": 64}, {"loss": null}):
         assert lost(**wrong) == BAD and returned(**wrong) == BAD, wrong
-    needed = lib.nanoep_balance_loss_workspace_bytes(100_000, 64, 1)
-    assert needed > 0 and lib.nanoep_balance_loss_workspace_bytes(10, 64, 1) == 0 and lib.nanoep_balance_loss_workspace_bytes(10, 0, 1) == 0
+    needed = lib.nanoep_balance_loss_workspace_bytes(100_000, 64, 8, 1)
+    assert needed > 0 and lib.nanoep_balance_loss_workspace_bytes(10, 64, 8, 1) == 0 and lib.nanoep_balance_loss_workspace_bytes(10, 0, 8, 1) == 0
     assert lost(tokens=100_000, workspace=64, size=needed - 1) == NO_WORKSPACE
     assert lost(tokens=100_000, workspace=null, size=needed) == BAD and lost(tokens=100_000, workspace=72, size=needed) == BAD
 
