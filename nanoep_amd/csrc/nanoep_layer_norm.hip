@@ -9,6 +9,7 @@
 // All of it in fp32, every output rounded once.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "nanoep_lanes.h"
 #include "nanoep_operators.h"
@@ -20,6 +21,8 @@ constexpr int kMostThreads = 1024;
 constexpr int kBackwardThreads = 512;  // two wavefronts a SIMD: 256 registers a lane
 constexpr int kMostRowWaves = kMostThreads / kWave;
 constexpr int kMostHidden = 16384;
+constexpr int kWaitForLoads = 0x0f70;    // an operand of s_waitcnt: no vector memory access is left
+constexpr int kRawBuffer = 0x00020000;  // the last word of a buffer of plain 32-bit data
 
 struct Bf16 {};  // two bytes a value
 struct Fp32 {};
@@ -65,6 +68,18 @@ struct HeldParameters {
         }
     }
 };
+
+// A store to the row's vector `at`, dropped where that is behind its `size` bytes, without a branch around it: where a store may be
+// skipped, a wait for the loads ahead of it is a wait for it as well, since both are counted together, in their order.
+template <bool kNonTemporal, class V>
+__device__ __forceinline__ void store_within(void* row, int size, int at, const V v) {
+    const __amdgpu_buffer_rsrc_t within = __builtin_amdgcn_make_buffer_rsrc(row, 0, size, kRawBuffer);
+    constexpr int kCache = kNonTemporal ? 2 : 0;
+    if constexpr (sizeof(V) == 16)
+        __builtin_amdgcn_raw_buffer_store_b128(v, within, at * 16, 0, kCache);
+    else
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), within, at * 4, 0, kCache);
+}
 
 // What the wavefronts of a row left in LDS, one in each of 16 neighbouring lanes; nothing behind the last.
 __device__ __forceinline__ float2 of_wavefront(const float2* places, int waves) {
@@ -145,9 +160,12 @@ __global__ void __launch_bounds__(kMostThreads) layer_norm_kernel(const u32x4* _
             shifts[v].load(beta, place[v]);
     }
     int turn = 0;
+    __builtin_amdgcn_s_waitcnt(kWaitForLoads);  // (in the loop, a wait that suits the first row as well would be one for the last row's stores)
     for (int64_t first = group * teams; first < rows; first += apart, turn ^= 1) {
         const int64_t row = first + team;
         const bool here = row < rows;
+        const int64_t base = here ? row * vectors : 0;
+        const int size = here ? vectors * 16 : 0;
         float s[kVectors][kColumns];
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
@@ -159,13 +177,11 @@ __global__ void __launch_bounds__(kMostThreads) layer_norm_kernel(const u32x4* _
                 for (int i = 0; i < kColumns; ++i)
                     s[v][i] += added[i];
                 const u32x4 packed = Row::pack(s[v]);
-                if (here && in_row[v])
-                    store_vec<!kPastCache>(total + row * vectors + place[v], packed);
+                store_within<!kPastCache>(total + base, size, threadIdx.x + v * blockDim.x, packed);
                 Row::unpack(packed, s[v]);
             }
         }
-        if (first + apart < rows)
-            load(row + apart);
+        load(row + apart);
         float mean = 0.0f, squares = 0.0f;
         if (centred) {
 #pragma unroll
@@ -200,13 +216,9 @@ __global__ void __launch_bounds__(kMostThreads) layer_norm_kernel(const u32x4* _
             squares = lanes_sum<kMostRowWaves>(squares);
         }
         const float rstd = rsqrtf(fmaf(squares, per_column, eps));
-        if (!here)
-            continue;
-        if (threadIdx.x == 0) {
-            rstds[row] = rstd;
-            if (centred)
-                means[row] = mean;
-        }
+        store_within<false>(rstds + (here ? row : 0), here ? 4 : 0, threadIdx.x, rstd);
+        if (centred)
+            store_within<false>(means + (here ? row : 0), here ? 4 : 0, threadIdx.x, mean);
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
             float factor[kColumns];
@@ -221,8 +233,7 @@ __global__ void __launch_bounds__(kMostThreads) layer_norm_kernel(const u32x4* _
                 for (int i = 0; i < kColumns; ++i)
                     s[v][i] += shift[i];
             }
-            if (in_row[v])
-                store_vec<!kPastCache>(normalized + row * vectors + place[v], Row::pack(s[v]));
+            store_within<!kPastCache>(normalized + base, size, threadIdx.x + v * blockDim.x, Row::pack(s[v]));
         }
     }
 }
@@ -232,14 +243,14 @@ __global__ void __launch_bounds__(kMostThreads) layer_norm_kernel(const u32x4* _
 // ([workgroups][2][columns] fp32), which parameter_gradient_kernel adds up in a fixed order.  No atomics.
 // With d = s - mean, along = sum(u * d): dx = r * u - r * mean(u) - d * r^3 * along / H.  d and u stay in registers between a row's sums
 // and its output; the next row's inputs are on their way meanwhile.
-template <class T, class P, int kVectors>
+template <class T, class P, int kVectors, bool kAdded, bool kInput>
 __global__ void __launch_bounds__(kBackwardThreads) layer_norm_backward_kernel(const u32x4* __restrict__ grad,   // [T][vectors]
                                                                                const u32x4* __restrict__ total,  // [T][vectors]
                                                                                const u32x4* __restrict__ gamma,
                                                                                const float* __restrict__ means,  // null: the root-mean-square norm
                                                                                const float* __restrict__ rstds,
-                                                                               const u32x4* __restrict__ grad_residual,  // [T][vectors] or null
-                                                                               u32x4* __restrict__ grad_x,               // [T][vectors] or null
+                                                                               const u32x4* __restrict__ grad_residual,  // [T][vectors], if kAdded
+                                                                               u32x4* __restrict__ grad_x,               // [T][vectors], if kInput
                                                                                float* __restrict__ sums,                 // null: not wanted
                                                                                int64_t rows,
                                                                                int64_t groups,
@@ -283,7 +294,7 @@ __global__ void __launch_bounds__(kBackwardThreads) layer_norm_backward_kernel(c
             in.total[v] = row_total[place[v]];
             in.grad[v] = row_grad[place[v]];
         }
-        if (grad_residual != nullptr) {
+        if (kAdded) {
             const u32x4* row_added = grad_residual + row * vectors;
 #pragma unroll
             for (int v = 0; v < kVectors; ++v)
@@ -295,6 +306,7 @@ __global__ void __launch_bounds__(kBackwardThreads) layer_norm_backward_kernel(c
     const int64_t apart = groups * teams;
     load(group * teams + team, next);
     int turn = 0;
+    __builtin_amdgcn_s_waitcnt(kWaitForLoads);  // (in the loop, a wait that suits the first row as well would be one for the last row's stores)
     for (int64_t first = group * teams; first < rows; first += apart, turn ^= 1) {
         const int64_t row = first + team;
         const bool here = row < rows;
@@ -307,7 +319,8 @@ __global__ void __launch_bounds__(kBackwardThreads) layer_norm_backward_kernel(c
             Row::unpack(next.total[v], d[v]);
             Row::unpack(next.grad[v], u[v]);
             held[v].unpack(factor);
-            added[v] = next.added[v];
+            if (kAdded)
+                added[v] = next.added[v];
             if (here && in_row[v]) {
 #pragma unroll
                 for (int i = 0; i < kColumns; ++i) {
@@ -322,7 +335,7 @@ __global__ void __launch_bounds__(kBackwardThreads) layer_norm_backward_kernel(c
             }
         }
         load(row + apart, next);
-        if (grad_x != nullptr) {
+        if (kInput) {
             both[0] = lanes_sum<kWave>(both[0]);
             both[1] = lanes_sum<kWave>(both[1]);
             if (waves > 1) {
@@ -339,15 +352,14 @@ __global__ void __launch_bounds__(kBackwardThreads) layer_norm_backward_kernel(c
 #pragma unroll
                 for (int i = 0; i < kColumns; ++i)
                     u[v][i] = fmaf(u[v][i], rstd, fmaf(d[v][i], along, across));
-                if (grad_residual != nullptr) {
+                if (kAdded) {
                     float more[kColumns];
                     Row::unpack(added[v], more);
 #pragma unroll
                     for (int i = 0; i < kColumns; ++i)
                         u[v][i] += more[i];
                 }
-                if (here && in_row[v])
-                    store_vec<true>(grad_x + row * vectors + place[v], Row::pack(u[v]));
+                store_within<true>(grad_x + (here ? row * vectors : 0), here ? vectors * 16 : 0, threadIdx.x + v * blockDim.x, Row::pack(u[v]));
             }
         }
     }
@@ -391,45 +403,50 @@ __global__ void __launch_bounds__(kBackwardThreads) layer_norm_backward_kernel(c
     }
 }
 
-// dgamma and dbeta from the workgroups' sums: 64 columns a workgroup, its 64 groups of 16 lanes share out the rows of sums.
-constexpr int kSumLanes = 16, kSumGroups = 64;
+// dgamma and dbeta from the workgroups' sums: 64 columns a workgroup, its 16 groups of 16 lanes share out the rows of sums, all loads of
+// 16 rows on their way at once; then a thread a column adds up the groups'.
+constexpr int kSumLanes = 16, kSumGroups = 16, kSumRows = 16;
 template <class P>
 __global__ void __launch_bounds__(kSumLanes * kSumGroups) parameter_gradient_kernel(const u32x4* __restrict__ sums,  // [groups][2][columns / 4]
                                                                                     void* __restrict__ grad_gamma,
                                                                                     void* __restrict__ grad_beta,
                                                                                     int64_t groups,
                                                                                     int quads) {
-    __shared__ float parts[kSumGroups][kSumLanes][4];
+    __shared__ float parts[kSumGroups][kSumLanes * 4];
     const int lane = threadIdx.x % kSumLanes, part = threadIdx.x / kSumLanes;
-    const int at = blockIdx.x * kSumLanes + lane;
+    const int at = blockIdx.x * kSumLanes + lane, from = at < quads ? at : 0;
     const int which = blockIdx.y;
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (at < quads) {
-#pragma unroll 4
-        for (int64_t group = part; group < groups; group += kSumGroups) {
-            const u32x4 data = sums[(2 * group + which) * quads + at];
+    for (int64_t base = part; base < groups; base += kSumGroups * kSumRows) {
+        u32x4 data[kSumRows];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                sum[i] += __uint_as_float(data[i]);
+        for (int r = 0; r < kSumRows; ++r) {
+            const int64_t group = base + r * kSumGroups;
+            data[r] = sums[(2 * (group < groups ? group : base) + which) * quads + from];
         }
+#pragma unroll
+        for (int r = 0; r < kSumRows; ++r)
+            if (base + r * kSumGroups < groups)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    sum[i] += __uint_as_float(data[r][i]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        parts[part][lane][i] = sum[i];
-    for (int half = kSumGroups / 2; half > 0; half /= 2) {
-        __syncthreads();
-        if (part < half)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                parts[part][lane][i] = sum[i] += parts[part + half][lane][i];
-    }
-    if (part > 0 || at >= quads)
+        parts[part][lane * 4 + i] = sum[i];
+    __syncthreads();
+    const int column = blockIdx.x * kSumLanes * 4 + threadIdx.x;
+    if (threadIdx.x >= kSumLanes * 4 || column >= quads * 4)
         return;
+    float all = 0.0f;
+#pragma unroll
+    for (int other = 0; other < kSumGroups; ++other)
+        all += parts[other][threadIdx.x];
     void* out = which == 0 ? grad_gamma : grad_beta;
     if constexpr (RowType<P>::kColumns == 8)
-        static_cast<uint2*>(out)[at] = make_uint2(to_bf16_pair(sum[0], sum[1]), to_bf16_pair(sum[2], sum[3]));
+        static_cast<uint16_t*>(out)[column] = static_cast<uint16_t>(to_bf16_pair(all, 0.0f));
     else
-        static_cast<u32x4*>(out)[at] = RowType<Fp32>::pack(sum);
+        static_cast<float*>(out)[column] = all;
 }
 
 // Lanes and vectors a lane for rows of `vectors` vectors: two vectors a lane, more only where `most` lanes would not do.  By the
@@ -519,14 +536,23 @@ int launch_backward(const BackwardPlan& plan, const void* grad, const void* tota
                                                  static_cast<u32x4*>(grad_x), grad_gamma != nullptr ? static_cast<float*>(workspace) : nullptr,
                                                  num_tokens, plan.groups, plan.vectors, static_cast<float>(hidden));
         };
+        const auto pick = [&](auto vectors_held) {
+            constexpr int kHeld = decltype(vectors_held)::value;
+            if (grad_x == nullptr)
+                launch(layer_norm_backward_kernel<T, P, kHeld, false, false>);
+            else if (grad_residual == nullptr)
+                launch(layer_norm_backward_kernel<T, P, kHeld, false, true>);
+            else
+                launch(layer_norm_backward_kernel<T, P, kHeld, true, true>);
+        };
         if (plan.shape.held == 1)
-            launch(layer_norm_backward_kernel<T, P, 1>);
+            pick(std::integral_constant<int, 1>{});
         else if (plan.shape.held == 2)
-            launch(layer_norm_backward_kernel<T, P, 2>);
+            pick(std::integral_constant<int, 2>{});
         else if (plan.shape.held == 4)
-            launch(layer_norm_backward_kernel<T, P, 4>);
+            pick(std::integral_constant<int, 4>{});
         else if constexpr (RowType<T>::kColumns == 4)
-            launch(layer_norm_backward_kernel<T, P, 8>);
+            pick(std::integral_constant<int, 8>{});
         NANOEP_HIP_TRY(hipGetLastError());
     }
     if (grad_gamma != nullptr) {
