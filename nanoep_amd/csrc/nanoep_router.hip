@@ -717,15 +717,21 @@ __device__ __forceinline__ void clip(const Balance& a, int64_t sequence, int64_t
     to = end < to ? end : to;
 }
 
-// The sequences that end at or ahead of a token, counted by the threads of a wavefront: the first that can have it.
+// The sequences that end at or ahead of a token, and so the first that can have it: a search with 64 probes at a time.
 __device__ __forceinline__ int64_t sequences_ahead(const Balance& a, int64_t token) {
-    int64_t ahead = 0;
-    if (a.offsets != nullptr)
-        for (int64_t base = 0; base < a.sequences; base += kWave) {
-            const int64_t sequence = base + threadIdx.x % kWave;
-            ahead += __popcll(__ballot(sequence < a.sequences && a.offsets[sequence + 1] <= token));
-        }
-    return ahead;
+    if (a.offsets == nullptr)
+        return 0;
+    int64_t low = 0, high = a.sequences;
+    while (low < high) {
+        const int64_t apart = (high - low + kWave - 1) / kWave, probe = low + threadIdx.x % kWave * apart;
+        const int ended = __popcll(__ballot(probe < high && a.offsets[probe + 1] <= token));
+        if (ended == 0)
+            return low;
+        const int64_t last = low + (ended - 1) * apart;
+        low = last + 1;
+        high = last + apart < high ? last + apart : high;
+    }
+    return low;
 }
 
 // A token of each group of kLanes lanes: its logits, and choice k in lane k.
@@ -1204,9 +1210,9 @@ int bits_of(int64_t least) {
     return bits;
 }
 
-// How the loss's tokens are dealt out: a workgroup has one round of tokens, more where that would be more than two workgroups a compute
-// unit, or a few rounds of one sequence, which then take one launch.  Each leaves rows of sums, which several workgroups add up for one
-// sequence, and one each for several.
+// How the loss's tokens are dealt out: a workgroup has one round of tokens, more (but no more than a sequence's) where that would be more
+// than two workgroups a compute unit, or a few rounds of one sequence, which then take one launch.  Each leaves rows of sums, which several
+// workgroups add up for one sequence, and one each for several.
 struct BalancePlan {
     Spread spread;
     int chunk_bits, slice_bits;
@@ -1216,7 +1222,8 @@ BalancePlan plan_balance(int64_t num_tokens, int experts, int topk, int64_t sequ
     BalancePlan plan;
     plan.spread = spread_of(experts, topk);
     const int64_t round = kBlockThreads / plan.spread.lanes, most = int64_t{2} * current_topology(current_tuning()).cus;
-    plan.chunk_bits = bits_of(sequences == 1 && num_tokens <= 4 * round ? 4 * round : std::max(round, (num_tokens + most - 1) / most));
+    const int64_t average = (num_tokens + sequences - 1) / sequences;
+    plan.chunk_bits = bits_of(sequences == 1 && num_tokens <= 4 * round ? 4 * round : std::max(round, std::min(average, (num_tokens + most - 1) / most)));
     plan.chunks = (num_tokens + (int64_t{1} << plan.chunk_bits) - 1) >> plan.chunk_bits;
     plan.rows = sequences == 1 && plan.chunks == 1 ? 0 : plan.chunks + sequences;
     plan.slice_bits = 0;
@@ -1355,7 +1362,8 @@ int nanoep_balance_loss_backward(const float* grad, const void* logits, int64_t 
         return NANOEP_OK;
     if (grad == nullptr || logits == nullptr || ids == nullptr || counts == nullptr || tokens == nullptr || grad_logits == nullptr)
         return NANOEP_ERR_INVALID_ARGUMENT;
-    // a wavefront one round of tokens, more where that would be more than 16 wavefronts a compute unit
+    // a wavefront one round of tokens, more where that would be more than 16 wavefronts a compute unit (us with 4, 8, 16, 32 of them: 32768
+    // tokens of 64 experts 9.0, 6.8, 6.7, 7.1; of 128, 64 sequences, 15.0, 11.6, 11.0, 12.6)
     const Spread spread = spread_of(num_experts, num_topk);
     const int64_t held = int64_t{16} * current_topology(current_tuning()).cus;
     const int chunk_bits = bits_of(std::max<int64_t>(kWave / spread.lanes, (num_tokens + held - 1) / held));

@@ -8,8 +8,9 @@ go through dispatch as bf16 rows of half the length; both products read them seg
 are applied on the way back, where the shared expert's output (here: the residual) is added.  Nothing is copied to the
 host between the steps.  The output is compared with a dense evaluation of the same 8-bit weights.
 
-Training: the rows go out and back through `dispatch_rows` and `combine_weighted`, whose gradients autograd finds; the experts in
-between are any differentiable function of the rows (here: one gain a channel).
+Training: the rows are normed and routed, go out and back through `dispatch_rows` and `combine_weighted`, and the loss that
+balances the experts is added; autograd finds the gradients of all of it.  The experts in between are any differentiable function of the
+rows (here: one gain a channel).
 """
 
 from __future__ import annotations
@@ -23,6 +24,8 @@ import nanoep_amd as ep
 
 # A product of 8-bit activations: each of them is off by at most 2^-4 of itself.
 TOLERANCE = 2.0**-4
+EPS = 1e-6
+BALANCE = 0.01  # the balance loss's part of the objective
 
 
 def make_layer(options, device):
@@ -44,9 +47,8 @@ def make_layer(options, device):
 
 def route(layer, normalized, topk):
     """Expert ids [T, K] and gate weights [T, K]."""
-    scores = torch.softmax(normalized.float() @ layer["router"].T, dim=1)
-    weights, ids = scores.topk(topk, dim=1)
-    return ids.contiguous(), (weights / weights.sum(dim=1, keepdim=True)).contiguous()
+    routing = ep.route_topk(normalized.float() @ layer["router"].T, topk)
+    return routing.ids, routing.weights
 
 
 def forward(buffer, layer, x, residual, options):
@@ -100,27 +102,35 @@ def train(options):
     generator = torch.Generator().manual_seed(3)
     shape = (options.tokens, options.hidden)
     x, grad = (torch.randn(*shape, generator=generator).to(torch.bfloat16).to(device) for _ in range(2))
-    x.requires_grad_()
-    gains = (1.0 + 0.1 * torch.randn(options.experts, options.hidden, generator=generator)).to(torch.bfloat16).to(device).requires_grad_()
-    logits = torch.randn(options.tokens, options.experts, generator=generator).to(device).requires_grad_()
-
-    def gates():
-        scores, ids = torch.softmax(logits, dim=1).topk(options.topk, dim=1)
-        return scores, ids.contiguous()
+    gains = (1.0 + 0.1 * torch.randn(options.experts, options.hidden, generator=generator)).to(torch.bfloat16).to(device)
+    logits = torch.randn(options.tokens, options.experts, generator=generator).to(device)
+    gamma = (1.0 + 0.1 * torch.randn(options.hidden, generator=generator)).to(device)
+    leaves = [tensor.requires_grad_() for tensor in (x, gamma, gains, logits)]
+    share = torch.full((), BALANCE, device=device)
 
     with ep.Buffer(None, ep.EPConfig(options.experts, options.topk, options.hidden, max(1, options.tokens))) as buffer:
-        weights, ids = gates()
-        handle = buffer.dispatch(x.detach(), topk_idx=ids, do_expand=True, alignment=options.alignment).handle
+        normed = ep.rms_norm(x, gamma, eps=EPS).normalized
+        routing = ep.route_topk(logits, options.topk, normalize=False)
+        handle = buffer.dispatch(normed.detach(), topk_idx=routing.ids, do_expand=True, alignment=options.alignment).handle
         layout = handle.layout
-        rows = ep.dispatch_rows(buffer, x, handle)
+        rows = ep.dispatch_rows(buffer, normed, handle)
         slot = torch.arange(rows.shape[0], device=device)
         expert = torch.searchsorted(layout.expert_offsets[1:].contiguous(), slot, right=True).clamp(max=options.experts - 1)
-        out = ep.combine_weighted(rows * gains[expert], handle.token_slots, weights, expert_offsets=layout.expert_offsets,
+        out = ep.combine_weighted(rows * gains[expert], handle.token_slots, routing.weights, expert_offsets=layout.expert_offsets,
                                   expert_counts=layout.expert_counts)
-        found = torch.autograd.grad(out, (x, gains, logits), grad)
-    weights, ids = gates()
-    dense_out = (x.float()[:, None] * gains.float()[ids] * weights[:, :, None]).sum(1)
-    for got, want in zip((out, *found), (dense_out, *torch.autograd.grad(dense_out, (x, gains, logits), grad.float()))):
+        balance = ep.balance_loss(logits, routing.ids)
+        found = torch.autograd.grad((out, balance.loss), leaves, (grad, share))
+
+    # the same in fp32, choice by choice at the source
+    wide = x.float()
+    wide = wide * torch.rsqrt(wide.square().mean(dim=1, keepdim=True) + EPS) * gamma
+    scores = torch.softmax(logits, dim=1)
+    dense_out = (wide[:, None] * gains.float()[routing.ids] * scores.gather(1, routing.ids)[:, :, None]).sum(1)
+    chosen = torch.bincount(routing.ids.reshape(-1), minlength=options.experts)
+    dense_balance = options.experts * (chosen / chosen.sum() * scores.mean(dim=0)).sum()
+    wanted = torch.autograd.grad((dense_out, dense_balance), leaves, (grad.float(), share))
+    assert torch.equal(balance.counts, chosen)
+    for got, want in zip((out, balance.loss, *found), (dense_out, dense_balance, *wanted)):
         assert (got.float() - want.float()).norm() <= TOLERANCE * want.float().norm()
 
 

@@ -251,6 +251,30 @@ def test_norm_gradients_that_arrive_in_other_layouts(device):
     assert same_bits(found, want)
 
 
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("tokens,hidden,rows,parameters,residual", [(8200, 8192, BF16, BF16, True), (7000, 8200, BF16, FP32, True), (30000, 1032, FP32, FP32, True),
+                                                                    (1600, 16384, FP32, FP32, True), (250000, 504, BF16, FP32, False)])
+def test_norm_of_more_rows_than_the_last_level_cache_holds(device, kind, tokens, hidden, rows, parameters, residual):
+    generator = torch.Generator(device=device).manual_seed(hidden)
+    x = (3 * torch.randn(tokens, hidden, device=device, generator=generator) + 0.3).to(rows)
+    other = torch.randn(tokens, hidden, device=device, generator=generator).to(rows) if residual else None
+    gamma = (1 + 0.2 * torch.randn(hidden, device=device, generator=generator)).to(parameters)
+    beta = (0.5 * torch.randn(hidden, device=device, generator=generator)).to(parameters) if kind == "layer" else None
+    print("norm, many rows", kind, tokens, hidden, rows, flush=True)
+    got = run_norm(kind, x, gamma, beta, other, 1e-5)
+    some = torch.cat([torch.arange(5), torch.arange(tokens // 2, tokens // 2 + 40), torch.arange(tokens - 19, tokens)])
+    s = oracle.total_of(x[some].cpu(), None if other is None else other[some].cpu())
+    if residual:
+        assert same_bits(got.residual[some].cpu(), s) and same_bits(got.residual, (x.float() + other.float()).to(rows))
+    y, mean, rstd = oracle.norm(s, gamma.cpu(), None if beta is None else beta.cpu(), 1e-5, kind == "layer")
+    oracle.check_rounded(got.normalized[some], *y, rows)
+    oracle.check_rounded(got.rstd[some], *rstd, FP32)
+    # all of them are what they are in a smaller batch
+    for at in range(0, tokens, 1000):
+        part = run_norm(kind, x[at : at + 1000], gamma, beta, None if other is None else other[at : at + 1000], 1e-5)
+        assert same_bits(got.normalized[at : at + 1000], part.normalized) and same_bits(got.rstd[at : at + 1000], part.rstd)
+
+
 def test_norm_rows_beyond_32_bit_offsets(device):
     tokens, hidden = 330_000, 7168
     gamma = torch.ones(hidden, dtype=BF16, device=device)
@@ -335,6 +359,32 @@ def test_ties_go_to_the_lowest_index(device, experts, biased):
                 check_route(device, logits.to(dtype), topk, scoring=scoring, bias=bias)
                 if experts % 4 == 0:
                     check_route(device, logits.to(dtype), min(topk, experts // 2), scoring=scoring, bias=bias, groups=4, topk_groups=2)
+
+
+@pytest.mark.parametrize("scoring", SCORINGS)
+def test_route_of_long_batches(device, scoring):
+    """More tokens than a device's wavefronts take one each of: fewer lanes a token."""
+    for experts, topk, groups, topk_groups in ((3, 2, 1, 1), (8, 6, 4, 3), (16, 3, 1, 1), (31, 12, 1, 1), (32, 4, 8, 4), (60, 6, 3, 2), (64, 16, 1, 1), (100, 4, 5, 2), (128, 8, 1, 1),
+                                               (200, 16, 8, 3), (256, 8, 8, 4), (300, 20, 1, 1), (512, 6, 16, 5)):
+        tokens = 8200 + experts
+        print("route, long", tokens, experts, topk, scoring, flush=True)
+        logits = 2 * randn(experts, tokens, experts)
+        logits[:200] = logits[:200].round()  # equal ones
+        logits[300, 1:] = -math.inf
+        logits[301:308] = 0.5  # all of them
+        logits[308] = -math.inf
+        mask = torch.arange(tokens) < tokens - 5
+        bias = (20 * randn(experts + 1, experts)).round() / 100
+        grad = randn(9, tokens, topk)
+        for normalize, dtype in ((True, BF16), (False, FP32)):
+            got = check_route(device, logits.to(dtype), topk, scoring=scoring, normalize=normalize, mask=mask)
+            check_route(device, logits.to(dtype), topk, scoring=scoring, normalize=normalize, bias=bias, groups=groups, topk_groups=topk_groups)
+            check_route(device, logits.to(dtype), topk, scoring=scoring, normalize=normalize, groups=groups, topk_groups=topk_groups)
+            check_route(device, logits.to(dtype), topk, scoring=scoring, normalize=normalize, bias=torch.zeros(experts))
+            logits[308] = 0.0
+            found = ep.route_topk_backward(grad.to(device), logits.to(dtype).to(device), got.ids, scoring=scoring, normalize=normalize)
+            oracle.check_rounded(found, *oracle.weigh_backward(grad, logits.to(dtype), got.ids.cpu(), scoring, normalize, 1.0), dtype)
+            logits[308] = -math.inf
 
 
 @pytest.mark.parametrize("scoring", SCORINGS)
@@ -501,6 +551,18 @@ def test_balance_loss_of_sequences(device, offsets, experts, scoring):
     ids[3:130] = -1  # (a sequence of padding)
     print("balance of sequences", len(offsets), experts, scoring, flush=True)
     check_balance(device, logits, ids, scoring, offsets)
+
+
+@pytest.mark.parametrize("scoring", SCORINGS)
+def test_balance_loss_of_many_short_sequences(device, scoring):
+    """Some empty, most of a few tokens, more than are searched at once."""
+    generator = torch.Generator().manual_seed(89)
+    for tokens, sequences, experts, topk in ((5000, 4500, 24, 3), (9000, 300, 60, 12), (700, 66, 130, 20)):
+        lengths = torch.randint(0, 2 * tokens // sequences + 1, (sequences,), generator=generator)
+        offsets = torch.cat([torch.zeros(1, dtype=torch.int64), lengths.cumsum(0)]).clamp(max=tokens - 3).tolist()
+        print("balance, short sequences", tokens, sequences, experts, topk, scoring, flush=True)
+        logits, ids = make_balance(tokens, experts, topk, experts)
+        check_balance(device, logits, ids, scoring, offsets)
 
 
 def test_balance_loss_of_long_batches(device):
