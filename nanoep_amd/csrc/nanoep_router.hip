@@ -30,31 +30,40 @@ __device__ __forceinline__ float load_logit(const Logits& logits, int64_t token,
     return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(logits.data)[at]) << 16);
 }
 
-// A token's logits over the kLanes lanes that share it: expert i * kLanes + lane in place i, -infinity behind the last expert and
-// where there is no token.  Neighbouring lanes read neighbours, whatever the rows' alignment.  All loads are on their way before any is
-// looked at: lanes without an expert read the first one's, of a token that there is.
+// A token's logits over the kLanes lanes that share it: expert i * kLanes + lane in place i.  Neighbouring lanes read neighbours, whatever
+// the rows' alignment.  All loads are on their way before any is looked at: lanes without an expert read the first one's, of a token that
+// there is.
 template <int kLanes, int kEach>
-__device__ __forceinline__ void load_spread(const Logits& logits, int64_t token, bool here, int experts, float (&out)[kEach]) {
+__device__ __forceinline__ void load_raw(const Logits& logits, int64_t token, bool here, int experts, uint32_t (&out)[kEach]) {
     const int lane = threadIdx.x % kLanes;
     const int64_t row = here ? token * logits.stride : 0;
     if (logits.wide) {
-        const float* from = static_cast<const float*>(logits.data) + row;
+        const uint32_t* from = static_cast<const uint32_t*>(logits.data) + row;
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
             out[i] = from[i * kLanes + lane < experts ? i * kLanes + lane : 0];
     } else {
         const uint16_t* from = static_cast<const uint16_t*>(logits.data) + row;
-        uint16_t narrow[kEach];
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
-            narrow[i] = from[i * kLanes + lane < experts ? i * kLanes + lane : 0];
-#pragma unroll
-        for (int i = 0; i < kEach; ++i)
-            out[i] = __uint_as_float(static_cast<uint32_t>(narrow[i]) << 16);
+            out[i] = from[i * kLanes + lane < experts ? i * kLanes + lane : 0];
     }
+}
+
+// Their values: -infinity behind the last expert and where there is no token.
+template <int kLanes, int kEach>
+__device__ __forceinline__ void logits_of_raw(const Logits& logits, const uint32_t (&raw)[kEach], bool here, int experts, float (&out)[kEach]) {
+    const int lane = threadIdx.x % kLanes, shift = logits.wide ? 0 : 16;
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
-        out[i] = here && i * kLanes + lane < experts ? out[i] : -INFINITY;
+        out[i] = here && i * kLanes + lane < experts ? __uint_as_float(raw[i] << shift) : -INFINITY;
+}
+
+template <int kLanes, int kEach>
+__device__ __forceinline__ void load_spread(const Logits& logits, int64_t token, bool here, int experts, float (&out)[kEach]) {
+    uint32_t raw[kEach];
+    load_raw<kLanes, kEach>(logits, token, here, experts, raw);
+    logits_of_raw<kLanes, kEach>(logits, raw, here, experts, out);
 }
 
 template <int kLanes, int kEach>
@@ -582,10 +591,16 @@ __device__ __forceinline__ void shares_of(const float (&logit)[kEach], bool sigm
             const float tail = exp_below(-fabsf(logit[i])), inverse = __builtin_amdgcn_rcpf(1.0f + tail);
             share[i] = logit[i] >= 0.0f ? inverse : tail * inverse;
             rest[i] = logit[i] >= 0.0f ? tail * inverse : inverse;
-            if (shifted && logit[i] < 0.0f)
-                share[i] = exp_below(logit[i] - shift) * inverse;
-            total += share[i];
         }
+        if (shifted) {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+                if (logit[i] < 0.0f)
+                    share[i] = exp_below(logit[i] - shift) * __builtin_amdgcn_rcpf(1.0f + exp_below(logit[i]));
+        }
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            total += share[i];
     } else {
         const float shift = largest == -INFINITY ? 0.0f : largest;
 #pragma unroll
@@ -734,10 +749,10 @@ __device__ __forceinline__ int64_t sequences_ahead(const Balance& a, int64_t tok
     return low;
 }
 
-// A token of each group of kLanes lanes: its logits, and choice k in lane k.
+// A token of each group of kLanes lanes: its logits as they lie in memory, and choice k in lane k.
 template <int kEach>
 struct BalanceToken {
-    float logit[kEach];
+    uint32_t logit[kEach];
     int64_t named;
     bool here;
 };
@@ -748,7 +763,7 @@ __device__ __forceinline__ void load_token(const Balance& a, int64_t token, bool
     out.named = -1;
     if (here && lane < a.topk)
         out.named = a.ids[token * a.topk + lane];
-    load_spread<kLanes, kEach>(a.logits, token, here, a.experts, out.logit);
+    load_raw<kLanes, kEach>(a.logits, token, here, a.experts, out.logit);
 }
 
 __device__ __forceinline__ float workgroup_sum(float v, float* place) {
@@ -816,8 +831,9 @@ __global__ void __launch_bounds__(kBlockThreads) balance_loss_kernel(const Balan
                 atomicAdd(&chosen[token.named], 1);
             const bool live = lanes_where<kLanes>(valid) != 0;
             number += live ? 1 : 0;
-            float share[kEach], rest[kEach];
-            shares_of<kLanes, kEach>(token.logit, a.sigmoid, share, rest);
+            float logit[kEach], share[kEach], rest[kEach];
+            logits_of_raw<kLanes, kEach>(a.logits, token.logit, token.here, a.experts, logit);
+            shares_of<kLanes, kEach>(logit, a.sigmoid, share, rest);
 #pragma unroll
             for (int i = 0; i < kEach; ++i)
                 own[i] += live ? share[i] : 0.0f;
@@ -1007,18 +1023,21 @@ __global__ void __launch_bounds__(kBlockThreads) balance_loss_backward_kernel(co
             break;
         BalanceToken<kEach> next;
         load_token<kLanes, kEach>(a, from + group, from + group < to, next);
+        int64_t count[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            count[i] = counts[sequence * a.experts + (i * kLanes + lane < a.experts ? i * kLanes + lane : 0)];
+        const int64_t live_tokens = tokens[sequence];
+        const float of_loss = grad[sequence];
+        __builtin_amdgcn_sched_barrier(0);  // (a conversion behind every load would wait for each of them)
         float factor[kEach], number = 0.0f;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const int expert = i * kLanes + lane;
-            const float count = static_cast<float>(counts[sequence * a.experts + (expert < a.experts ? expert : 0)]);
-            factor[i] = expert < a.experts ? count : 0.0f;
+            factor[i] = i * kLanes + lane < a.experts ? static_cast<float>(count[i]) : 0.0f;
             number += factor[i];
         }
         number = lanes_sum<kLanes>(number);
-        const int64_t live_tokens = tokens[sequence];
-        const float each =
-            live_tokens > 0 && number > 0.0f ? grad[sequence] * static_cast<float>(a.experts) / number / static_cast<float>(live_tokens) : 0.0f;
+        const float each = live_tokens > 0 && number > 0.0f ? of_loss * static_cast<float>(a.experts) / number / static_cast<float>(live_tokens) : 0.0f;
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
             factor[i] *= each;
@@ -1026,8 +1045,9 @@ __global__ void __launch_bounds__(kBlockThreads) balance_loss_backward_kernel(co
             const BalanceToken<kEach> token = next;
             load_token<kLanes, kEach>(a, first + kTokens + group, first + kTokens + group < to, next);
             const bool live = lanes_where<kLanes>(token.named >= 0 && token.named < a.experts) != 0;
-            float share[kEach], rest[kEach], out[kEach], along = 0.0f;
-            shares_of<kLanes, kEach>(token.logit, a.sigmoid, share, rest);
+            float logit[kEach], share[kEach], rest[kEach], out[kEach], along = 0.0f;
+            logits_of_raw<kLanes, kEach>(a.logits, token.logit, token.here, a.experts, logit);
+            shares_of<kLanes, kEach>(logit, a.sigmoid, share, rest);
 #pragma unroll
             for (int i = 0; i < kEach; ++i)
                 along = fmaf(factor[i], share[i], along);
