@@ -27,6 +27,10 @@ __device__ __forceinline__ uint32_t lanes_moved(uint32_t v) {
     return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), kControl, 0xf, 0xf, true));
 }
 template <int kControl>
+__device__ __forceinline__ int lanes_moved(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, kControl, 0xf, 0xf, true);
+}
+template <int kControl>
 __device__ __forceinline__ float lanes_moved(float v) {
     return __uint_as_float(lanes_moved<kControl>(__float_as_uint(v)));
 }
@@ -43,6 +47,13 @@ __device__ __forceinline__ void lanes_pair(uint32_t v, uint32_t& a, uint32_t& b)
     const auto both = kDistance == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
     a = both[0];
     b = both[1];
+}
+template <int kDistance>
+__device__ __forceinline__ void lanes_pair(int v, int& a, int& b) {
+    uint32_t x, y;
+    lanes_pair<kDistance>(static_cast<uint32_t>(v), x, y);
+    a = static_cast<int>(x);
+    b = static_cast<int>(y);
 }
 template <int kDistance>
 __device__ __forceinline__ void lanes_pair(float v, float& a, float& b) {

@@ -888,33 +888,21 @@ __global__ void __launch_bounds__(kBlockThreads) balance_loss_kernel(const Balan
     }
 }
 
-// The sum over `lanes` (a power of two) neighbouring lanes, in all of them.
-template <class T>
-__device__ __forceinline__ T sum_of_lanes(T v, int lanes) {
-    T a, b;
-    v += lanes >= 2 ? lanes_moved<0xB1>(v) : T{0};
-    v += lanes >= 4 ? lanes_moved<0x4E>(v) : T{0};
-    v += lanes >= 8 ? lanes_moved<0x141>(v) : T{0};
-    v += lanes >= 16 ? lanes_moved<0x140>(v) : T{0};
-    lanes_pair<16>(v, a, b);
-    v = lanes >= 32 ? a + b : v;
-    lanes_pair<32>(v, a, b);
-    return lanes >= 64 ? a + b : v;
-}
-
-// A sequence's rows are added up by 2^slice_bits workgroups, each for its part of the experts: four columns a thread, the rows shared out
-// among neighbouring threads, whose sums are then added in a fixed order.  Each leaves its part of sum c_e * share_e and of C; the one that
-// arrives last adds those up, in their order as well.  (Several slices only for one sequence: rows are many then.)  A chain of latencies
-// (offsets, rows, the slices' arrival), not of bytes.
-constexpr int kMostSlices = 16, kRowsAtOnce = 8;
-__global__ void __launch_bounds__(kBlockThreads) balance_finish_kernel(const Balance a, int width,  // columns of a row's half: 8 to 4096
+// A sequence's rows are added up by 2^slice_bits workgroups, each for its part of the experts: four columns a thread, neighbouring threads
+// neighbouring columns, the rows shared out among groups of threads, whose sums are then added in a fixed order.  Each leaves its part
+// of sum c_e * share_e and of C; the one that arrives last adds those up, in their order as well.  (Several slices only for one sequence:
+// rows are many then.)  A chain of latencies (offsets, rows, the slices' arrival), not of bytes.
+constexpr int kMostSlices = 16, kRowsAtOnce = 8, kFinishThreads = 1024;
+__global__ void __launch_bounds__(kFinishThreads) balance_finish_kernel(const Balance a, int width,  // columns of a row's half: 8 to 4096
                                                                        int slice_bits, const u32x4* __restrict__ rows,
                                                                        const int* __restrict__ live_of_rows, int* __restrict__ arrived,
                                                                        uint64_t* __restrict__ parts_of_loss,  // [slices]: sum's bits, C's above them
                                                                        float* __restrict__ loss, int64_t* __restrict__ counts,
                                                                        int64_t* __restrict__ tokens) {
-    __shared__ float place[kWavesPerBlock][2];
-    __shared__ int live_place[kWavesPerBlock];
+    __shared__ float share_parts[4 * kFinishThreads];
+    __shared__ uint32_t count_parts[4 * kFinishThreads];
+    __shared__ float place[kFinishThreads / kWave][2];
+    __shared__ int live_place[kFinishThreads / kWave];
     const int64_t sequence = workgroup_number() >> slice_bits;
     const int slices = 1 << slice_bits, slice = static_cast<int>(workgroup_number()) & (slices - 1);
     if (sequence >= a.sequences)
@@ -922,15 +910,16 @@ __global__ void __launch_bounds__(kBlockThreads) balance_finish_kernel(const Bal
     int64_t from = 0, to = a.tokens;
     clip(a, sequence, from, to);
     const int64_t first = (from >> a.chunk_bits) + sequence, end = to > from ? ((to - 1) >> a.chunk_bits) + sequence + 1 : first;
+    const int threads = blockDim.x;
     int live = 0;
-    for (int64_t row = first + threadIdx.x; row < end; row += kBlockThreads)
+    for (int64_t row = first + threadIdx.x; row < end; row += threads)
         live += live_of_rows[row];
     const int quads = width / 4 >> slice_bits;  // of this slice's columns
-    const int groups = quads >= kBlockThreads ? 1 : kBlockThreads / quads > kWave ? kWave : kBlockThreads / quads;
-    const int group = threadIdx.x & (groups - 1);
+    const int across = quads < threads ? quads : threads, groups = threads / across;
+    const int group = threadIdx.x / across, lane = threadIdx.x % across;
     float sum = 0.0f, number = 0.0f;
-    for (int quad = threadIdx.x / groups; quad < quads; quad += kBlockThreads) {
-        const int at = slice * quads + quad;
+    for (int some = 0; some < quads; some += across) {
+        const int at = slice * quads + some;
         float share[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         u32x4 count = {0u, 0u, 0u, 0u};
         for (int64_t base = first + group; base < end; base += kRowsAtOnce * groups) {
@@ -938,8 +927,8 @@ __global__ void __launch_bounds__(kBlockThreads) balance_finish_kernel(const Bal
 #pragma unroll
             for (int r = 0; r < kRowsAtOnce; ++r) {
                 const int64_t row = base + r * groups < end ? base + r * groups : base;
-                other[r] = rows[row * (width / 2) + at];
-                more[r] = rows[row * (width / 2) + width / 4 + at];
+                other[r] = rows[row * (width / 2) + at + lane];
+                more[r] = rows[row * (width / 2) + width / 4 + at + lane];
             }
 #pragma unroll
             for (int r = 0; r < kRowsAtOnce; ++r)
@@ -952,18 +941,29 @@ __global__ void __launch_bounds__(kBlockThreads) balance_finish_kernel(const Bal
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            share[i] = sum_of_lanes(share[i], groups);
-            count[i] = sum_of_lanes(count[i], groups);
-            if (group == 0 && at * 4 + i < a.experts) {
-                counts[sequence * a.experts + at * 4 + i] = count[i];
-                sum = fmaf(static_cast<float>(count[i]), share[i], sum);
-                number += static_cast<float>(count[i]);
+            share_parts[(group * across + lane) * 4 + i] = share[i];
+            count_parts[(group * across + lane) * 4 + i] = count[i];
+        }
+        __syncthreads();
+        for (int column = threadIdx.x; column < across * 4; column += threads) {
+            float shares = 0.0f;
+            uint32_t chosen = 0;
+#pragma unroll 8
+            for (int part = 0; part < groups; ++part) {
+                shares += share_parts[part * across * 4 + column];
+                chosen += count_parts[part * across * 4 + column];
+            }
+            if (at * 4 + column < a.experts) {
+                counts[sequence * a.experts + at * 4 + column] = chosen;
+                sum = fmaf(static_cast<float>(chosen), shares, sum);
+                number += static_cast<float>(chosen);
             }
         }
+        __syncthreads();
     }
     sum = lanes_sum<kWave>(sum);
     number = lanes_sum<kWave>(number);
-    live = static_cast<int>(sum_of_lanes(static_cast<uint32_t>(live), kWave));
+    live = lanes_sum<kWave>(live);
     if (threadIdx.x % kWave == 0) {
         place[threadIdx.x / kWave][0] = sum;
         place[threadIdx.x / kWave][1] = number;
@@ -974,7 +974,7 @@ __global__ void __launch_bounds__(kBlockThreads) balance_finish_kernel(const Bal
         return;
     sum = number = 0.0f;
     live = 0;
-    for (int w = 0; w < kWavesPerBlock; ++w) {
+    for (int w = 0; w < threads / kWave; ++w) {
         sum += place[w][0];
         number += place[w][1];
         live += live_place[w];
@@ -1095,6 +1095,12 @@ Spread spread_of(int experts, int needed) {
 // then (us with 16, 32 and 64 lanes of 256 experts, a bias: 1 token 5.7, 4.8, 4.4; 4096 tokens 8.4, 6.9, 7.8; 32768 tokens 19.2, 22.4, 41.6).
 Spread spread_for_choices(int64_t num_tokens, int experts, int needed) {
     return spread_of(experts, std::max(needed, num_tokens <= int64_t{32} * current_topology(current_tuning()).cus ? 32 : 1));
+}
+
+// For the loss, the same, and 32 lanes for more than 128 experts, because twice as many experts a lane leave a SIMD half of its
+// wavefronts (the gradient of 14681 tokens of 211 experts: 16 lanes 12.2 us, 32 lanes 9.7).
+Spread spread_for_balance(int64_t num_tokens, int experts, int topk) {
+    return spread_for_choices(num_tokens, experts, experts > 128 ? std::max(topk, 32) : topk);
 }
 
 // CALL(lanes, experts a lane) for a Spread of 8 lanes or more, and of 16 or more.
@@ -1240,15 +1246,14 @@ struct BalancePlan {
 };
 BalancePlan plan_balance(int64_t num_tokens, int experts, int topk, int64_t sequences) {
     BalancePlan plan;
-    plan.spread = spread_of(experts, topk);
+    plan.spread = spread_for_balance(num_tokens, experts, topk);
     const int64_t round = kBlockThreads / plan.spread.lanes, most = int64_t{2} * current_topology(current_tuning()).cus;
     const int64_t average = (num_tokens + sequences - 1) / sequences;
     plan.chunk_bits = bits_of(sequences == 1 && num_tokens <= 4 * round ? 4 * round : std::max(round, std::min(average, (num_tokens + most - 1) / most)));
     plan.chunks = (num_tokens + (int64_t{1} << plan.chunk_bits) - 1) >> plan.chunk_bits;
     plan.rows = sequences == 1 && plan.chunks == 1 ? 0 : plan.chunks + sequences;
-    plan.slice_bits = 0;
-    while (sequences == 1 && (1 << plan.slice_bits) < kMostSlices && (1 << plan.slice_bits) < plan.spread.lanes * plan.spread.each / 4)
-        ++plan.slice_bits;
+    // (256 bytes of a row at least: E = 64, 512 rows 5.5 us)
+    plan.slice_bits = sequences == 1 ? std::min(bits_of(kMostSlices), bits_of((plan.spread.lanes * plan.spread.each + 63) / 64)) : 0;
     return plan;
 }
 // The slices' parts of the loss, rows, their numbers of tokens, the number of slices that are done.
@@ -1364,7 +1369,7 @@ int nanoep_balance_loss(const void* logits, int64_t logits_stride, int logits_ty
     }
     if (plan.rows > 0) {
         const int slice_bits = plan.chunks > 0 ? plan.slice_bits : 0;  // (without tokens nobody cleared the number of those done)
-        balance_finish_kernel<<<grid_of(sequences << slice_bits), kBlockThreads, 0, on>>>(arguments, width, slice_bits, reinterpret_cast<const u32x4*>(rows),
+        balance_finish_kernel<<<grid_of(sequences << slice_bits), sequences == 1 ? kFinishThreads : kBlockThreads, 0, on>>>(arguments, width, slice_bits, reinterpret_cast<const u32x4*>(rows),
                                                                                    live_of_rows, arrived, parts_of_loss, loss, counts, tokens);
         NANOEP_HIP_TRY(hipGetLastError());
     }
@@ -1384,7 +1389,7 @@ int nanoep_balance_loss_backward(const float* grad, const void* logits, int64_t 
         return NANOEP_ERR_INVALID_ARGUMENT;
     // a wavefront one round of tokens, more where that would be more than 16 wavefronts a compute unit (us with 4, 8, 16, 32 of them: 32768
     // tokens of 64 experts 9.0, 6.8, 6.7, 7.1; of 128, 64 sequences, 15.0, 11.6, 11.0, 12.6)
-    const Spread spread = spread_of(num_experts, num_topk);
+    const Spread spread = spread_for_balance(num_tokens, num_experts, num_topk);
     const int64_t held = int64_t{16} * current_topology(current_tuning()).cus;
     const int chunk_bits = bits_of(std::max<int64_t>(kWave / spread.lanes, (num_tokens + held - 1) / held));
     const Balance arguments = {logits_of(logits, logits_stride, logits_type), ids, sequence_offsets, num_tokens, sequences, chunk_bits, num_experts, num_topk,
