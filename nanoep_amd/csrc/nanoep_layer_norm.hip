@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kMostThreads) layer_norm_kernel(const u32x4* _
             }
             squares = lanes_sum<kMostRowWaves>(squares);
         }
-        const float rstd = rsqrtf(fmaf(squares, per_column, eps));
+        const float rstd = 1.0f / sqrtf(fmaf(squares, per_column, eps));
         store_within<false>(rstds + (here ? row : 0), here ? 4 : 0, threadIdx.x, rstd);
         if (centred)
             store_within<false>(means + (here ? row : 0), here ? 4 : 0, threadIdx.x, mean);
@@ -241,8 +241,7 @@ __global__ void __launch_bounds__(kMostThreads) layer_norm_kernel(const u32x4* _
 // The gradient.  A workgroup works through rows (those of a turn are neighbours over all workgroups; `teams` of them at a time in a
 // workgroup) and keeps the two sums over rows in registers; at its end it writes them, added over its teams, to its row of `sums`
 // ([workgroups][2][columns] fp32), which parameter_gradient_kernel adds up in a fixed order.  No atomics.
-// With d = s - mean, along = sum(u * d): dx = r * u - r * mean(u) - d * r^3 * along / H.  d and u stay in registers between a row's sums
-// and its output; the next row's inputs are on their way meanwhile.
+// z and u stay in registers between a row's sums and its output; the next row's inputs are on their way meanwhile.
 template <class T, class P, int kVectors, bool kAdded, bool kInput>
 __global__ void __launch_bounds__(kBackwardThreads) layer_norm_backward_kernel(const u32x4* __restrict__ grad,   // [T][vectors]
                                                                                const u32x4* __restrict__ total,  // [T][vectors]
@@ -311,12 +310,12 @@ __global__ void __launch_bounds__(kBackwardThreads) layer_norm_backward_kernel(c
         const int64_t row = first + team;
         const bool here = row < rows;
         const float mean = next.mean, rstd = next.rstd;
-        float d[kVectors][kColumns], u[kVectors][kColumns], both[2] = {0.0f, 0.0f};
+        float z[kVectors][kColumns], u[kVectors][kColumns], both[2] = {0.0f, 0.0f};
         u32x4 added[kVectors];
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
             float factor[kColumns];
-            Row::unpack(next.total[v], d[v]);
+            Row::unpack(next.total[v], z[v]);
             Row::unpack(next.grad[v], u[v]);
             held[v].unpack(factor);
             if (kAdded)
@@ -325,12 +324,12 @@ __global__ void __launch_bounds__(kBackwardThreads) layer_norm_backward_kernel(c
 #pragma unroll
                 for (int i = 0; i < kColumns; ++i) {
                     const float g = u[v][i];
-                    d[v][i] -= mean;
+                    z[v][i] = (z[v][i] - mean) * rstd;
                     u[v][i] *= factor[i];
                     sum_g[v][i] += g;
-                    sum_z[v][i] = fmaf(g * rstd, d[v][i], sum_z[v][i]);
+                    sum_z[v][i] = fmaf(g, z[v][i], sum_z[v][i]);
                     both[0] += u[v][i];
-                    both[1] = fmaf(u[v][i], d[v][i], both[1]);
+                    both[1] = fmaf(u[v][i], z[v][i], both[1]);
                 }
             }
         }
@@ -346,12 +345,12 @@ __global__ void __launch_bounds__(kBackwardThreads) layer_norm_backward_kernel(c
                 both[0] = lanes_sum<kMostRowWaves>(other.x);
                 both[1] = lanes_sum<kMostRowWaves>(other.y);
             }
-            const float across = means != nullptr ? both[0] * per_column * -rstd : 0.0f, along = both[1] * per_column * rstd * rstd * -rstd;
+            const float across = means != nullptr ? both[0] * per_column * -rstd : 0.0f, along = both[1] * per_column * -rstd;
 #pragma unroll
             for (int v = 0; v < kVectors; ++v) {
 #pragma unroll
                 for (int i = 0; i < kColumns; ++i)
-                    u[v][i] = fmaf(u[v][i], rstd, fmaf(d[v][i], along, across));
+                    u[v][i] = fmaf(u[v][i], rstd, fmaf(z[v][i], along, across));
                 if (kAdded) {
                     float more[kColumns];
                     Row::unpack(added[v], more);

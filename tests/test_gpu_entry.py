@@ -90,6 +90,18 @@ def test_norm_of_rows_far_from_zero(device, rows):
 
 
 @pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("rows", [BF16, FP32])
+@pytest.mark.parametrize("power", [-58, -20, 20, 55])
+def test_norm_of_very_small_and_very_large_rows(device, kind, rows, power):
+    """As far as the squares are in fp32, a factor of all rows is one of nothing but the statistics and the gradient."""
+    total, _, gamma, beta = make_norm(9, 520, rows, FP32, 6, residual=False)
+    total = total * 2.0**power
+    print("norm of scaled rows", kind, rows, power, flush=True)
+    check_norm(device, kind, total, None, gamma, beta, 0.0)
+    check_norm_backward(device, kind, randn(7, 9, 520).to(rows), total, gamma, None, eps=0.0)
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
 @pytest.mark.parametrize("hidden", [512, 2816])
 def test_norm_of_zeros_infinities_and_nan(device, kind, hidden):
     x, _, gamma, beta = make_norm(9, hidden, BF16, BF16, 7, residual=False)
