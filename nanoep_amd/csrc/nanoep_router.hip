@@ -662,7 +662,8 @@ __global__ void __launch_bounds__(kBlockThreads) route_topk_backward_kernel(cons
         load_spread<kLanes, kEach>(a.logits, token, here, a.experts, out);
         shares_of<kLanes, kEach>(out, false, share, rest);
     } else if (a.normalize) {
-        const float largest = lanes_max<kLanes>(logit);
+        float largest = lanes_max<kLanes>(logit);
+        largest = largest == -INFINITY ? 0.0f : largest;  // (nothing but experts that cannot be chosen: no weights)
         float score = 0.0f, rest = 1.0f;
         if (a.sigmoid) {
             const float tail = expf(-fabsf(logit)), inverse = 1.0f / (1.0f + tail);
@@ -673,7 +674,7 @@ __global__ void __launch_bounds__(kBlockThreads) route_topk_backward_kernel(cons
         }
         score = valid ? score : 0.0f;
         const float total = lanes_sum<kLanes>(score);
-        score = valid ? score / total : 0.0f;
+        score = valid && total != 0.0f ? score / total : 0.0f;
         g = score * rest * (g - lanes_sum<kLanes>(score * g));
     } else {
         const float tail = expf(-fabsf(logit)), inverse = 1.0f / (1.0f + tail);

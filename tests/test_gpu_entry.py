@@ -503,6 +503,28 @@ def test_route_backward(device, experts, scoring, normalize):
 
 @pytest.mark.parametrize("scoring", SCORINGS)
 @pytest.mark.parametrize("normalize", [True, False])
+def test_route_backward_of_masked_and_extreme_logits(device, scoring, normalize):
+    """Choices of experts that could not have been chosen among them, and gradients of masked choices that are not looked at."""
+    tokens, experts, topk = 8, 40, 4
+    logits, grad = randn(73, tokens, experts), randn(74, tokens, topk)
+    ids = torch.arange(topk).repeat(tokens, 1) * 9
+    logits[0] = -math.inf
+    logits[0, 39] = 1.0
+    logits[1, :20] = -math.inf
+    logits[2] = LOWEST
+    logits[3, 9] = LOWEST
+    logits[4] = -300.0 - torch.arange(experts)
+    logits[5] = 90.0 + torch.arange(experts)
+    ids[6, 1], ids[6, 3] = -1, experts
+    grad[6, 1], grad[6, 3] = math.nan, math.inf
+    print("route backward, extreme", scoring, normalize, flush=True)
+    found = ep.route_topk_backward(grad.to(device), logits.to(device), ids.to(device), scoring=scoring, normalize=normalize)
+    oracle.check_rounded(found, *oracle.weigh_backward(grad, logits, ids, scoring, normalize, 1.0), FP32)
+    assert found.isfinite().all()
+
+
+@pytest.mark.parametrize("scoring", SCORINGS)
+@pytest.mark.parametrize("normalize", [True, False])
 def test_the_routers_gradient_is_the_difference(device, scoring, normalize):
     tokens, experts, topk = 9, 40, 5
     logits, grad = randn(71, tokens, experts), randn(72, tokens, topk)
