@@ -32,22 +32,28 @@ __device__ __forceinline__ float load_logit(const Logits& logits, int64_t token,
 
 // A token's logits over the kLanes lanes that share it: expert i * kLanes + lane in place i.  Neighbouring lanes read neighbours, whatever
 // the rows' alignment.  All loads are on their way before any is looked at: lanes without an expert read the first one's, of a token that
-// there is.
-template <int kLanes, int kEach>
-__device__ __forceinline__ void load_raw(const Logits& logits, int64_t token, bool here, int experts, uint32_t (&out)[kEach]) {
+// there is.  Rows that fill their lanes, as most do, need neither that nor an address for each place.
+template <int kLanes, int kEach, class T>
+__device__ __forceinline__ void load_row(const T* from, int experts, uint32_t (&out)[kEach]) {
     const int lane = threadIdx.x % kLanes;
-    const int64_t row = here ? token * logits.stride : 0;
-    if (logits.wide) {
-        const uint32_t* from = static_cast<const uint32_t*>(logits.data) + row;
+    if (experts == kLanes * kEach) {
+        from += lane;
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
-            out[i] = from[i * kLanes + lane < experts ? i * kLanes + lane : 0];
+            out[i] = from[i * kLanes];
     } else {
-        const uint16_t* from = static_cast<const uint16_t*>(logits.data) + row;
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
             out[i] = from[i * kLanes + lane < experts ? i * kLanes + lane : 0];
     }
+}
+template <int kLanes, int kEach>
+__device__ __forceinline__ void load_raw(const Logits& logits, int64_t token, bool here, int experts, uint32_t (&out)[kEach]) {
+    const int64_t row = here ? token * logits.stride : 0;
+    if (logits.wide)
+        load_row<kLanes, kEach>(static_cast<const uint32_t*>(logits.data) + row, experts, out);
+    else
+        load_row<kLanes, kEach>(static_cast<const uint16_t*>(logits.data) + row, experts, out);
 }
 
 // Their values: -infinity behind the last expert and where there is no token.
@@ -66,34 +72,49 @@ __device__ __forceinline__ void load_spread(const Logits& logits, int64_t token,
     logits_of_raw<kLanes, kEach>(logits, raw, here, experts, out);
 }
 
+template <int kLanes, int kEach, class Put>
+__device__ __forceinline__ void store_row(bool here, int experts, Put put) {
+    const int lane = threadIdx.x % kLanes;
+    if (experts == kLanes * kEach) {
+        if (here)
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+                put(i);
+    } else {
+        const int mine = here ? experts : 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (i * kLanes + lane < mine)
+                put(i);
+    }
+}
 template <int kLanes, int kEach>
 __device__ __forceinline__ void store_spread(void* out, bool wide, int64_t token, bool here, int experts, const float (&v)[kEach]) {
-    const int lane = threadIdx.x % kLanes, mine = here ? experts : 0;
-    const int64_t row = here ? token * experts : 0;
+    const int64_t row = (here ? token * experts : 0) + threadIdx.x % kLanes;
     if (wide) {
         float* to = static_cast<float*>(out) + row;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i)
-            if (i * kLanes + lane < mine)
-                to[i * kLanes + lane] = v[i];
+        store_row<kLanes, kEach>(here, experts, [&](int i) { to[i * kLanes] = v[i]; });
     } else {
         uint16_t* to = static_cast<uint16_t*>(out) + row;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i)
-            if (i * kLanes + lane < mine)
-                to[i * kLanes + lane] = static_cast<uint16_t>(to_bf16_pair(v[i], 0.0f));
+        store_row<kLanes, kEach>(here, experts, [&](int i) { to[i * kLanes] = static_cast<uint16_t>(to_bf16_pair(v[i], 0.0f)); });
     }
+}
+
+// e^x for x <= 0, good to 2^-22: 2^n times 2 to the rest of x log2 e, with log2 e in two parts.
+__device__ __forceinline__ float exp_below(float x) {
+    x = x < -200.0f ? -200.0f : x;  // (a NaN stays one)
+    const float whole = rintf(x * 0x1.715476p+0f);
+    const float rest = fmaf(x, 0x1.4ae0cp-26f, fmaf(x, 0x1.715476p+0f, -whole));
+    return ldexpf(__builtin_amdgcn_exp2f(rest), static_cast<int>(whole));
 }
 
 // Values as unsigned integers in the same order: 0 for -infinity, which stands for an expert that cannot be chosen, NaN above
 // everything, both zeros alike.
+constexpr uint32_t kLowestKey = 0x007fffffu;  // of -infinity, ahead of its subtraction
 __device__ __forceinline__ uint32_t key_of(float v) {
     const uint32_t bits = __float_as_uint(v + 0.0f);
-    if (v != v)
-        return 0xffffffffu;
-    if (bits == 0xff800000u)
-        return 0u;
-    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+    const uint32_t key = bits ^ (static_cast<uint32_t>(static_cast<int>(bits) >> 31) | 0x80000000u);
+    return v != v ? 0xffffffffu : key - kLowestKey;
 }
 __device__ __forceinline__ uint64_t key_of(double v) {
     const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(v + 0.0));
@@ -104,9 +125,8 @@ __device__ __forceinline__ uint64_t key_of(double v) {
     return bits >> 63 ? ~bits : bits | uint64_t{1} << 63;
 }
 __device__ __forceinline__ float value_of(uint32_t key) {
-    if (key == 0)
-        return -INFINITY;
-    return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);  // all ones: a NaN
+    const uint32_t bits = key + (key == 0xffffffffu ? 0u : kLowestKey);
+    return __uint_as_float(bits >> 31 ? bits & 0x7fffffffu : ~bits);  // all ones: a NaN
 }
 __device__ __forceinline__ double value_of(uint64_t key) {
     if (key == 0)
@@ -164,6 +184,45 @@ __device__ __forceinline__ void choose_in_turn(Key (&key)[kEach], int rounds, ui
 #pragma unroll
             for (int i = 0; i < kEach; ++i)
                 key[i] = i * kLanes + lane == expert ? 0 : key[i];
+        }
+    }
+    wavefront_sync();
+}
+
+// The same for few keys a lane, which are sorted first, so that a round looks at a lane's first one and moves the others up: with four
+// of them, eight rounds and the sort are 150 vector instructions where eight rounds over all are 250.
+template <int kLanes, int kEach>
+__device__ __forceinline__ void choose_sorted(uint32_t (&key)[kEach], int rounds, uint32_t* chosen_expert, uint32_t* chosen_key) {
+    uint32_t expert[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+        expert[i] = i * kLanes + threadIdx.x % kLanes;
+#pragma unroll
+    for (int last = kEach - 1; last > 0; --last)
+#pragma unroll
+        for (int i = 0; i < last; ++i) {  // neighbours only, so that equal ones stay in their order
+            const uint32_t one = key[i], other = key[i + 1], expert_of_one = expert[i], expert_of_other = expert[i + 1];
+            key[i] = other > one ? other : one;
+            key[i + 1] = other > one ? one : other;
+            expert[i] = other > one ? expert_of_other : expert_of_one;
+            expert[i + 1] = other > one ? expert_of_one : expert_of_other;
+        }
+    for (int round = 0; round < rounds; ++round) {
+        const uint32_t top = lanes_max<kLanes>(key[0]);
+        bool wins = key[0] == top;
+        if (__popcll(__ballot(wins)) > kWave / kLanes) {  // more lanes than tokens have theirs: equal keys
+            const uint32_t lowest = lanes_min<kLanes>(wins ? expert[0] : kNoExpert);
+            wins = wins && expert[0] == lowest;
+        }
+        if (wins) {
+            chosen_expert[round] = top != 0 ? expert[0] : kNoExpert;
+            chosen_key[round] = top;
+#pragma unroll
+            for (int i = 0; i + 1 < kEach; ++i) {
+                key[i] = key[i + 1];
+                expert[i] = expert[i + 1];
+            }
+            key[kEach - 1] = 0;
         }
     }
     wavefront_sync();
@@ -277,13 +336,13 @@ __device__ __forceinline__ void store_choices(const Route& a, int64_t token, uin
     if (a.sigmoid) {
         // numerators and denominators times e^-shift, so that their sum is not lost where all scores are tiny
         const float shift = a.normalize ? fminf(lanes_max<kLanes>(valid ? logit : -INFINITY), 0.0f) : 0.0f;
-        weight = expf(fminf(logit, 0.0f) - shift) / (1.0f + expf(-fabsf(logit)));
+        weight = exp_below(fminf(logit, 0.0f) - shift) / (1.0f + exp_below(-fabsf(logit)));
         if (logit != logit)
             weight = logit;
     } else {
         if (a.normalize)
             largest = lanes_max<kLanes>(valid ? logit : -INFINITY);
-        weight = broken ? NAN : expf(logit - largest);
+        weight = broken ? NAN : exp_below(logit - largest);
     }
     weight = valid ? weight : 0.0f;
     if (a.normalize)
@@ -308,7 +367,7 @@ __device__ __forceinline__ void softmax_of(const float (&logit)[kEach], float (&
     largest = largest == -INFINITY ? 0.0f : largest;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-        exponential[i] = expf(logit[i] - largest);
+        exponential[i] = exp_below(logit[i] - largest);
         total += exponential[i];
     }
     total = lanes_sum<kLanes>(total);
@@ -371,7 +430,9 @@ __global__ void __launch_bounds__(kBlockThreads) route_topk_kernel(const Route a
             wavefront_sync();
         }
     }
-    if (!listed)  // (or many equal keys, or all of the largest in a few lanes)
+    if constexpr (kEach <= 4)
+        choose_sorted<kLanes, kEach>(key, a.topk, experts, keys);
+    else if (!listed)  // (many equal keys, or all of the largest in a few lanes)
         choose_in_turn<kLanes, kEach>(key, a.topk, experts, keys);
     uint32_t expert = kNoExpert;
     float chosen = 0.0f;
@@ -570,14 +631,6 @@ __global__ void __launch_bounds__(kBlockThreads) route_values_kernel(const Route
 
 // ------------------------------------------------------------------ gradients of a token's scores
 
-// e^x for x <= 0, good to 2^-22: the product with log2 e is kept with its rounding.
-__device__ __forceinline__ float exp_below(float x) {
-    x = x < -200.0f ? -200.0f : x;  // (a NaN stays one)
-    const float whole = x * 0x1.715476p+0f;
-    const float rounding = fmaf(x, 0x1.4ae0cp-26f, fmaf(x, 0x1.715476p+0f, -whole));
-    return fmaf(__builtin_amdgcn_exp2f(whole), rounding * 0x1.62e43p-1f, __builtin_amdgcn_exp2f(whole));
-}
-
 // Every expert's share of its token: softmax, or sigmoid over its sum.  rest: what is left of its sigmoid to one (softmax: 1).
 // Experts at -infinity have none; a token of nothing else has no shares.
 template <int kLanes, int kEach>
@@ -672,18 +725,18 @@ __global__ void __launch_bounds__(kBlockThreads) route_topk_backward_kernel(cons
         largest = largest == -INFINITY ? 0.0f : largest;  // (nothing but experts that cannot be chosen: no weights)
         float score = 0.0f, rest = 1.0f;
         if (a.sigmoid) {
-            const float tail = expf(-fabsf(logit)), inverse = 1.0f / (1.0f + tail);
-            score = logit != logit ? logit : expf(fminf(logit, 0.0f) - fminf(largest, 0.0f)) * inverse;
+            const float tail = exp_below(-fabsf(logit)), inverse = 1.0f / (1.0f + tail);
+            score = logit != logit ? logit : exp_below(fminf(logit, 0.0f) - fminf(largest, 0.0f)) * inverse;
             rest = logit >= 0.0f ? tail * inverse : inverse;
         } else {
-            score = expf(logit - largest);
+            score = exp_below(logit - largest);
         }
         score = valid ? score : 0.0f;
         const float total = lanes_sum<kLanes>(score);
         score = valid && total != 0.0f ? score / total : 0.0f;
         g = score * rest * (g - lanes_sum<kLanes>(score * g));
     } else {
-        const float tail = expf(-fabsf(logit)), inverse = 1.0f / (1.0f + tail);
+        const float tail = exp_below(-fabsf(logit)), inverse = 1.0f / (1.0f + tail);
         g = g * tail * inverse * inverse;
     }
     all_choices[place][lane] = make_float2(__int_as_float(expert), g);
