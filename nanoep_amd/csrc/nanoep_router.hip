@@ -6,6 +6,7 @@
 // in 64 bits.  Weights, losses and gradients are fp32.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "nanoep_lanes.h"
 #include "nanoep_operators.h"
@@ -315,13 +316,14 @@ __device__ __forceinline__ auto keep_groups(Key (&key)[kEach], const Route& a, K
     const uint64_t open = lanes_where<kLanes>(kept && of_group != 0);
     const Key last = ~largest_key<kLanes>(kept ? ~of_group : Key{0}), first_out = largest_key<kLanes>(lane < groups && !kept ? of_group : Key{0});
     // (a quotient of the middle of an expert's place: never near a whole number)
-    const float per_group = 1.0f / static_cast<float>(size);
+    const float per_group = 1.0f / static_cast<float>(size), first = (static_cast<float>(lane) + 0.5f) * per_group;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-        const int expert = i * kLanes + lane;
-        const int of = static_cast<int>((static_cast<float>(expert) + 0.5f) * per_group);
-        const bool stays = kLanes == kWave ? open >> (of & 63) & 1 : static_cast<uint32_t>(open) >> (of & 31) & 1;
-        key[i] = stays && expert < a.experts ? key[i] : 0;
+        const uint32_t of = static_cast<uint32_t>(fmaf(static_cast<float>(i * kLanes), per_group, first));
+        if constexpr (kLanes == kWave)
+            key[i] = open >> (of & 63) & 1 ? key[i] : 0;
+        else
+            key[i] &= static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(open), of, 1));  // (a bit, as all of a word)
     }
     return value_of(last) - value_of(first_out);
 }
@@ -409,24 +411,33 @@ __global__ void __launch_bounds__(kBlockThreads) route_topk_kernel(const Route a
         });
         listed = most <= kListed;
         if (listed) {
-            const uint64_t one = list[lane], other = list[kLanes + lane];
-            int ahead = 0, other_ahead = 0;
-#pragma unroll 4
-            for (uint32_t j = 0; j < most; ++j) {
-                const uint64_t against = list[j];
-                ahead += against > one ? 1 : 0;
-                other_ahead += against > other ? 1 : 0;
-            }
             if (lane >= static_cast<int>(number))
                 experts[lane] = kNoExpert;
-            if (one != 0 && ahead < a.topk) {
-                experts[ahead] = ~static_cast<uint32_t>(one);
-                keys[ahead] = static_cast<uint32_t>(one >> 32);
-            }
-            if (other != 0 && other_ahead < a.topk) {
-                experts[other_ahead] = ~static_cast<uint32_t>(other);
-                keys[other_ahead] = static_cast<uint32_t>(other >> 32);
-            }
+            const auto choose = [&](auto listed_each) {  // one or two of the list a lane
+                constexpr int kListedEach = decltype(listed_each)::value;
+                uint64_t own[kListedEach];
+                int ahead[kListedEach] = {};
+#pragma unroll
+                for (int which = 0; which < kListedEach; ++which)
+                    own[which] = list[which * kLanes + lane];
+#pragma unroll 4
+                for (uint32_t j = 0; j < most; ++j) {
+                    const uint64_t against = list[j];
+#pragma unroll
+                    for (int which = 0; which < kListedEach; ++which)
+                        ahead[which] += against > own[which] ? 1 : 0;
+                }
+#pragma unroll
+                for (int which = 0; which < kListedEach; ++which)
+                    if (own[which] != 0 && ahead[which] < a.topk) {
+                        experts[ahead[which]] = ~static_cast<uint32_t>(own[which]);
+                        keys[ahead[which]] = static_cast<uint32_t>(own[which] >> 32);
+                    }
+            };
+            if (most <= kLanes)
+                choose(std::integral_constant<int, 1>{});
+            else
+                choose(std::integral_constant<int, 2>{});
             wavefront_sync();
         }
     }
@@ -572,7 +583,7 @@ __global__ void __launch_bounds__(kBlockThreads) route_values_kernel(const Route
     wavefront_sync();
     uint32_t most;
     const uint32_t number = list_candidates<kLanes, kEach>(key, bound, kListed, most, [&](uint32_t at, int i) {
-        list[at] = {1 + static_cast<uint64_t>(__float_as_uint(bias[i])), static_cast<uint32_t>(i * kLanes + lane), logit[i]};
+        list[at] = {uint64_t{1} << 32 | __float_as_uint(bias[i]), static_cast<uint32_t>(i * kLanes + lane), logit[i]};
     });
     again = again || number > kListed;
     double wide_total = 0.0;
@@ -590,27 +601,34 @@ __global__ void __launch_bounds__(kBlockThreads) route_values_kernel(const Route
             if (which == 1 && most <= kLanes)
                 break;
             if (own[which].key != 0) {
-                own[which].key = key_of(value_of_expert(a, own[which].logit, __uint_as_float(static_cast<uint32_t>(own[which].key - 1)), largest, wide_total));
+                own[which].key = key_of(value_of_expert(a, own[which].logit, __uint_as_float(static_cast<uint32_t>(own[which].key)), largest, wide_total));
                 list[which * kLanes + lane].key = own[which].key;
             }
         }
         wavefront_sync();
-        int ahead[2] = {0, 0};
-#pragma unroll 4
-        for (uint32_t j = 0; j < most; ++j) {
-            const Candidate against = list[j];
-#pragma unroll
-            for (int which = 0; which < 2; ++which)
-                ahead[which] += against.key > own[which].key || (against.key == own[which].key && against.expert < own[which].expert) ? 1 : 0;
-        }
         if (lane >= static_cast<int>(number))
             experts[lane] = kNoExpert;
+        const auto choose = [&](auto listed_each) {  // one or two of the list a lane
+            constexpr int kListedEach = decltype(listed_each)::value;
+            int ahead[kListedEach] = {};
+#pragma unroll 4
+            for (uint32_t j = 0; j < most; ++j) {
+                const Candidate against = list[j];
 #pragma unroll
-        for (int which = 0; which < 2; ++which)
-            if (own[which].key != 0 && ahead[which] < a.topk) {
-                experts[ahead[which]] = own[which].expert;
-                logits[ahead[which]] = own[which].logit;
+                for (int which = 0; which < kListedEach; ++which)
+                    ahead[which] += against.key > own[which].key || (against.key == own[which].key && against.expert < own[which].expert) ? 1 : 0;
             }
+#pragma unroll
+            for (int which = 0; which < kListedEach; ++which)
+                if (own[which].key != 0 && ahead[which] < a.topk) {
+                    experts[ahead[which]] = own[which].expert;
+                    logits[ahead[which]] = own[which].logit;
+                }
+        };
+        if (most <= kLanes)
+            choose(std::integral_constant<int, 1>{});
+        else
+            choose(std::integral_constant<int, 2>{});
         wavefront_sync();
     } else {
         again = true;
