@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kBackwardThreads) layer_norm_backward_kernel(c
                                                                                const float* __restrict__ rstds,
                                                                                const u32x4* __restrict__ grad_residual,  // [T][vectors], if kAdded
                                                                                u32x4* __restrict__ grad_x,               // [T][vectors], if kInput
-                                                                               float* __restrict__ sums,                 // null: not wanted
+                                                                               u32x4* __restrict__ sums,                 // null: not wanted
                                                                                int64_t rows,
                                                                                int64_t groups,
                                                                                int vectors,
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(kBackwardThreads) layer_norm_backward_kernel(c
     using Row = RowType<T>;
     constexpr int kColumns = Row::kColumns;
     __shared__ float2 places[2][kBackwardThreads / kWave];
-    extern __shared__ float team_sums[];  // [blockDim.y - 1][columns], if there are several teams
+    extern __shared__ u32x4 team_sums[];  // [teams][columns / 4], if there are several
     // (a wavefront is one team's: what goes by the row is scalar)
     const int waves = blockDim.x / kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int teams = blockDim.y, team = __builtin_amdgcn_readfirstlane(threadIdx.y), first_wave = team * waves;
@@ -370,41 +370,44 @@ __global__ void __launch_bounds__(kBackwardThreads) layer_norm_backward_kernel(c
     }
     if (sums == nullptr)
         return;
-    // the teams' sums in the order of the teams, first of g * z, then of g
-    const int64_t width = static_cast<int64_t>(vectors) * kColumns;
+    // first of g * z, then of g; those of several teams in the order of the teams, four columns a thread of all of them
+    constexpr int kQuads = kColumns / 4;  // of a vector
+    const int quads = vectors * kQuads;
+    u32x4* to = sums + 2 * group * quads;
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
+    for (int which = 0; which < 2; ++which, to += quads) {
         if (which == 1 && means == nullptr)
             break;
-        auto& own = which == 0 ? sum_z : sum_g;
-        if (teams > 1) {
-            __syncthreads();
-            if (team > 0)
-#pragma unroll
-                for (int v = 0; v < kVectors; ++v) {
-                    const int at = threadIdx.x + v * blockDim.x;
-                    if (at < vectors)
-#pragma unroll
-                        for (int i = 0; i < kColumns; ++i)
-                            team_sums[(team - 1) * width + at * kColumns + i] = own[v][i];
-                }
-            __syncthreads();
-        }
-        if (team == 0)
+        const auto& own = which == 0 ? sum_z : sum_g;
+        const auto put = [&](u32x4* into) {
 #pragma unroll
             for (int v = 0; v < kVectors; ++v) {
                 const int at = threadIdx.x + v * blockDim.x;
-                if (at >= vectors)
-                    continue;
-                for (int other = 1; other < teams; ++other)
+                if (at < vectors)
 #pragma unroll
-                    for (int i = 0; i < kColumns; ++i)
-                        own[v][i] += team_sums[(other - 1) * width + at * kColumns + i];
-                float* to = sums + (2 * group + which) * width + static_cast<int64_t>(at) * kColumns;
-#pragma unroll
-                for (int i = 0; i < kColumns; i += 4)
-                    *reinterpret_cast<u32x4*>(to + i) = RowType<Fp32>::pack({own[v][i], own[v][i + 1], own[v][i + 2], own[v][i + 3]});
+                    for (int q = 0; q < kQuads; ++q)
+                        into[at * kQuads + q] = RowType<Fp32>::pack({own[v][4 * q], own[v][4 * q + 1], own[v][4 * q + 2], own[v][4 * q + 3]});
             }
+        };
+        if (teams == 1) {
+            put(to);
+            continue;
+        }
+        __syncthreads();  // (the last sums are read)
+        put(team_sums + team * quads);
+        __syncthreads();
+        for (int at = team * blockDim.x + threadIdx.x; at < quads; at += teams * blockDim.x) {
+            float sum[4], more[4];
+            RowType<Fp32>::unpack(team_sums[at], sum);
+#pragma unroll 4
+            for (int other = 1; other < teams; ++other) {
+                RowType<Fp32>::unpack(team_sums[other * quads + at], more);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    sum[i] += more[i];
+            }
+            to[at] = RowType<Fp32>::pack(sum);
+        }
     }
 }
 
@@ -533,12 +536,12 @@ int launch_backward(const BackwardPlan& plan, const void* grad, const void* tota
                     const void* grad_residual, int64_t num_tokens, int hidden, void* grad_x, void* grad_gamma, void* grad_beta, void* workspace,
                     hipStream_t stream) {
     if (plan.groups > 0) {
-        const size_t lds = grad_gamma != nullptr ? static_cast<size_t>(plan.teams - 1) * hidden * sizeof(float) : 0;
+        const size_t lds = grad_gamma != nullptr && plan.teams > 1 ? static_cast<size_t>(plan.teams) * hidden * sizeof(float) : 0;
         const dim3 grid(static_cast<unsigned>(plan.groups)), block(plan.shape.threads, plan.teams);
         const auto launch = [&](auto kernel) {
             kernel<<<grid, block, lds, stream>>>(static_cast<const u32x4*>(grad), static_cast<const u32x4*>(total),
                                                  static_cast<const u32x4*>(gamma), mean, rstd, static_cast<const u32x4*>(grad_residual),
-                                                 static_cast<u32x4*>(grad_x), grad_gamma != nullptr ? static_cast<float*>(workspace) : nullptr,
+                                                 static_cast<u32x4*>(grad_x), grad_gamma != nullptr ? static_cast<u32x4*>(workspace) : nullptr,
                                                  num_tokens, plan.groups, plan.vectors, static_cast<float>(hidden));
         };
         const auto pick = [&](auto vectors_held) {
