@@ -687,7 +687,7 @@ __device__ __forceinline__ void shares_of(const float (&logit)[kEach], bool sigm
         }
     }
     total = lanes_sum<kLanes>(total);
-    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    const float inverse = total == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(total);  // (half of the largest share at least: no tiny one)
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
         share[i] *= inverse;
@@ -842,6 +842,11 @@ __device__ __forceinline__ void load_token(const Balance& a, int64_t token, bool
     if (here && lane < a.topk)
         out.named = a.ids[token * a.topk + lane];
     load_raw<kLanes, kEach>(a.logits, token, here, a.experts, out.logit);
+}
+
+// (a count of 64 bits in three instructions: its halves are whole numbers, the larger one rounded once more where there is one)
+__device__ __forceinline__ float float_of(int64_t count) {
+    return fmaf(static_cast<float>(static_cast<uint32_t>(count >> 32)), 0x1p32f, static_cast<float>(static_cast<uint32_t>(count)));
 }
 
 __device__ __forceinline__ float workgroup_sum(float v, float* place) {
@@ -1114,11 +1119,11 @@ __global__ void __launch_bounds__(kBlockThreads) balance_loss_backward_kernel(co
         float factor[kEach], number = 0.0f;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            factor[i] = i * kLanes + lane < a.experts ? static_cast<float>(count[i]) : 0.0f;
+            factor[i] = i * kLanes + lane < a.experts ? float_of(count[i]) : 0.0f;
             number += factor[i];
         }
         number = lanes_sum<kLanes>(number);
-        const float each = live_tokens > 0 && number > 0.0f ? of_loss * static_cast<float>(a.experts) / number / static_cast<float>(live_tokens) : 0.0f;
+        const float each = live_tokens > 0 && number > 0.0f ? of_loss * static_cast<float>(a.experts) / number / float_of(live_tokens) : 0.0f;
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
             factor[i] *= each;
