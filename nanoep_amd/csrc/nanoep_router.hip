@@ -157,6 +157,8 @@ struct Route {
     int experts, topk, groups, topk_groups;
     bool sigmoid, normalize;
     float scale;
+    int group_size, group_bits;  // experts of a group; the groups' number is 2^group_bits at most
+    float per_group;             // 1 / group_size
 };
 
 // K rounds over a token's keys: the largest of all, the lowest expert that has it.  chosen_expert, chosen_key: the token's in LDS.
@@ -270,24 +272,69 @@ __device__ __forceinline__ uint32_t list_candidates(const uint32_t (&key)[kEach]
     return number;
 }
 
-// Strikes out the experts of all groups but the best ones, a group being as good as the sum of its two largest values.  The keys go
-// through LDS ([kLanes * kEach] of the token), where lanes share out every group to find the two; the groups' sums go through it too, and
-// every group counts how many are ahead of it.  Returns how far the last group that was kept is above the first that was not.
+// How good a group is, from its two largest values' keys: their sum.
+template <class Key>
+__device__ __forceinline__ Key key_of_group(Key best, Key second) {
+    return best == 0 || second == 0 ? best : key_of(value_of(best) + value_of(second));
+}
+
+// The best groups as bits; lane g has group g's key.  Every group counts how many are ahead of it.  keys: LDS of the token, a key a group.
+template <int kLanes, class Key>
+__device__ __forceinline__ uint64_t best_groups(const Route& a, Key of_group, Key* keys, bool& kept) {
+    const int lane = threadIdx.x % kLanes, groups = a.groups;
+    if (lane < groups)
+        keys[lane] = of_group;
+    wavefront_sync();
+    int ahead = 0;
+#pragma unroll 8
+    for (int other = 0; other < groups; ++other) {
+        const Key against = keys[other];
+        ahead += against > of_group || (against == of_group && other < lane) ? 1 : 0;
+    }
+    kept = lane < groups && ahead < a.topk_groups;
+    return lanes_where<kLanes>(kept && of_group != 0);
+}
+
+// A lane's experts' groups: (expert + 1/2) / (experts of a group), rounded down.  (A quotient of the middle of an expert's place is never
+// near a whole number.)
+template <int kLanes>
+struct GroupOf {
+    float per_group, first;
+    __device__ __forceinline__ explicit GroupOf(const Route& a)
+        : per_group(a.per_group), first((static_cast<float>(threadIdx.x % kLanes) + 0.5f) * per_group) {}
+    __device__ __forceinline__ uint32_t of_place(int i) const { return static_cast<uint32_t>(fmaf(static_cast<float>(i * kLanes), per_group, first)); }
+    __device__ __forceinline__ int of_expert(uint32_t expert) const { return static_cast<int>((static_cast<float>(expert) + 0.5f) * per_group); }
+};
+
+// Strikes out the experts of all groups but the open ones.
 template <int kLanes, int kEach, class Key>
-__device__ __forceinline__ auto keep_groups(Key (&key)[kEach], const Route& a, Key* keys) {
-    const int lane = threadIdx.x % kLanes, groups = a.groups, size = a.experts / groups;
+__device__ __forceinline__ void strike_out(Key (&key)[kEach], const Route& a, uint64_t open) {
+    const GroupOf<kLanes> group(a);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        if constexpr (kLanes == kWave)
+            key[i] = open >> (group.of_place(i) & 63) & 1 ? key[i] : 0;
+        else
+            key[i] &= static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(open), group.of_place(i), 1));  // (a bit, as all of a word)
+    }
+}
+
+// The best groups as bits, a group being as good as the sum of its two largest values.  The keys go through LDS ([kLanes * kEach] of the
+// token), where lanes share out every group to find the two (lane g then has the second of group g); the groups' sums go through it too.
+// margin: how far the last group that was kept is above the first that was not.
+template <int kLanes, int kEach, class Key, class Value>
+__device__ __forceinline__ uint64_t find_groups(const Key (&key)[kEach], const Route& a, Key* keys, Key& second, Value& margin) {
+    const int lane = threadIdx.x % kLanes, groups = a.groups, size = a.group_size;
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
         keys[i * kLanes + lane] = key[i];
     wavefront_sync();
-    int width = 1;  // lanes from a part of a group to the next: a power of two
-    while (width < groups)
-        width *= 2;
-    const int group = lane % width, parts = kLanes / width;
-    Key best = 0, second = 0;
+    const int width = 1 << a.group_bits, group = lane & (width - 1), parts = kLanes >> a.group_bits;  // width: from a part of a group to the next
+    Key best = 0;
+    second = 0;
     if (group < groups)
 #pragma unroll 8
-        for (int at = lane / width; at < size; at += parts) {
+        for (int at = lane >> a.group_bits; at < size; at += parts) {
             const Key other = keys[group * size + at];
             const Key lower = other < best ? other : best;
             second = lower > second ? lower : second;
@@ -300,32 +347,12 @@ __device__ __forceinline__ auto keep_groups(Key (&key)[kEach], const Route& a, K
         second = lower > higher ? lower : higher;
     }
     wavefront_sync();
-    Key of_group = 0;
-    if (lane < groups && best != 0)
-        of_group = second == 0 ? best : key_of(value_of(best) + value_of(second));
-    if (lane < groups)
-        keys[lane] = of_group;
-    wavefront_sync();
-    int ahead = 0;
-#pragma unroll 8
-    for (int other = 0; other < groups; ++other) {
-        const Key against = keys[other];
-        ahead += against > of_group || (against == of_group && other < lane) ? 1 : 0;
-    }
-    const bool kept = lane < groups && ahead < a.topk_groups;
-    const uint64_t open = lanes_where<kLanes>(kept && of_group != 0);
+    const Key of_group = lane < groups ? key_of_group(best, second) : 0;
+    bool kept;
+    const uint64_t open = best_groups<kLanes>(a, of_group, keys, kept);
     const Key last = ~largest_key<kLanes>(kept ? ~of_group : Key{0}), first_out = largest_key<kLanes>(lane < groups && !kept ? of_group : Key{0});
-    // (a quotient of the middle of an expert's place: never near a whole number)
-    const float per_group = 1.0f / static_cast<float>(size), first = (static_cast<float>(lane) + 0.5f) * per_group;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        const uint32_t of = static_cast<uint32_t>(fmaf(static_cast<float>(i * kLanes), per_group, first));
-        if constexpr (kLanes == kWave)
-            key[i] = open >> (of & 63) & 1 ? key[i] : 0;
-        else
-            key[i] &= static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(open), of, 1));  // (a bit, as all of a word)
-    }
-    return value_of(last) - value_of(first_out);
+    margin = value_of(last) - value_of(first_out);
+    return open;
 }
 
 // Weights of the choices, lane k with choice k, and both to memory.  largest, total: of the softmax over all experts, if the weights
@@ -377,8 +404,9 @@ __device__ __forceinline__ void softmax_of(const float (&logit)[kEach], float (&
 
 // Experts by their logits; kLanes neighbouring lanes a token, its experts spread over them.  With few experts a lane in K rounds; else
 // those that reach a bound that K of them reach go to a list, and each counts how many of the list are ahead of it.
-// Vector instructions and latencies, not bytes: 32768 tokens of 64 experts (12 MB) 8.7 us, of 256 experts 11.8 (K rounds 16.0; a whole
-// wavefront a token and K rounds 22.2); 4096 of 256 4.4 (480 vector instructions a wavefront of two tokens); one token 2.9, a launch.
+// Vector instructions and latencies, not bytes: 32768 tokens of 64 experts (12 MB) 6.7 us (350 vector instructions a wavefront of
+// four tokens: 90 % of its time), of 256 experts 10.4 (K rounds 16.0; a whole wavefront a token and K rounds 22.2); 4096 of 256 4.2; one
+// token 2.8, a launch.
 template <int kLanes, int kEach>
 __global__ void __launch_bounds__(kBlockThreads) route_topk_kernel(const Route a) {
     constexpr int kTokens = kBlockThreads / kLanes, kListed = 2 * kLanes;
@@ -490,8 +518,11 @@ __device__ __forceinline__ void choose_by_value(const Route& a, int64_t token, u
         const float bias = a.bias != nullptr && expert < a.experts ? a.bias[expert] : 0.0f;
         key[i] = logit[i] == -INFINITY ? 0 : key_of(value_of_expert(a, logit[i], bias, largest, total));
     }
-    if (a.groups > 1)
-        keep_groups<kWave, kEach>(key, a, keys);
+    if (a.groups > 1) {
+        uint64_t second;
+        double margin;
+        strike_out<kWave, kEach>(key, a, find_groups<kWave, kEach>(key, a, keys, second, margin));
+    }
     choose_in_turn<kWave, kEach>(key, a.topk, experts, all_chosen[threadIdx.x / kWave]);
     if (lane < a.topk && experts[lane] != kNoExpert)
         logits[lane] = load_logit(a.logits, token, experts[lane]);
@@ -503,11 +534,12 @@ constexpr int key_words(int lanes, int each) { return kWave * (lanes == kWave ? 
 
 // Experts by their values: scores plus bias, and groups.  Values in fp32, with a bound on their error, find the groups and list
 // those experts that can be among the first K; the values of the list, one or two a lane, are then computed in 64 bits, and each
-// counts how many are ahead of it.  A token whose groups fp32 cannot tell apart (one in a thousand), or whose list is too long (all values
-// equal), is done again in 64 bits throughout, by its whole wavefront.
-// 4096 tokens of 256 experts, bias, four of eight groups: 8.7 us (all values in 64 bits: 11.6), half of the time instructions (1080
-// vector instructions a wavefront of two tokens, 270 of them for the groups), half waits for LDS and memory; without groups 7.0, 32768
-// tokens 20.5; one token 6.2, without groups 4.9.
+// counts how many are ahead of it.  Groups that fp32 cannot tell apart (one token in ten thousand) are found in the same way from a list of
+// those that can be among their two largest.  A token whose list is too long (all values equal) is done again in 64 bits throughout, by
+// its whole wavefront.
+// 4096 tokens of 256 experts, bias, four of eight groups: 7.9 us (all values in 64 bits: 11.6), half of the time instructions (970 vector
+// instructions a wavefront of two tokens, 200 of them for the groups), half waits for LDS and memory; without groups 6.4, 32768
+// tokens 17; one token 5.7, without groups 4.5.  Groups in 64 bits add 2 us to a launch (with the whole wavefront's second go: 5).
 template <int kLanes, int kEach>
 __global__ void __launch_bounds__(kBlockThreads) route_values_kernel(const Route a) {
     constexpr int kTokens = kBlockThreads / kLanes, kListed = 2 * kLanes;
@@ -563,29 +595,6 @@ __global__ void __launch_bounds__(kBlockThreads) route_values_kernel(const Route
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
         key[i] = logit[i] == -INFINITY ? 0 : key_of(value[i]);
-    bool again = false;
-    if (a.groups > 1) {
-        float size = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i)
-            size = fmaxf(size, key[i] != 0 ? fabsf(value[i]) : 0.0f);
-        size = lanes_max<kLanes>(size);
-        const float margin = keep_groups<kLanes, kEach>(key, a, keys + place % (kWave / kLanes) * kLanes * kEach);
-        // Two sums of two, rounded.  Without a bias no value is off by more than the largest one is.
-        const float each = a.bias != nullptr ? off : size * (0x1.4p-22f - 0x1.8p-24f * fminf(__log2f(size), 0.0f));
-        again = !(margin > 4.0f * each + 0x1p-21f * size);
-    }
-    uint32_t bound = bound_of<kLanes, kEach>(key, a.topk, all_maxima[place]);
-    const float least = value_of(bound);
-    if (fabsf(least) < INFINITY)
-        bound = key_of(least - 2.0f * off - 4.0f * part * fabsf(least));
-    list[lane].key = list[kLanes + lane].key = 0;
-    wavefront_sync();
-    uint32_t most;
-    const uint32_t number = list_candidates<kLanes, kEach>(key, bound, kListed, most, [&](uint32_t at, int i) {
-        list[at] = {uint64_t{1} << 32 | __float_as_uint(bias[i]), static_cast<uint32_t>(i * kLanes + lane), logit[i]};
-    });
-    again = again || number > kListed;
     double wide_total = 0.0;
     if (!a.sigmoid && a.bias != nullptr) {
 #pragma unroll
@@ -593,8 +602,18 @@ __global__ void __launch_bounds__(kBlockThreads) route_values_kernel(const Route
             wide_total += exp(static_cast<double>(logit[i]) - largest);
         wide_total = lanes_sum<kLanes>(wide_total);
     }
-    if (most <= kListed) {
-        Candidate own[2] = {list[lane], list[kLanes + lane]};
+    // Candidates go to the list with their bias and logit, then those of a lane, one or two, have their values in 64 bits as keys.
+    uint32_t most, number;
+    const auto list_those = [&](const uint32_t (&of)[kEach], uint32_t from) {
+        list[lane].key = list[kLanes + lane].key = 0;
+        wavefront_sync();
+        number = list_candidates<kLanes, kEach>(of, from, kListed, most, [&](uint32_t at, int i) {
+            list[at] = {uint64_t{1} << 32 | __float_as_uint(bias[i]), static_cast<uint32_t>(i * kLanes + lane), logit[i]};
+        });
+    };
+    const auto key_of_listed = [&](Candidate (&own)[2]) {
+        own[0] = list[lane];
+        own[1] = list[kLanes + lane];
         wavefront_sync();
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
@@ -606,6 +625,63 @@ __global__ void __launch_bounds__(kBlockThreads) route_values_kernel(const Route
             }
         }
         wavefront_sync();
+    };
+    bool again = false;
+    if (a.groups > 1) {
+        uint32_t* own_keys = keys + place % (kWave / kLanes) * key_words(kLanes, kEach) / (kWave / kLanes);
+        float size = 0.0f, margin;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            size = fmaxf(size, key[i] != 0 ? fabsf(value[i]) : 0.0f);
+        size = lanes_max<kLanes>(size);
+        uint32_t second;
+        uint64_t open = find_groups<kLanes, kEach>(key, a, own_keys, second, margin);
+        // Two sums of two, rounded.  Without a bias no value is off by more than the largest one is.
+        const float each = a.bias != nullptr ? off : size * (0x1.4p-22f - 0x1.8p-24f * fminf(__log2f(size), 0.0f));
+        const float unsure = 4.0f * each + 0x1p-21f * size;
+        const bool close = !(margin > unsure) && routed;
+        if (__any(close)) {
+            // Again from values in 64 bits of all that can be among a group's two largest, two or three a group.
+            const GroupOf<kLanes> group(a);
+            const float least = value_of(second);
+            wavefront_sync();
+            if (lane < a.groups)
+                own_keys[lane] = fabsf(least) < INFINITY ? key_of(least - 0.5f * unsure) : second;
+            wavefront_sync();
+            uint32_t among[kEach];
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+                among[i] = key[i] != 0 && key[i] >= own_keys[group.of_place(i)] ? key[i] : 0;
+            list_those(among, 1);
+            if (most <= kListed) {
+                Candidate own[2];
+                key_of_listed(own);
+                uint64_t first = 0, next = 0;
+                for (uint32_t j = 0; j < number; ++j) {
+                    const Candidate other = list[j];
+                    if (group.of_expert(other.expert) == lane) {
+                        const uint64_t lower = other.key < first ? other.key : first;
+                        next = lower > next ? lower : next;
+                        first = other.key > first ? other.key : first;
+                    }
+                }
+                bool kept;
+                open = best_groups<kLanes>(a, key_of_group(first, next), reinterpret_cast<uint64_t*>(own_keys), kept);
+            } else {
+                again = close;
+            }
+        }
+        strike_out<kLanes, kEach>(key, a, open);
+    }
+    uint32_t bound = bound_of<kLanes, kEach>(key, a.topk, all_maxima[place]);
+    const float least = value_of(bound);
+    if (fabsf(least) < INFINITY)
+        bound = key_of(least - 2.0f * off - 4.0f * part * fabsf(least));
+    list_those(key, bound);
+    again = again || number > kListed;
+    if (most <= kListed) {
+        Candidate own[2];
+        key_of_listed(own);
         if (lane >= static_cast<int>(number))
             experts[lane] = kNoExpert;
         const auto choose = [&](auto listed_each) {  // one or two of the list a lane
@@ -711,7 +787,7 @@ struct RouteBackward {
 //   sigmoids                          dl_k = c g_k s_k (1 - s_k)
 // and zero for every other expert.  Only the second reads more than the chosen logits.  An expert that is named twice has both
 // gradients: its first choice adds them up, in their order.  Choices become experts' through a row in LDS.
-// 8192 tokens of 128 experts, softmax over all (9 MB) 4.2 us, 32768 of 64 (19 MB) 6.2, 1537 of 60 3.0: a launch and the bytes.
+// 8192 tokens of 128 experts, softmax over all (9 MB) 4.2 us, 32768 of 64 (19 MB) 6.0, 1537 of 60 3.0: a launch and the bytes.
 template <int kLanes, int kEach>
 __global__ void __launch_bounds__(kBlockThreads) route_topk_backward_kernel(const RouteBackward a) {
     __shared__ float2 all_choices[kBlockThreads / kLanes][kLanes];  // expert's bits, gradient
@@ -871,7 +947,7 @@ __device__ __forceinline__ float loss_of(int experts, float sum, float number, i
 // wavefront's tokens, then those of the wavefronts are added in a fixed order.  Chunk c leaves its part of sequence s in row c + s of
 // `rows` (from one to the next either c or s goes up by one), shares, then counts, as wide as the lanes' experts, for
 // balance_finish_kernel, whose count of workgroups that have arrived the first one clears.  One sequence of one chunk is finished here.
-// 32768 tokens of 64 experts (10 MB) 6.2 us, 8192 of 128 in 17 sequences 6.4: half of a wavefront's time is waiting for its offsets, then its
+// 32768 tokens of 64 experts (10 MB) 6.3 us, 8192 of 128 in 17 sequences 6.4: half of a wavefront's time is waiting for its offsets, then its
 // tokens.  (A workgroup a part of a sequence, a wavefront a token: 11.6 and 16.4.)
 template <int kLanes, int kEach>
 __global__ void __launch_bounds__(kBlockThreads) balance_loss_kernel(const Balance a, uint32_t* __restrict__ rows,  // null: finished here
@@ -976,8 +1052,8 @@ __global__ void __launch_bounds__(kBlockThreads) balance_loss_kernel(const Balan
 // A sequence's rows are added up by 2^slice_bits workgroups, each for its part of the experts: four columns a thread, neighbouring threads
 // neighbouring columns, the rows shared out among groups of threads, whose sums are then added in a fixed order.  Each leaves its part
 // of sum c_e * share_e and of C; the one that arrives last adds those up, in their order as well.  (Several slices only for one sequence:
-// rows are many then.)  A chain of latencies (offsets, rows, the slices' arrival), not of bytes: 512 rows of 64 experts 6.2 us, 17 sequences of
-// some 31 rows of 128 5.6.  Neighbouring threads on neighbouring rows instead: 9.2 and 11.2.
+// rows are many then.)  A chain of latencies (offsets, rows, the slices' arrival), not of bytes: 512 rows of 64 experts 6.3 us, 17 sequences of
+// some 31 rows of 128 5.0.  Neighbouring threads on neighbouring rows instead: 9.2 and 11.2.
 constexpr int kMostSlices = 16, kRowsAtOnce = 8, kFinishThreads = 1024;
 __global__ void __launch_bounds__(kFinishThreads) balance_finish_kernel(const Balance a, int width,  // columns of a row's half: 8 to 4096
                                                                        int slice_bits, const u32x4* __restrict__ rows,
@@ -1090,7 +1166,7 @@ __global__ void __launch_bounds__(kFinishThreads) balance_finish_kernel(const Ba
 
 // The gradient: with F_e = g E c_e / (C T') of the token's sequence, p_e (F_e - sum of F p) (times 1 - s_e for sigmoids); zero for
 // tokens without a choice and for those of no sequence.  A wavefront has a chunk of tokens, whatever sequences they are of; the next
-// tokens' inputs are on their way.  32768 tokens of 64 experts (19 MB) 7.3 us, 8192 of 128 in 17 sequences 6.9, 14681 of 211 (25 MB) 10.3.
+// tokens' inputs are on their way.  32768 tokens of 64 experts (19 MB) 7.0 us, 8192 of 128 in 17 sequences 6.6, 14681 of 211 (25 MB) 10.4.
 template <int kLanes, int kEach>
 __global__ void __launch_bounds__(kBlockThreads) balance_loss_backward_kernel(const Balance a, const float* __restrict__ grad,  // [S]
                                                                               const int64_t* __restrict__ counts, const int64_t* __restrict__ tokens,
@@ -1368,7 +1444,8 @@ int nanoep_route_topk(const void* logits, int64_t logits_stride, int logits_type
     if (logits == nullptr || ids == nullptr || weights == nullptr)
         return NANOEP_ERR_INVALID_ARGUMENT;
     const Route arguments = {logits_of(logits, logits_stride, logits_type), bias, mask, ids, weights, num_tokens, num_experts, num_topk,
-                             topk_groups < groups ? groups : 1, topk_groups, scoring == NANOEP_SIGMOID, normalize != 0, scale};
+                             topk_groups < groups ? groups : 1, topk_groups, scoring == NANOEP_SIGMOID, normalize != 0, scale,
+                             num_experts / groups, bits_of(groups), static_cast<float>(groups) / static_cast<float>(num_experts)};
     const bool by_value = bias != nullptr || arguments.groups > 1;
     const Spread spread = spread_for_choices(num_tokens, num_experts, std::max({num_topk, arguments.groups, by_value ? 16 : 1}));
     const int threads = spread.each > 16 ? kWave : kBlockThreads;  // (LDS)

@@ -414,6 +414,30 @@ def test_values_that_fp32_cannot_tell_apart(device, scoring):
 
 
 @pytest.mark.parametrize("scoring", SCORINGS)
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("groups,size", [(8, 32), (16, 1), (16, 2), (12, 5), (64, 4), (4, 200)])
+def test_groups_that_fp32_cannot_tell_apart(device, scoring, biased, groups, size):
+    """Every group's largest value is a neighbour of the others' largest, some are equal; their second ones are the same."""
+    tokens, experts = 70, groups * size
+    logits = randn(67, tokens, groups, size).clamp(max=0.5) - 2.0
+    step = torch.stack([torch.randperm(groups, generator=torch.Generator().manual_seed(t)) for t in range(tokens)])
+    step[1::3] //= 2  # equal ones
+    logits[:, :, size // 2] = 1.0 + 2.0**-23 * step
+    if size > 2:
+        logits[:, :, size - 1] = 0.75
+        logits[5] = 1.0  # all of them, more than a list holds
+        logits[6, : groups // 2] = 1.0 + 2.0**-23 * step[6, : groups // 2, None]
+        logits[7, 1:3] = -math.inf
+    logits = logits.reshape(tokens, experts)
+    bias = torch.full((experts,), 0.125) if biased else None
+    print("groups, neighbours", scoring, biased, groups, size, flush=True)
+    for kept in (1, groups // 2, groups - 1):
+        topk = min(8, kept * size)
+        check_route(device, logits, topk, scoring=scoring, bias=bias, groups=groups, topk_groups=kept)
+        check_route(device, logits[:1], topk, scoring=scoring, bias=bias, groups=groups, topk_groups=kept)
+
+
+@pytest.mark.parametrize("scoring", SCORINGS)
 @pytest.mark.parametrize("normalize", [True, False])
 @pytest.mark.parametrize("biased", [False, True])
 @pytest.mark.parametrize("experts", [6, 64, 256])
