@@ -1,7 +1,8 @@
 // MI355X (gfx950, wave64) kernels for one rank's expert-parallel dispatch / combine, and the
 // C ABI declared in include/nanoep_hip.h: nanoep_layout.hip, nanoep_dispatch.hip,
 // nanoep_combine.hip, nanoep_abi.hip.  This header holds what they share.  (The expert layer's operators around the two,
-// nanoep_norm.hip, nanoep_experts.hip and nanoep_weighted.hip, are described there and in nanoep_operators.h.)
+// nanoep_norm.hip, nanoep_experts.hip and nanoep_weighted.hip, and its entry, nanoep_layer_norm.hip and nanoep_router.hip, are described
+// there and in nanoep_operators.h.)
 //
 // Data layout in HBM (all row-major, contiguous):
 //   x, recv_x, y, out_x, bias : bf16 rows of H elements, moved as 16-byte vectors (H/8 per row)

@@ -1254,7 +1254,8 @@ Spread spread_of(int experts, int needed) {
 }
 
 // For the router's choices: a lane for each of them, and 32 while that is no more than four wavefronts a SIMD, which have little work each
-// then (us with 16, 32 and 64 lanes of 256 experts, a bias: 1 token 5.7, 4.8, 4.4; 4096 tokens 8.4, 6.9, 7.8; 32768 tokens 19.2, 22.4, 41.6).
+// then (us a call with 16, 32 and 64 lanes, 256 experts, a bias: 1 token 5.6, 5.2, 5.1; 4096 tokens 6.6, 5.9, 7.2; 8192 tokens 7.2, 7.5, 11.9;
+// 32768 tokens 16.6, 23.0, 40.3).
 Spread spread_for_choices(int64_t num_tokens, int experts, int needed) {
     return spread_of(experts, std::max(needed, num_tokens <= int64_t{32} * current_topology(current_tuning()).cus ? 32 : 1));
 }
