@@ -966,10 +966,10 @@ __global__ void __launch_bounds__(kBlockThreads) balance_loss_kernel(const Balan
         *arrived = 0;
     const int64_t end = begin + length < a.tokens ? begin + length : a.tokens;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-    for (int64_t sequence = sequences_ahead(a, begin); sequence < a.sequences; ++sequence) {
+    for (int64_t sequence = rows == nullptr ? 0 : sequences_ahead(a, begin); sequence < a.sequences; ++sequence) {
         int64_t from = begin, to = end;
         clip(a, sequence, from, to);
-        if (from >= end)
+        if (from >= end && rows != nullptr)  // (the one sequence that is finished here may have none of the tokens)
             break;
         BalanceToken<kEach> next;
         load_token<kLanes, kEach>(a, from + group, from + group < to, next);

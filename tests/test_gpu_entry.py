@@ -673,6 +673,17 @@ def test_balance_loss_of_an_even_batch_is_one(device):
         assert abs(float(got.loss) - 1.0) <= 64 * oracle.FP32 and (got.counts == tokens * 4 // experts).all() and got.tokens == tokens
 
 
+def test_balance_loss_of_one_sequence_without_tokens(device):
+    """The batch's tokens are behind it; nothing that lay in the outputs' memory stays."""
+    for tokens, experts in ((1, 1045), (3, 64), (40, 8), (500, 16), (3000, 256)):
+        logits, ids = make_balance(tokens, experts, 4, 90)
+        for offsets in ([0, 0], [0, tokens // 2], [0, 0, 0]):
+            print("balance, one sequence", tokens, experts, offsets, flush=True)
+            filled = [torch.full((size,), 77, dtype=torch.int64, device=device) for size in (1, 2, experts, 2 * experts) for _ in range(8)]
+            del filled
+            check_balance(device, logits, ids, "softmax", offsets)
+
+
 def test_balance_loss_of_nothing(device):
     empty, ids = torch.empty(0, 8, device=device), torch.empty(0, 2, dtype=torch.int64, device=device)
     got = ep.balance_loss(empty, ids)
