@@ -10,6 +10,8 @@ autograd finds their gradients.  The two `_backward` calls are those gradients, 
 
 Calls run on the caller's current stream; nothing is copied to the host.  `ValueError` for misuse of arguments, as `Buffer` has it;
 `RuntimeError` where a derivative is asked for that an operator does not have: in forward mode, or of a gradient.
+Calls can be captured into a graph, and so can autograd's backward pass, as long as no eager result of the same leaves is kept
+meanwhile: autograd would wait for its stream.
 None of this has a counterpart in the reference.
 """
 

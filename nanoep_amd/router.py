@@ -11,6 +11,8 @@ A score is a token's softmax over the experts, or the sigmoid of each logit.
 
 Calls run on the caller's current stream; nothing is copied to the host.  `ValueError` for misuse of arguments, as `Buffer` has it;
 `RuntimeError` where a derivative is asked for that an operator does not have: in forward mode, or of a gradient.
+Calls can be captured into a graph, and so can autograd's backward pass, as long as no eager result of the same leaves is kept
+meanwhile: autograd would wait for its stream.
 None of this has a counterpart in the reference, whose routing is the caller's.
 """
 

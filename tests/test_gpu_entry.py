@@ -820,6 +820,43 @@ def test_captured_entries_replay(device):
                 assert same_bits(got, value)
 
 
+def test_a_captured_step_with_its_gradients_replays(device):
+    """Autograd's own passes in a graph: captured when no eager result of the same leaves is left."""
+    x, residual, gamma, beta, logits, grad, grad_weights, offsets = make_entry(device, 121)
+    share = torch.tensor([0.5, 1.0, 2.0], device=device)
+
+    def step(*leaves):
+        x, residual, gamma, beta, logits = leaves
+        entered = ep.layer_norm(x, gamma, beta, residual=residual)
+        routing = ep.route_topk(logits, 8, scoring="sigmoid")
+        balance = ep.balance_loss(logits, routing.ids, scoring="sigmoid", sequence_offsets=offsets)
+        found = torch.autograd.grad((entered.normalized, entered.residual, routing.weights, balance.loss), leaves, (grad, grad, grad_weights, share))
+        return [*found, entered.normalized.detach(), routing.weights.detach(), balance.loss.detach()]
+
+    leaves = [tensor.clone().requires_grad_() for tensor in (x, residual, gamma, beta, logits)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(*leaves)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outputs = step(*leaves)
+    for turn in range(4):
+        print("replay of a step", turn, flush=True)
+        fresh = make_entry(device, 300 + 10 * turn)
+        with torch.no_grad():
+            for leaf, value in zip(leaves, fresh):
+                leaf.copy_(value)
+        graph.replay()
+        want = step(*(value.requires_grad_() for value in fresh[:5]))
+        torch.cuda.synchronize()
+        for got, value in zip(outputs, want):
+            assert same_bits(got, value)
+
+
 def test_entries_at_once_on_two_streams(device):
     states = [make_entry(device, seed) for seed in (121, 131)]
     want = [entry(*state) for state in states]
