@@ -244,10 +244,11 @@ __global__ void __launch_bounds__(kMostThreads) layer_norm_kernel(const u32x4* _
 // workgroup) and keeps the two sums over rows in registers; at its end it writes them, added over its teams, to its row of `sums`
 // ([workgroups][2][columns] fp32), which parameter_gradient_kernel adds up in a fixed order.  No atomics.
 // z and u stay in registers between a row's sums and its output; the next row's inputs are on their way meanwhile.
-// HBM-bound up to the sums: 4096 x 7168 with grad_residual (235 MB) 44.5 us, without the parameters' gradients 41.6 (5.6 TB/s, a library's
-// addition of two such arrays into a third 5.5); 15 MB of sums at the end and parameter_gradient_kernel's 4.9 are the rest of a call.
-// 1537 x 2816 in fp32 parameters 8.0 + 3.2 (three teams of three wavefronts instead of two 8.2, five 9.0).  A workgroup's rows next to one another: 54 a call instead of 50; two workgroups a compute
-// unit, so twice the sums: 59; fourteen wavefronts a row instead of seven: 55; two rows ahead: the same.
+// HBM-bound up to the sums: 4096 x 7168 with grad_residual (235 MB) 44.5 us, without the parameters' gradients 41.4 (5.7 TB/s; a library's
+// addition of two such arrays into a third 5.5); 15 MB of sums at the end and parameter_gradient_kernel's 4.8 are the rest of a call.
+// 1537 x 2816 with fp32 parameters 8.0 + 3.2 (three teams instead of two 8.2, five 9.0).  A workgroup's rows next to one another: 54 a call
+// instead of 50; two workgroups a compute unit, so twice the sums: 59; fourteen wavefronts a row instead of seven: 55; two teams of
+// seven: 47 instead of 44.5; two rows ahead: the same.
 template <class T, class P, int kVectors, bool kAdded, bool kInput>
 __global__ void __launch_bounds__(kBackwardThreads) layer_norm_backward_kernel(const u32x4* __restrict__ grad,   // [T][vectors]
                                                                                const u32x4* __restrict__ total,  // [T][vectors]
