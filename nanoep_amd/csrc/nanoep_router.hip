@@ -636,8 +636,9 @@ __global__ void __launch_bounds__(kBlockThreads) route_values_kernel(const Route
         size = lanes_max<kLanes>(size);
         uint32_t second;
         uint64_t open = find_groups<kLanes, kEach>(key, a, own_keys, second, margin);
-        // Two sums of two, rounded.  Without a bias no value is off by more than the largest one is.
-        const float each = a.bias != nullptr ? off : size * (0x1.4p-22f - 0x1.8p-24f * fminf(__log2f(size), 0.0f));
+        // Two sums of two, rounded.  Without a bias no value is off by more than the largest one is (where there is none but zeros, as
+        // of sigmoids below e^-89 or next to an infinite logit, nothing is known, and all are told apart in 64 bits).
+        const float each = a.bias != nullptr ? off : size * (0x1.4p-22f - 0x1.8p-24f * fminf(__log2f(fmaxf(size, 0x1p-126f)), 0.0f));
         const float unsure = 4.0f * each + 0x1p-21f * size;
         const bool close = !(margin > unsure) && routed;
         if (__any(close)) {

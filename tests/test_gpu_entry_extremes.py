@@ -1,0 +1,121 @@
+"""The router where fp32 has nothing left to tell values apart by: groups of scores that are tiny, lost, infinite or NaN.
+
+Choices go by values in 64 bits, found here one by one (a library's vectorised sigmoid may give equal logits two values).  Inputs are such that
+values which are not equal differ by far more than a last bit of 64."""
+
+import math
+
+import pytest
+import torch
+
+import entry_oracle as oracle
+import nanoep_amd as ep
+from test_gpu_entry import BF16, FP32, SCORINGS, randn, same_bits
+
+pytestmark = pytest.mark.gpu
+
+
+def values_of(logits, scoring, bias):
+    """A token's scores plus bias: a softmax's numerators where there is none, since their sum is a factor of all."""
+    top = max((v for v in logits if v == v), default=0.0)
+    top = 0.0 if top == -math.inf else top
+
+    def exp(v):
+        return v if v != v else math.inf if v > 709.0 else math.exp(v)
+
+    if scoring == "sigmoid":
+        values = [1.0 / (1.0 + exp(-v)) for v in logits]
+    else:
+        values = [exp(v - top) for v in logits]
+        if bias is not None:
+            total = sum(values) or 1.0  # (nothing but -infinity: nothing is left in any case)
+            values = [v / total for v in values]
+    return values if bias is None else [v + b for v, b in zip(values, bias)]
+
+
+def descending(value):
+    return (0, 0.0) if value != value else (1, -value)  # NaN ahead of everything
+
+
+def choose_of_token(logits, topk, scoring, bias, groups, topk_groups):
+    values = values_of(logits, scoring, bias)
+    left = [e for e, v in enumerate(values) if logits[e] != -math.inf and v != -math.inf]
+    size = len(logits) // groups
+    of_group = []
+    for g in range(groups):
+        best = sorted((values[e] for e in left if e // size == g), key=descending)[:2]
+        if best:
+            of_group.append((sum(best), g))
+    kept = {g for _, g in sorted(of_group, key=lambda entry: (descending(entry[0]), entry[1]))[:topk_groups]}
+    chosen = sorted((e for e in left if e // size in kept), key=lambda e: (descending(values[e]), e))[:topk]
+    return chosen + [-1] * (topk - len(chosen))
+
+
+def choose(logits, topk, scoring, bias, groups, topk_groups):
+    bias = None if bias is None else bias.double().tolist()
+    return torch.tensor([choose_of_token(row, topk, scoring, bias, groups, topk_groups) for row in logits.double().tolist()])
+
+
+def route(device, logits, topk, bias, **options):
+    return ep.route_topk(logits.to(device), topk, bias=None if bias is None else bias.to(device), **options)
+
+
+def check_groups(device, logits, topk, scoring, bias, groups, topk_groups, normalize=True):
+    """A batch, and each of its tokens as a call of its own: the ids of the definition, and the batch's bits."""
+    options = {"scoring": scoring, "groups": groups, "topk_groups": topk_groups, "normalize": normalize}
+    got = route(device, logits, topk, bias, **options)
+    want = choose(logits, topk, scoring, bias, groups, topk_groups)
+    wrong = (got.ids.cpu() != want).any(1).nonzero().flatten().tolist()
+    assert not wrong, [(t, got.ids[t].tolist(), want[t].tolist()) for t in wrong[:4]]
+    for t in range(min(logits.shape[0], 24)):
+        one = route(device, logits[t : t + 1], topk, bias, **options)
+        assert same_bits(one.ids[0], got.ids[t]) and same_bits(one.weights[0], got.weights[t]), t
+    return got
+
+
+def extreme(experts, dtype, seed):
+    lowest = torch.finfo(dtype).min
+    logits = randn(seed, 16, experts)
+    logits[1] = -88.0  # sigmoids at the end of fp32's range, and beyond it
+    logits[2] = -89.0
+    logits[3] = -120.0
+    logits[4] = lowest  # masked with the type's lowest value: experts like others
+    logits[5, 3:] = lowest
+    logits[6, : experts // 2] = lowest
+    logits[7] -= 90.0
+    logits[8] = -200.0 - torch.arange(experts)
+    logits[9] = 80.0 + torch.arange(experts) % 32
+    logits[10] = -math.inf
+    logits[11, 1:] = -math.inf
+    logits[12] = -95.0
+    logits[12, experts // 2 :] = -math.inf
+    logits[13] *= 30.0
+    logits[14, 5] = 1e30  # all other numerators are zero
+    return logits.to(dtype)
+
+
+@pytest.mark.parametrize("scoring", SCORINGS)
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("experts,groups,topk_groups,topk", [(16, 16, 5, 4), (64, 8, 3, 6), (60, 3, 2, 6), (256, 4, 2, 8), (256, 64, 40, 8)])
+def test_groups_of_extreme_logits(device, scoring, biased, dtype, experts, groups, topk_groups, topk):
+    print("groups, extreme", scoring, biased, dtype, experts, groups, flush=True)
+    bias = 0.01 * randn(102, experts) if biased else None
+    check_groups(device, extreme(experts, dtype, 101), topk, scoring, bias, groups, topk_groups)
+
+
+@pytest.mark.parametrize("scoring", SCORINGS)
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("experts,groups,topk_groups,topk", [(64, 8, 3, 6), (60, 3, 2, 6), (256, 4, 2, 8)])
+def test_groups_of_nan_and_infinity(device, scoring, biased, experts, groups, topk_groups, topk):
+    logits = randn(103, 8, experts)
+    logits[1, 17] = math.inf
+    logits[2, 17] = math.nan
+    logits[3] = math.nan
+    logits[4, [3, experts - 1]] = math.inf
+    logits[5, [3, experts - 1]] = math.nan
+    logits[6, 17], logits[6, 0] = math.inf, math.nan
+    bias = 0.01 * randn(104, experts) if biased else None
+    print("groups, nan", scoring, biased, experts, groups, flush=True)
+    got = check_groups(device, logits, topk, scoring, bias, groups, topk_groups)
+    assert got.weights[[0, 7]].isfinite().all()
