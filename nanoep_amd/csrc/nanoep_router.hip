@@ -575,8 +575,9 @@ __global__ void __launch_bounds__(kBlockThreads) route_values_kernel(const Route
     // What a value is off by: `off`, and `part` of itself.  A sigmoid's argument is rounded by 1.5 l 2^-24, of which s (1 - s) is left; with the
     // exponential, a sum and a reciprocal that is 5 * 2^-24 at most.  A softmax's share: 2^-17 of the largest (the sum's terms have
     // arguments that are rounded by (1 + log E) 2^-24 on average, and go through 70 additions).  The sum with the bias is rounded.
-    // Without a bias, where a softmax is compared by its numerators: parts of themselves, with arguments of up to 88.
-    float off = 0.0f, part = 0x1p-16f;
+    // Without a bias, where a softmax is compared by its numerators: parts of themselves, with arguments of up to 88, and all of
+    // those below 2^-126, where exponentials overflow and results lose their digits or are zero.
+    float off = 0x1p-126f, part = 0x1p-16f;
     if (a.sigmoid)
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
@@ -636,9 +637,9 @@ __global__ void __launch_bounds__(kBlockThreads) route_values_kernel(const Route
         size = lanes_max<kLanes>(size);
         uint32_t second;
         uint64_t open = find_groups<kLanes, kEach>(key, a, own_keys, second, margin);
-        // Two sums of two, rounded.  Without a bias no value is off by more than the largest one is (where there is none but zeros, as
-        // of sigmoids below e^-89 or next to an infinite logit, nothing is known, and all are told apart in 64 bits).
-        const float each = a.bias != nullptr ? off : size * (0x1.4p-22f - 0x1.8p-24f * fminf(__log2f(fmaxf(size, 0x1p-126f)), 0.0f));
+        // Two sums of two, rounded.  Without a bias no value is off by more than the largest one is (which may be zero, as of sigmoids
+        // below e^-89 or next to an infinite logit: all are told apart in 64 bits then).
+        const float each = a.bias != nullptr ? off : fmaf(size, 0x1.4p-22f - 0x1.8p-24f * fminf(__log2f(fmaxf(size, 0x1p-126f)), 0.0f), off);
         const float unsure = 4.0f * each + 0x1p-21f * size;
         const bool close = !(margin > unsure) && routed;
         if (__any(close)) {

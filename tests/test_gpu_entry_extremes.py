@@ -119,3 +119,31 @@ def test_groups_of_nan_and_infinity(device, scoring, biased, experts, groups, to
     print("groups, nan", scoring, biased, experts, groups, flush=True)
     got = check_groups(device, logits, topk, scoring, bias, groups, topk_groups)
     assert got.weights[[0, 7]].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_groups_of_sigmoids_that_end_within_fp32s_range(device, dtype):
+    """Two sigmoids that fp32 loses against one that it holds: at e^-88.7 their exponential overflows, from e^-87.3 on results lose digits."""
+    experts, groups = 16, 2
+    logits = torch.full((12, experts), -200.0)
+    for t, (two, one) in enumerate([(-89.0, -88.5), (-87.5, -87.0), (-88.75, -88.25), (-88.0, -87.5), (-90.0, -89.5), (-87.25, -86.75)]):
+        for group in (0, 1):  # the two are worth more, wherever they are
+            logits[2 * t + group, [8 * group + 2, 8 * group + 5]] = two
+            logits[2 * t + group, 8 * (1 - group) + 3] = one
+    print("groups, end of the range", dtype, flush=True)
+    check_groups(device, logits.to(dtype), 2, "sigmoid", None, groups, 1)
+    check_groups(device, (-86.0 - 4.0 * torch.rand(200, 64, generator=torch.Generator().manual_seed(105))).to(dtype), 6, "sigmoid", None, 8, 3)
+
+
+@pytest.mark.parametrize("scoring", SCORINGS)
+@pytest.mark.parametrize("experts,topk", [(32, 8), (256, 8), (256, 1)])
+def test_experts_whose_scores_end_within_fp32s_range(device, scoring, experts, topk):
+    """Candidates of a group whose numerators or sigmoids have few digits left, or none."""
+    generator = torch.Generator().manual_seed(106)
+    logits = -84.0 - 22.0 * torch.rand(200, experts, generator=generator)
+    if scoring == "softmax":
+        logits[:, 0] = 0.0
+        logits[100:] += 40.0  # differences are rounded
+    logits[::2, 1:] = logits[::2, 1:].clamp(max=-95.0)
+    print("experts, end of the range", scoring, experts, topk, flush=True)
+    check_groups(device, logits, topk, scoring, None, 2, 1)
