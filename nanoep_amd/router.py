@@ -93,8 +93,9 @@ def route_topk(
 
     logits: bf16 or fp32 [tokens, experts], up to 4096 experts, rows any distance apart; topk up to 32.  An expert whose logit (or
     value) is -infinity is never chosen; choices that find no expert are -1 with weight 0, and so are all choices of tokens whose
-    `mask` (bool [tokens]) is False, whose logits are not looked at.  NaN is above everything and makes the weights NaN; ids stay
-    distinct.  The weights have a gradient in the logits."""
+    `mask` (bool [tokens]) is False, whose logits are not looked at.  NaN is above everything; ids stay distinct.  A NaN makes all of its
+    token's weights NaN, and so does an infinite logit in a softmax; of sigmoids without `normalize` only the NaN's own weight is.
+    The weights have a gradient in the logits."""
     arguments = (logits, topk, _scoring(scoring), bias, mask, groups, topk_groups, normalize, scale)
     if logits.requires_grad and torch.is_grad_enabled():
         return Routing(*_Route.apply(*arguments))

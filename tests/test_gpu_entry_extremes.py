@@ -147,3 +147,31 @@ def test_experts_whose_scores_end_within_fp32s_range(device, scoring, experts, t
     logits[::2, 1:] = logits[::2, 1:].clamp(max=-95.0)
     print("experts, end of the range", scoring, experts, topk, flush=True)
     check_groups(device, logits, topk, scoring, None, 2, 1)
+
+
+@pytest.mark.parametrize("scoring", SCORINGS)
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("groups,biased", [(1, False), (1, True), (4, False), (4, True)])
+def test_weights_of_tokens_with_nan_or_infinity(device, scoring, normalize, groups, biased):
+    """All of a token's weights, but of plain sigmoids the NaN's own alone; an infinity breaks a softmax and no sigmoid."""
+    experts, topk = 64, 6
+    logits = randn(107, 5, experts)
+    logits[1, [17, 40]] = math.nan
+    logits[2, 17] = math.inf
+    logits[3, 17], logits[3, 40] = math.inf, math.nan
+    bias = 0.01 * randn(108, experts) if biased else None
+    print("weights, nan", scoring, normalize, groups, biased, flush=True)
+    got = route(device, logits, topk, bias, scoring=scoring, normalize=normalize, groups=groups, topk_groups=max(1, groups // 2))
+    ids, broken = got.ids.cpu(), got.weights.cpu().isnan()
+    expected = torch.zeros(5, topk, dtype=torch.bool)
+    if scoring == "softmax":
+        expected[1:4] = True
+    elif normalize:
+        expected[[1, 3]] = True
+    else:
+        expected = logits.gather(1, ids).isnan()
+        assert expected.sum(1).tolist() == [0, 2, 0, 1, 0]
+    assert torch.equal(broken, expected)
+    fine = ~broken.any(1)
+    weights, slack = oracle.weigh(logits[fine], ids[fine], scoring, normalize, 1.0)
+    assert ((got.weights.cpu()[fine] - weights).abs() <= slack).all()
