@@ -1,4 +1,5 @@
-"""The router where fp32 has nothing left to tell values apart by: groups of scores that are tiny, lost, infinite or NaN.
+"""The router and the balance loss at extreme logits, and groups of scores that are tiny, lost, infinite or NaN, where fp32 has nothing left
+to tell values apart by.
 
 Choices go by values in 64 bits, found here one by one (a library's vectorised sigmoid may give equal logits two values).  Inputs are such that
 values which are not equal differ by far more than a last bit of 64."""
@@ -10,7 +11,7 @@ import torch
 
 import entry_oracle as oracle
 import nanoep_amd as ep
-from test_gpu_entry import BF16, FP32, SCORINGS, randn, same_bits
+from test_gpu_entry import BF16, FP32, SCORINGS, check_balance, check_route, make_balance, randn, same_bits
 
 pytestmark = pytest.mark.gpu
 
@@ -175,3 +176,43 @@ def test_weights_of_tokens_with_nan_or_infinity(device, scoring, normalize, grou
     fine = ~broken.any(1)
     weights, slack = oracle.weigh(logits[fine], ids[fine], scoring, normalize, 1.0)
     assert ((got.weights.cpu()[fine] - weights).abs() <= slack).all()
+
+
+@pytest.fixture
+def tight(monkeypatch):
+    """The oracle's bounds for logits of any size.  What is rounded is the difference of a logit and its token's largest, by 2^-24 of itself,
+    however large the two are; and e^-110 (the largest being e^0) is zero to within LEAST, so no difference above that rounds anything."""
+
+    def spread(logits):
+        logits, finite = logits.double(), logits.isfinite()
+        top = logits.masked_fill(~finite, -math.inf).amax(1, keepdim=True)
+        return (top - logits.masked_fill(~finite, math.inf).amin(1, keepdim=True)).clamp(min=0.0, max=110.0)
+
+    monkeypatch.setattr(oracle, "_spread", spread)
+
+
+@pytest.mark.parametrize("scoring", SCORINGS)
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("experts,topk", [(16, 3), (60, 6), (256, 8)])
+def test_weights_and_gradients_of_extreme_logits(device, tight, scoring, normalize, dtype, experts, topk):
+    logits, grad = extreme(experts, dtype, 109), randn(110, 16, topk)
+    print("weights, extreme", scoring, normalize, dtype, experts, flush=True)
+    got = check_route(device, logits, topk, scoring=scoring, normalize=normalize)
+    some = [t for t in range(16) if t != 10]  # (the one has no softmax)
+    # the router's own choices, and others, some of experts that could not have been chosen
+    for ids in (got.ids.cpu()[some], torch.randint(-1, experts, (len(some), topk), generator=torch.Generator().manual_seed(111))):
+        found = ep.route_topk_backward(grad[some].to(device), logits[some].to(device), ids.to(device), scoring=scoring, normalize=normalize)
+        oracle.check_rounded(found, *oracle.weigh_backward(grad[some], logits[some], ids, scoring, normalize, 1.0), dtype)
+
+
+@pytest.mark.parametrize("scoring", SCORINGS)
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("experts,topk", [(16, 3), (60, 6), (256, 8)])
+@pytest.mark.parametrize("offsets", [None, [0, 5, 5, 30, 48]])
+def test_balance_loss_of_extreme_logits(device, tight, scoring, dtype, experts, topk, offsets):
+    logits, ids = make_balance(48, experts, topk, 112, dtype)
+    logits[::3] = extreme(experts, dtype, 113)
+    print("balance, extreme", scoring, dtype, experts, offsets, flush=True)
+    got, grad = check_balance(device, logits, ids, scoring, offsets)
+    assert got.loss.isfinite().all() and grad.isfinite().all()
