@@ -105,6 +105,27 @@ __device__ __forceinline__ T lanes_sum(T v) {
     return lanes_reduce<kLanes>(v, LanesSum{});
 }
 
+// The sum over kLanes lanes with the lanes that are farthest apart added first: whoever has added 64 values down to kLanes of them, those farthest
+// apart first as well, has the same sum for any kLanes.
+template <int kLanes, class T>
+__device__ __forceinline__ T lanes_sum_from_afar(T v) {
+    static_assert(kLanes == 8 || kLanes == 16 || kLanes == 32 || kLanes == 64, "8 to 64 lanes");
+    T a, b;
+    if constexpr (kLanes >= 64) {
+        lanes_pair<32>(v, a, b);
+        v = a + b;
+    }
+    if constexpr (kLanes >= 32) {
+        lanes_pair<16>(v, a, b);
+        v = a + b;
+    }
+    if constexpr (kLanes >= 16)
+        v += lanes_moved<0x128>(v);  // row_ror 8
+    v += lanes_moved<0x141>(v);      // row_half_mirror
+    v += lanes_moved<0x4E>(v);       // quad_perm 2 3 0 1
+    return v + lanes_moved<0xB1>(v);  // quad_perm 1 0 3 2
+}
+
 // The lanes of a group of kLanes for which `condition` holds, the group's first lane as bit 0.
 template <int kLanes>
 __device__ __forceinline__ uint64_t lanes_where(bool condition) {

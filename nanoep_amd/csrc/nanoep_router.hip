@@ -384,22 +384,36 @@ __device__ __forceinline__ void store_choices(const Route& a, int64_t token, uin
     }
 }
 
+// The sum over a token's experts of `of` their places, in an order that goes by the experts alone, so that a token has the same sum however many
+// lanes it is spread over: every 64th expert in turn, then those of the 64 sums that are farthest apart.
+template <int kLanes, int kEach, class Of>
+__device__ __forceinline__ auto experts_sum(Of of) {
+    constexpr int kHeld = kWave / kLanes < kEach ? kWave / kLanes : kEach;  // of the 64, in a lane
+    decltype(of(0)) sum[kHeld];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+        sum[i % kHeld] = i < kHeld ? of(i) : sum[i % kHeld] + of(i);
+#pragma unroll
+    for (int half = kHeld / 2; half > 0; half /= 2)
+#pragma unroll
+        for (int i = 0; i < half; ++i)
+            sum[i] += sum[i + half];
+    return lanes_sum_from_afar<kLanes>(sum[0]);
+}
+
 // The largest logit (0 where there is none), and the sum of e^(logit - largest).
 template <int kLanes, int kEach>
 __device__ __forceinline__ void softmax_of(const float (&logit)[kEach], float (&exponential)[kEach], float& largest, float& total) {
     largest = -INFINITY;
-    total = 0.0f;
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
         largest = fmaxf(largest, logit[i]);
     largest = lanes_max<kLanes>(largest);
     largest = largest == -INFINITY ? 0.0f : largest;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
+    for (int i = 0; i < kEach; ++i)
         exponential[i] = exp_below(logit[i] - largest);
-        total += exponential[i];
-    }
-    total = lanes_sum<kLanes>(total);
+    total = experts_sum<kLanes, kEach>([&](int i) { return exponential[i]; });
 }
 
 // Experts by their logits; kLanes neighbouring lanes a token, its experts spread over them.  With few experts a lane in K rounds; else
@@ -505,12 +519,8 @@ __device__ __forceinline__ void choose_by_value(const Route& a, int64_t token, u
     largest = lanes_max<kWave>(largest);
     largest = largest == -INFINITY ? 0.0f : largest;
     double total = 0.0;
-    if (!a.sigmoid && a.bias != nullptr) {
-#pragma unroll
-        for (int i = 0; i < kEach; ++i)
-            total += exp(static_cast<double>(logit[i]) - largest);
-        total = lanes_sum<kWave>(total);
-    }
+    if (!a.sigmoid && a.bias != nullptr)
+        total = experts_sum<kWave, kEach>([&](int i) { return exp(static_cast<double>(logit[i]) - largest); });
     uint64_t key[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
@@ -597,12 +607,8 @@ __global__ void __launch_bounds__(kBlockThreads) route_values_kernel(const Route
     for (int i = 0; i < kEach; ++i)
         key[i] = logit[i] == -INFINITY ? 0 : key_of(value[i]);
     double wide_total = 0.0;
-    if (!a.sigmoid && a.bias != nullptr) {
-#pragma unroll
-        for (int i = 0; i < kEach; ++i)
-            wide_total += exp(static_cast<double>(logit[i]) - largest);
-        wide_total = lanes_sum<kLanes>(wide_total);
-    }
+    if (!a.sigmoid && a.bias != nullptr)
+        wide_total = experts_sum<kLanes, kEach>([&](int i) { return exp(static_cast<double>(logit[i]) - largest); });
     // Candidates go to the list with their bias and logit, then those of a lane, one or two, have their values in 64 bits as keys.
     uint32_t most, number;
     const auto list_those = [&](const uint32_t (&of)[kEach], uint32_t from) {

@@ -216,3 +216,18 @@ def test_balance_loss_of_extreme_logits(device, tight, scoring, dtype, experts, 
     print("balance, extreme", scoring, dtype, experts, offsets, flush=True)
     got, grad = check_balance(device, logits, ids, scoring, offsets)
     assert got.loss.isfinite().all() and grad.isfinite().all()
+
+
+@pytest.mark.parametrize("scoring", SCORINGS)
+@pytest.mark.parametrize("experts,topk", [(7, 2), (16, 8), (32, 8), (60, 6), (64, 16), (100, 8), (200, 4), (256, 8), (400, 16), (512, 2)])
+def test_a_tokens_choice_is_the_same_bits_in_any_batch(device, scoring, experts, topk):
+    """Batches of fewer and of more tokens than a device has 32 lanes for."""
+    logits = (2 * randn(114, 9001, experts)).to(device)
+    bias = (0.1 * randn(115, experts)).to(device)
+    print("same bits in any batch", scoring, experts, topk, flush=True)
+    for normalize in (True, False):
+        for options in ({}, {"bias": bias}):
+            whole = ep.route_topk(logits, topk, scoring=scoring, normalize=normalize, **options)
+            for first, last in ((0, 1), (9000, 9001), (1000, 3047)):
+                part = ep.route_topk(logits[first:last], topk, scoring=scoring, normalize=normalize, **options)
+                assert same_bits(part.ids, whole.ids[first:last]) and same_bits(part.weights, whole.weights[first:last]), (normalize, list(options), first)
