@@ -115,7 +115,8 @@ class _BalanceLoss(torch.autograd.Function):
     def forward(ctx, logits, ids, scoring, sequence_offsets):
         ctx.set_materialize_grads(False)
         loss, counts, tokens = load_extension().balance_loss(logits, ids, scoring, sequence_offsets)
-        ctx.save_for_backward(logits, ids, counts, tokens, sequence_offsets)
+        # (copies: a user adds up counts in place, over ranks with a collective that autograd does not see)
+        ctx.save_for_backward(logits, ids, counts.clone(), tokens.clone(), sequence_offsets)
         ctx.mark_non_differentiable(counts, tokens)
         ctx.scoring = scoring
         return loss, counts, tokens
@@ -140,7 +141,8 @@ def balance_loss(
     ids: int64 [tokens, topk], as `route_topk` gives them; ids outside the experts are masked choices.  A token without a choice is
     padding: its logits are not looked at, its gradient is zero.  With `sequence_offsets` (int64 [sequences + 1], from 0 on, ascending)
     each sequence [offsets[s], offsets[s + 1]) has a loss, counts and tokens of its own; tokens behind the last one are none's.  A
-    sequence without a choice has the loss 0.  The loss has a gradient in the logits; the counts are taken as they are."""
+    sequence without a choice has the loss 0.  The loss has a gradient in the logits, in which the counts are constants; the result's
+    `counts` and `tokens` may be changed or reduced in place ahead of the backward pass."""
     arguments = (logits, ids, _scoring(scoring), sequence_offsets)
     if logits.requires_grad and torch.is_grad_enabled():
         return BalanceResult(*_BalanceLoss.apply(*arguments))

@@ -231,3 +231,28 @@ def test_a_tokens_choice_is_the_same_bits_in_any_batch(device, scoring, experts,
             for first, last in ((0, 1), (9000, 9001), (1000, 3047)):
                 part = ep.route_topk(logits[first:last], topk, scoring=scoring, normalize=normalize, **options)
                 assert same_bits(part.ids, whole.ids[first:last]) and same_bits(part.weights, whole.weights[first:last]), (normalize, list(options), first)
+
+
+@pytest.mark.parametrize("offsets", [None, [0, 100, 260]])
+def test_counts_may_be_reduced_ahead_of_the_backward_pass(device, offsets):
+    """In place, as a collective over ranks does it, which autograd does not see (as it does not see changes of `data`)."""
+    logits, ids = make_balance(300, 60, 6, 116)
+    logits, ids = logits.to(device).requires_grad_(), ids.to(device)
+    bounds = None if offsets is None else torch.tensor(offsets, device=device)
+    print("counts, reduced", offsets, flush=True)
+
+    def found(change):
+        balance = ep.balance_loss(logits, ids, sequence_offsets=bounds)
+        change(balance)
+        return torch.autograd.grad(balance.loss.sum(), logits)[0]
+
+    def unseen(balance):
+        balance.counts.data.add_(torch.arange(60, device=device))
+        balance.tokens.data.mul_(2)
+
+    def seen(balance):
+        balance.counts.mul_(3)
+        balance.tokens.zero_()
+
+    want = found(lambda balance: None)
+    assert same_bits(found(unseen), want) and same_bits(found(seen), want)
