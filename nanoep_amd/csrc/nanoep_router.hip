@@ -1274,124 +1274,26 @@ Spread spread_for_balance(int64_t num_tokens, int experts, int topk) {
     return spread_for_choices(num_tokens, experts, experts > 128 ? std::max(topk, 32) : topk);
 }
 
-// CALL(lanes, experts a lane) for a Spread of 8 lanes or more, and of 16 or more.
-#define NANOEP_BY_SPREAD(SPREAD, CALL)              \
-    switch ((SPREAD).lanes * 100 + (SPREAD).each) { \
-        case 801:                                   \
-            CALL(8, 1);                             \
-            break;                                  \
-        case 802:                                   \
-            CALL(8, 2);                             \
-            break;                                  \
-        case 804:                                   \
-            CALL(8, 4);                             \
-            break;                                  \
-        case 1601:                                  \
-            CALL(16, 1);                            \
-            break;                                  \
-        case 1602:                                  \
-            CALL(16, 2);                            \
-            break;                                  \
-        case 1604:                                  \
-            CALL(16, 4);                            \
-            break;                                  \
-        case 1608:                                  \
-            CALL(16, 8);                            \
-            break;                                  \
-        case 1616:                                  \
-            CALL(16, 16);                           \
-            break;                                  \
-        case 3201:                                  \
-            CALL(32, 1);                            \
-            break;                                  \
-        case 3202:                                  \
-            CALL(32, 2);                            \
-            break;                                  \
-        case 3204:                                  \
-            CALL(32, 4);                            \
-            break;                                  \
-        case 3208:                                  \
-            CALL(32, 8);                            \
-            break;                                  \
-        case 3216:                                  \
-            CALL(32, 16);                           \
-            break;                                  \
-        case 6401:                                  \
-            CALL(64, 1);                            \
-            break;                                  \
-        case 6402:                                  \
-            CALL(64, 2);                            \
-            break;                                  \
-        case 6404:                                  \
-            CALL(64, 4);                            \
-            break;                                  \
-        case 6408:                                  \
-            CALL(64, 8);                            \
-            break;                                  \
-        case 6416:                                  \
-            CALL(64, 16);                           \
-            break;                                  \
-        case 6432:                                  \
-            CALL(64, 32);                           \
-            break;                                  \
-        default:                                    \
-            CALL(64, 64);                           \
-            break;                                  \
+// CALL(lanes, experts a lane) for a Spread: those that every kernel meets, and MORE that some do: 8 lanes, for up to 32 experts that are not chosen by
+// value; 16 lanes with 16 experts each, which the loss spreads over 32; whole wavefronts for fewer than 513 experts, with more than 32 groups.
+#define NANOEP_SPREAD(LANES, EACH, CALL) \
+    case (LANES) * 100 + (EACH):         \
+        CALL(LANES, EACH);               \
+        break;
+#define NANOEP_SPREADS_OF_8(CALL) NANOEP_SPREAD(8, 1, CALL) NANOEP_SPREAD(8, 2, CALL) NANOEP_SPREAD(8, 4, CALL)
+#define NANOEP_SPREAD_16_16(CALL) NANOEP_SPREAD(16, 16, CALL)
+#define NANOEP_SPREADS_OF_MANY_GROUPS(CALL) \
+    NANOEP_SPREAD(64, 1, CALL) NANOEP_SPREAD(64, 2, CALL) NANOEP_SPREAD(64, 4, CALL) NANOEP_SPREAD(64, 8, CALL)
+#define NANOEP_BY_SPREAD(SPREAD, CALL, MORE)                                                                                          \
+    switch ((SPREAD).lanes * 100 + (SPREAD).each) {                                                                                   \
+        NANOEP_SPREAD(16, 1, CALL) NANOEP_SPREAD(16, 2, CALL) NANOEP_SPREAD(16, 4, CALL) NANOEP_SPREAD(16, 8, CALL)                    \
+        NANOEP_SPREAD(32, 1, CALL) NANOEP_SPREAD(32, 2, CALL) NANOEP_SPREAD(32, 4, CALL) NANOEP_SPREAD(32, 8, CALL)                    \
+        NANOEP_SPREAD(32, 16, CALL) NANOEP_SPREAD(64, 16, CALL) NANOEP_SPREAD(64, 32, CALL) NANOEP_SPREAD(64, 64, CALL)                \
+        MORE                                                                                                                          \
+        default:                                                                                                                      \
+            return NANOEP_ERR_INVALID_ARGUMENT;                                                                                       \
     }
-#define NANOEP_BY_SPREAD_FROM_16(SPREAD, CALL)      \
-    switch ((SPREAD).lanes * 100 + (SPREAD).each) { \
-        case 1601:                                  \
-            CALL(16, 1);                            \
-            break;                                  \
-        case 1602:                                  \
-            CALL(16, 2);                            \
-            break;                                  \
-        case 1604:                                  \
-            CALL(16, 4);                            \
-            break;                                  \
-        case 1608:                                  \
-            CALL(16, 8);                            \
-            break;                                  \
-        case 1616:                                  \
-            CALL(16, 16);                           \
-            break;                                  \
-        case 3201:                                  \
-            CALL(32, 1);                            \
-            break;                                  \
-        case 3202:                                  \
-            CALL(32, 2);                            \
-            break;                                  \
-        case 3204:                                  \
-            CALL(32, 4);                            \
-            break;                                  \
-        case 3208:                                  \
-            CALL(32, 8);                            \
-            break;                                  \
-        case 3216:                                  \
-            CALL(32, 16);                           \
-            break;                                  \
-        case 6401:                                  \
-            CALL(64, 1);                            \
-            break;                                  \
-        case 6402:                                  \
-            CALL(64, 2);                            \
-            break;                                  \
-        case 6404:                                  \
-            CALL(64, 4);                            \
-            break;                                  \
-        case 6408:                                  \
-            CALL(64, 8);                            \
-            break;                                  \
-        case 6416:                                  \
-            CALL(64, 16);                           \
-            break;                                  \
-        case 6432:                                  \
-            CALL(64, 32);                           \
-            break;                                  \
-        default:                                    \
-            CALL(64, 64);                           \
-            break;                                  \
-    }
+
 bool router_sizes_fit(int64_t stride, int logits_type, int64_t num_tokens, int experts, int topk, int scoring) {
     return num_tokens >= 0 && num_tokens <= 0x7fffffff / kMaxTopk && experts >= 1 && experts <= kMostExperts && topk >= 1 && topk <= kMaxTopk &&
            stride >= experts && stride <= int64_t{1} << 31 && (logits_type == NANOEP_BF16 || logits_type == NANOEP_FP32) &&
@@ -1465,9 +1367,9 @@ int nanoep_route_topk(const void* logits, int64_t logits_stride, int logits_type
 #define NANOEP_LAUNCH_ROUTE(LANES, EACH) route_topk_kernel<LANES, EACH><<<grid, threads, 0, on>>>(arguments)
 #define NANOEP_LAUNCH_VALUES(LANES, EACH) route_values_kernel<LANES, EACH><<<grid, threads, lds, on>>>(arguments)
     if (by_value)
-        NANOEP_BY_SPREAD_FROM_16(spread, NANOEP_LAUNCH_VALUES)
+        NANOEP_BY_SPREAD(spread, NANOEP_LAUNCH_VALUES, NANOEP_SPREAD_16_16(NANOEP_LAUNCH_VALUES) NANOEP_SPREADS_OF_MANY_GROUPS(NANOEP_LAUNCH_VALUES))
     else
-        NANOEP_BY_SPREAD(spread, NANOEP_LAUNCH_ROUTE)
+        NANOEP_BY_SPREAD(spread, NANOEP_LAUNCH_ROUTE, NANOEP_SPREADS_OF_8(NANOEP_LAUNCH_ROUTE) NANOEP_SPREAD_16_16(NANOEP_LAUNCH_ROUTE))
 #undef NANOEP_LAUNCH_ROUTE
 #undef NANOEP_LAUNCH_VALUES
     NANOEP_HIP_TRY(hipGetLastError());
@@ -1493,7 +1395,7 @@ int nanoep_route_topk_backward(const float* grad, const void* logits, int64_t lo
     const dim3 grid = grid_of((num_tokens + tokens - 1) / tokens);
     const auto on = static_cast<hipStream_t>(stream);
 #define NANOEP_LAUNCH_ROUTE_BACKWARD(LANES, EACH) route_topk_backward_kernel<LANES, EACH><<<grid, threads, lds, on>>>(arguments)
-    NANOEP_BY_SPREAD(spread, NANOEP_LAUNCH_ROUTE_BACKWARD)
+    NANOEP_BY_SPREAD(spread, NANOEP_LAUNCH_ROUTE_BACKWARD, NANOEP_SPREADS_OF_8(NANOEP_LAUNCH_ROUTE_BACKWARD) NANOEP_SPREAD_16_16(NANOEP_LAUNCH_ROUTE_BACKWARD))
 #undef NANOEP_LAUNCH_ROUTE_BACKWARD
     NANOEP_HIP_TRY(hipGetLastError());
     return NANOEP_OK;
@@ -1536,7 +1438,7 @@ int nanoep_balance_loss(const void* logits, int64_t logits_stride, int logits_ty
     if (plan.chunks > 0) {
 #define NANOEP_LAUNCH_BALANCE(LANES, EACH)                                                                                                   \
     balance_loss_kernel<LANES, EACH><<<grid_of(plan.chunks), kBlockThreads, 0, on>>>(arguments, rows, live_of_rows, arrived, loss, counts, tokens)
-        NANOEP_BY_SPREAD(plan.spread, NANOEP_LAUNCH_BALANCE)
+        NANOEP_BY_SPREAD(plan.spread, NANOEP_LAUNCH_BALANCE, NANOEP_SPREADS_OF_8(NANOEP_LAUNCH_BALANCE))
 #undef NANOEP_LAUNCH_BALANCE
         NANOEP_HIP_TRY(hipGetLastError());
     }
@@ -1572,7 +1474,7 @@ int nanoep_balance_loss_backward(const float* grad, const void* logits, int64_t 
     const auto on = static_cast<hipStream_t>(stream);
 #define NANOEP_LAUNCH_BALANCE_BACKWARD(LANES, EACH) \
     balance_loss_backward_kernel<LANES, EACH><<<grid_of(blocks), kBlockThreads, 0, on>>>(arguments, grad, counts, tokens, grad_logits)
-    NANOEP_BY_SPREAD(spread, NANOEP_LAUNCH_BALANCE_BACKWARD)
+    NANOEP_BY_SPREAD(spread, NANOEP_LAUNCH_BALANCE_BACKWARD, NANOEP_SPREADS_OF_8(NANOEP_LAUNCH_BALANCE_BACKWARD))
 #undef NANOEP_LAUNCH_BALANCE_BACKWARD
     NANOEP_HIP_TRY(hipGetLastError());
     return NANOEP_OK;

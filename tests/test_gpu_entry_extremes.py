@@ -256,3 +256,37 @@ def test_counts_may_be_reduced_ahead_of_the_backward_pass(device, offsets):
 
     want = found(lambda balance: None)
     assert same_bits(found(unseen), want) and same_bits(found(seen), want)
+
+
+@pytest.mark.parametrize("experts", [1, 8, 9, 16, 17, 32, 33, 64, 65, 128, 129, 256, 257, 512, 513, 1024, 1025, 2048, 2049, 4096])
+def test_every_spread_of_experts_over_lanes(device, experts):
+    """Both sides of every size at which a token takes more lanes or a lane more experts, in short and in long batches.
+
+    Bounds, relative to sums of positive terms: a sigmoid's derivative has two exponentials and six roundings, 20 * 2^-22 with the topk
+    additions' shares; shares are off by 2 (20 * 2^-24 + 2^-22) + 104 * 2^-24 < 1e-5, the losses' products of up to three such by less than 1e-4."""
+    logits = randn(117, 8300, experts).to(device)
+    for topk in (1, 8, 9, 16, 17, 32):
+        print("spreads", experts, topk, flush=True)
+        for tokens in (3, 8300):
+            part, some = logits[:tokens], min(topk, experts)
+            want = part.sort(dim=1, descending=True, stable=True).indices[:, :some]
+            got = ep.route_topk(part, some)
+            assert torch.equal(got.ids, want)
+            assert torch.equal(ep.route_topk(part, some, scoring="sigmoid", bias=torch.zeros(experts, device=device)).ids, want)
+            for groups in (2, 33, 64):
+                if experts % groups == 0 and some <= experts - experts // groups:
+                    within = ep.route_topk(part, some, scoring="sigmoid", groups=groups, topk_groups=groups - 1).ids
+                    assert torch.equal(within[:3].cpu(), choose(part[:3].cpu(), some, "sigmoid", None, groups, groups - 1))
+            ids = torch.randint(0, experts, (tokens, topk), device=device, generator=torch.Generator(device).manual_seed(118))
+            grad = ep.route_topk_backward(torch.ones(tokens, topk, device=device), part, ids, scoring="sigmoid", normalize=False)
+            sigmoids = torch.sigmoid(part.double())
+            want = torch.zeros_like(sigmoids).scatter_add_(1, ids, torch.ones(tokens, topk, device=device, dtype=torch.float64)) * sigmoids * (1 - sigmoids)
+            assert ((grad - want).abs() <= topk * 20 * oracle.EXP * want + oracle.LEAST).all()
+            balance = ep.balance_loss(part, ids)
+            assert torch.equal(balance.counts, torch.bincount(ids.view(-1), minlength=experts)) and int(balance.tokens) == tokens
+            loss_grad = ep.balance_loss_backward(torch.ones((), device=device), part, ids, balance.counts, balance.tokens)
+            p = torch.softmax(part.double(), dim=1)
+            f = experts * balance.counts.double() / (tokens * topk) / tokens
+            want = p * (f - (p * f).sum(1, keepdim=True))
+            assert ((loss_grad - want).abs() <= 1e-4 * p * f.max() + oracle.LEAST).all()
+            assert abs(float(balance.loss) - float((f * p).sum())) <= 1e-4 * float(balance.loss)
