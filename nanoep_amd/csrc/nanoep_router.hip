@@ -547,7 +547,7 @@ constexpr int key_words(int lanes, int each) { return kWave * (lanes == kWave ? 
 // counts how many are ahead of it.  Groups that fp32 cannot tell apart (one token in ten thousand) are found in the same way from a list of
 // those that can be among their two largest.  A token whose list is too long (all values equal) is done again in 64 bits throughout, by
 // its whole wavefront.
-// 4096 tokens of 256 experts, bias, four of eight groups: 7.9 us (all values in 64 bits: 11.6), half of the time instructions (970 vector
+// 4096 tokens of 256 experts, bias, four of eight groups: 7.9 us (all values in 64 bits: 11.6), half of the time instructions (980 vector
 // instructions a wavefront of two tokens, 200 of them for the groups), half waits for LDS and memory; without groups 6.4, 32768
 // tokens 17; one token 5.7, without groups 4.5.  Groups in 64 bits add 2 us to a launch (with the whole wavefront's second go: 5).
 template <int kLanes, int kEach>

@@ -89,7 +89,7 @@ def route_topk(
     An expert's value is its logit, the order of its score; with `bias` (float32 [experts]) or groups it is its score, plus the bias,
     in 64 bits, so that neither the order of a sum nor an exponential's last bit decides.  The bias is in no weight and has no
     gradient.  With `topk_groups` < `groups`, the experts fall into groups of neighbours, a group is as good as the sum of its two
-    largest values, and only the `topk_groups` best groups are chosen from.
+    largest values (also without a bias), and only the `topk_groups` best groups are chosen from.
 
     logits: bf16 or fp32 [tokens, experts], up to 4096 experts, rows any distance apart; topk up to 32.  An expert whose logit (or
     value) is -infinity is never chosen; choices that find no expert are -1 with weight 0, and so are all choices of tokens whose
