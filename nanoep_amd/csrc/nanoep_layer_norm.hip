@@ -94,8 +94,7 @@ __device__ __forceinline__ float2 of_wavefront(const float2* places, int waves) 
 // mean = sum n_w m_w / H, squares = sum (squares_w + n_w (m_w - mean)^2), as good as squares about the row's mean.
 // kPastCache: the call's rows do not fit the last-level cache; then loads are the nontemporal ones, else the stores.
 // HBM-bound: 4096 x 7168 with a residual (235 MB) 38 to 40 us, 6 TB/s, 8192 x 2048 (134 MB) 21.2; fp32, 4096 x 4096 (268 MB) 42.8; one token 3.2, a
-// launch.  (A
-// workgroup a row, two barriers, the parameters from L2 for every row: 43.8.)
+// launch.  (A workgroup a row, two barriers, the parameters from L2 for every row: 43.8.)
 template <class T, class P, int kVectors, bool kPastCache>
 __global__ void __launch_bounds__(kMostThreads) layer_norm_kernel(const u32x4* __restrict__ x,         // [T][vectors]
                                                                   const u32x4* __restrict__ residual,  // [T][vectors] or null
@@ -248,9 +247,8 @@ __global__ void __launch_bounds__(kMostThreads) layer_norm_kernel(const u32x4* _
 // HBM-bound up to the sums: 4096 x 7168 with grad_residual (235 MB) 45.0 us, without the parameters' gradients 41.1 (5.7 TB/s; a library's
 // addition of two such arrays into a third 5.5); 15 MB of sums at the end and parameter_gradient_kernel's 4.8 are the rest of a call.
 // fp32 rows, 4096 x 4096 (268 MB) 48.1.  1537 x 2816 with fp32 parameters 8.2 + 3.2 (on a box where it was 8.0: three teams instead of two 8.2,
-// five 9.0).  A workgroup's rows next to one another: 54 a call
-// instead of 50; two workgroups a compute unit, so twice the sums: 59; fourteen wavefronts a row instead of seven: 55; two teams of
-// seven: 47 instead of 45; two rows ahead: the same.
+// five 9.0).  A workgroup's rows next to one another: 54 a call instead of 50; two workgroups a compute unit, so twice the sums: 59; fourteen
+// wavefronts a row instead of seven: 55; two teams of seven: 47 instead of 45; two rows ahead: the same.
 template <class T, class P, int kVectors, bool kAdded, bool kInput>
 __global__ void __launch_bounds__(kBackwardThreads) layer_norm_backward_kernel(const u32x4* __restrict__ grad,   // [T][vectors]
                                                                                const u32x4* __restrict__ total,  // [T][vectors]
